@@ -103,6 +103,26 @@ void decode_swiglu(torch::Tensor acc, torch::Tensor a, bool pdl);
 void gemm_decode(torch::Tensor x, torch::Tensor w, torch::Tensor acc, torch::Tensor err, bool pdl);
 }  // namespace libra
 
+namespace libra {
+namespace vocab {
+void control_logits(torch::Tensor logits, c10::optional<torch::Tensor> history,
+                    c10::optional<torch::Tensor> history_rows, c10::optional<torch::Tensor> history_lens,
+                    c10::optional<torch::Tensor> prompt_lens, c10::optional<torch::Tensor> repetition,
+                    c10::optional<torch::Tensor> presence, c10::optional<torch::Tensor> frequency,
+                    c10::optional<torch::Tensor> bias_offsets, c10::optional<torch::Tensor> bias_ids,
+                    c10::optional<torch::Tensor> bias_values, c10::optional<torch::Tensor> mask,
+                    c10::optional<torch::Tensor> mask_rows, torch::Tensor out, torch::Tensor err);
+std::vector<torch::Tensor> top_logprobs(torch::Tensor logits, int64_t k, c10::optional<torch::Tensor> temps,
+                                        double temperature);
+std::vector<torch::Tensor> distill_fwd(torch::Tensor logits, torch::Tensor ids, torch::Tensor lps, int64_t div,
+                                       double beta, bool drop, double T, c10::optional<torch::Tensor> targets,
+                                       torch::Tensor err);
+void distill_bwd(torch::Tensor logits, torch::Tensor out, double T, c10::optional<torch::Tensor> targets,
+                 torch::Tensor stats, torch::Tensor clean, torch::Tensor dk, torch::Tensor qk,
+                 c10::optional<torch::Tensor> g, c10::optional<torch::Tensor> g_lp);
+}  // namespace vocab
+}  // namespace libra
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_attention", &libra::decode_attention,
         "paged decode attention, stream-K over KV blocks with an in-kernel merge (no allocation)", py::arg("q"),
@@ -159,6 +179,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("pdl") = false);
   m.def("sample_tokens_filtered", &libra::rollout::sample_tokens_filtered,
         "top-k / top-p (nucleus) temperature sampling by radix-selected thresholds + Gumbel-max, with logprobs");
+  m.def("control_logits", &libra::vocab::control_logits,
+        "repetition / presence / frequency penalties, biases and grammar masks on rows of logits");
+  m.def("top_logprobs", &libra::vocab::top_logprobs, "k largest logits of every row with their logprobs");
+  m.def("distill_fwd", &libra::vocab::distill_fwd, "distillation loss from a teacher's top logprobs");
+  m.def("distill_bwd", &libra::vocab::distill_bwd, "gradient of distill_fwd with respect to the logits");
   m.def("flash_fwd", &libra::attn::flash_fwd, "tcgen05 varlen GQA attention forward", py::arg("q"), py::arg("k"),
         py::arg("v"), py::arg("cu_seqlens"), py::arg("tiles"), py::arg("scale"), py::arg("causal"), py::arg("err"),
         py::arg("cu_k") = py::none());

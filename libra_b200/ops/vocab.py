@@ -1,0 +1,206 @@
+"""Operators on rows of vocabulary logits: what a sampler needs before it
+(penalties, biases, grammar masks), what it reports beside the token (top
+logprobs), and the distillation loss that trains on such a report.
+
+They dispatch like the other operators of :mod:`libra_b200.ops`: CUDA tensors
+run the kernels of ``logit_controls.cu``, ``top_logprobs.cu`` and
+``distill.cu``; CPU tensors run :mod:`libra_b200.ops.reference`.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import reference as ref
+
+MAX_TOP = 256  # slots of a teacher's table, and the largest k of top_logprobs
+
+DIVERGENCES = {"forward": 0, "reverse": 1, "js": 2}
+TAILS = ("bucket", "drop")
+
+
+def _rows(logits: torch.Tensor, op: str) -> torch.Tensor:
+    if logits.dim() != 2:
+        raise ValueError(f"{op}: logits must be [rows, vocabulary], got {tuple(logits.shape)}")
+    if logits.is_cuda and logits.stride(1) != 1 and logits.shape[1] > 1:
+        return logits.contiguous()
+    return logits
+
+
+def control_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None,
+                   history_lens: Optional[torch.Tensor] = None, prompt_lens: Optional[torch.Tensor] = None,
+                   history_rows: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
+                   presence: Optional[torch.Tensor] = None, frequency: Optional[torch.Tensor] = None,
+                   bias_offsets: Optional[torch.Tensor] = None, bias_ids: Optional[torch.Tensor] = None,
+                   bias_values: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                   mask_rows: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Penalties, biases and grammar masks on logits [B, V] (bf16 or fp32).
+
+    * ``history`` int32 [H, L] holds token lists; batch row b reads row
+      ``history_rows[b]`` (int32; row b without it), its first
+      ``history_lens[b]`` tokens, of which the first ``prompt_lens[b]`` (0
+      without it) are the prompt.  Tokens outside the vocabulary are ignored.
+    * ``repetition`` fp32 [B] (> 0): a positive logit of a token in the history
+      is divided by it, any other multiplied.  ``frequency`` fp32 [B] is
+      subtracted once per occurrence behind the prompt and ``presence`` fp32
+      [B] once if there is one.
+    * row b's biases are the entries ``bias_offsets[b]`` to
+      ``bias_offsets[b + 1]`` (int32 [B + 1]) of ``bias_ids`` int32 /
+      ``bias_values`` fp32; a token listed twice gets the sum.  Made for
+      hundreds of entries a row; a ban of most tokens is a mask.
+    * ``mask`` int32 [M, >= ceil(V / 32)]: bit v % 32 of word v // 32 allows
+      token v.  Batch row b reads row ``mask_rows[b]`` (int32; row b without
+      it); a negative row number leaves the row unmasked.  Other tokens become
+      -inf, whatever their logit was; a row may end up with nothing else.
+
+    They apply in this order, in fp32, with one rounding to ``out`` (fp32
+    unless given; it may be ``logits`` itself).  Row numbers, lengths and
+    offsets that point outside their tables are not followed: they set the
+    error word that ``check_kernel_errors`` raises.
+    """
+    logits = _rows(logits, "control_logits")
+    if history is None and (history_lens is not None or history_rows is not None or prompt_lens is not None):
+        raise ValueError("control_logits: history lengths or rows without a history")
+    if mask is None and mask_rows is not None:
+        raise ValueError("control_logits: mask rows without a mask")
+    if (bias_offsets is None) != (bias_ids is None) or (bias_offsets is None) != (bias_values is None):
+        raise ValueError("control_logits: biases need offsets, ids and values")
+    if history is not None and history_lens is None:
+        raise ValueError("control_logits: history needs history_lens")
+    if logits.device.type != "cuda":
+        res = ref.control_logits(logits, history, history_lens, prompt_lens, history_rows, repetition, presence,
+                                 frequency, bias_offsets, bias_ids, bias_values, mask, mask_rows)
+        return res if out is None else out.copy_(res)
+    from . import error_flag, ext
+
+    if out is None:
+        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+    ext().control_logits(logits, history, history_rows, history_lens, prompt_lens, repetition, presence, frequency,
+                         bias_offsets, bias_ids, bias_values, mask, mask_rows, out, error_flag(logits.device))
+    return out
+
+
+def top_logprobs(logits: torch.Tensor, k: int, temperature: Union[float, torch.Tensor] = 1.0
+                 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The ``k`` (1 to 256) largest logits of every row [N, V], in descending
+    order with ties at the lowest index first: token ids int64 [N, k], their
+    logprobs under softmax(logits / temperature) fp32 [N, k] and the row's
+    log-sum-exp fp32 [N].  ``temperature``: a number or fp32 [N]; what is not
+    above 0 counts as 1.  A row of nothing but -inf has logprobs and
+    log-sum-exp of -inf; NaN ranks above +inf and makes the row's logprobs NaN."""
+    logits = _rows(logits, "top_logprobs")
+    k = int(k)
+    if not 1 <= k <= min(MAX_TOP, logits.shape[1]):
+        raise ValueError(f"top_logprobs: k must lie in [1, {min(MAX_TOP, logits.shape[1])}], got {k}")
+    per_row = isinstance(temperature, torch.Tensor)
+    if logits.device.type != "cuda":
+        return ref.top_logprobs(logits, k, temperature)
+    from . import ext
+
+    return tuple(ext().top_logprobs(logits.detach(), k, temperature if per_row else None,
+                                    1.0 if per_row else float(temperature)))
+
+
+def _check_distill(op: str, logits, ids, lps, divergence, beta, tail, temperature) -> None:
+    if divergence not in DIVERGENCES:
+        raise ValueError(f"{op}: divergence must be one of {sorted(DIVERGENCES)}, got {divergence!r}")
+    if tail not in TAILS:
+        raise ValueError(f"{op}: tail must be one of {TAILS}, got {tail!r}")
+    if tail == "drop" and divergence == "reverse":
+        raise ValueError(f"{op}: the reverse divergence needs the rest bucket (it is infinite without one)")
+    if divergence == "js" and not 0.0 < beta < 1.0:
+        raise ValueError(f"{op}: beta must lie between 0 and 1, got {beta}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"{op}: temperature must be above 0, got {temperature}")
+    if ids.dim() != 2 or ids.shape != lps.shape or ids.shape[0] != logits.shape[0]:
+        raise ValueError(f"{op}: teacher_ids and teacher_logprobs must be [rows, K], got {tuple(ids.shape)} and "
+                         f"{tuple(lps.shape)} for {logits.shape[0]} rows")
+    if not 1 <= ids.shape[1] <= MAX_TOP:
+        raise ValueError(f"{op}: 1 to {MAX_TOP} teacher tokens a row, got {ids.shape[1]}")
+
+
+class _DistillLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, lps, div, beta, drop, temperature, targets):
+        from . import error_flag, ext
+
+        loss, logp, stats, clean, dk, qk = ext().distill_fwd(logits, ids, lps, div, beta, drop, temperature, targets,
+                                                             error_flag(logits.device))
+        ctx.save_for_backward(logits, targets, stats, clean, dk, qk)
+        ctx.temperature = temperature
+        ctx.set_materialize_grads(False)
+        return loss, (logp if targets is not None else None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, g_lp):
+        from . import ext
+
+        logits, targets, stats, clean, dk, qk = ctx.saved_tensors
+        if g is None and g_lp is None:
+            return (None,) * 8
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        g = torch.zeros(logits.shape[0], device=logits.device) if g is None else g.contiguous()
+        ext().distill_bwd(logits, grad, ctx.temperature, targets, stats, clean, dk, qk, g,
+                          None if g_lp is None else g_lp.contiguous())
+        return (grad,) + (None,) * 7
+
+
+def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, *,
+                 divergence: str = "forward", beta: float = 0.5, tail: str = "bucket", temperature: float = 1.0,
+                 targets: Optional[torch.Tensor] = None):
+    """Divergence of student rows [N, V] (bf16 or fp32) from a teacher's top
+    logprobs, fp32 [N], differentiable with respect to the logits.
+
+    ``teacher_ids`` int64 / ``teacher_logprobs`` fp32 [N, K] (``top_logprobs``
+    of the teacher; K up to 256).  A slot whose id lies outside the vocabulary
+    or whose logprob is -inf or NaN is empty, and so is a token's second slot;
+    a row of empty slots has loss 0 and gradient 0, and so has a row of
+    nothing but -inf logits.  ``divergence``: "forward" KL(teacher | student),
+    "reverse" KL(student | teacher), or "js", beta KL(teacher | m) + (1 - beta)
+    KL(student | m) with m = beta teacher + (1 - beta) student.  ``tail``:
+    "bucket" compares the listed tokens and one bucket for all others (the
+    teacher's mass there is at least 2^-24); "drop" divides the teacher's
+    probabilities by their sum.  The student is softmax(logits / temperature).
+
+    With ``targets`` int64 [N] the result is (loss, logprob of the targets),
+    both from the same pass and both differentiable."""
+    logits = _rows(logits, "distill_loss")
+    _check_distill("distill_loss", logits, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature)
+    if logits.device.type != "cuda":
+        loss, logp = ref.distill_loss(logits, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature,
+                                      targets)
+    else:
+        loss, logp = _DistillLoss.apply(logits, teacher_ids.contiguous(), teacher_logprobs.contiguous(),
+                                        DIVERGENCES[divergence], float(beta), tail == "drop", float(temperature),
+                                        None if targets is None else targets.contiguous())
+    return loss if targets is None else (loss, logp)
+
+
+@torch.no_grad()
+def distill_loss_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, *,
+                      divergence: str = "forward", beta: float = 0.5, tail: str = "bucket", temperature: float = 1.0,
+                      out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``distill_loss`` and its gradient with respect to every row's logits for
+    an upstream gradient of one: (loss fp32 [N], gradient [N, V] of the
+    logits' type).  ``out``: where the gradient goes; it may be ``logits``."""
+    logits = _rows(logits, "distill_loss_grad")
+    _check_distill("distill_loss_grad", logits, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature)
+    if logits.device.type != "cuda":
+        with torch.enable_grad():
+            z = logits.detach().clone().requires_grad_(True)
+            loss, _ = ref.distill_loss(z, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature, None)
+            (grad,) = torch.autograd.grad(loss.sum(), z)
+        return loss.detach(), grad if out is None else out.copy_(grad)
+    from . import error_flag, ext
+
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    loss, _, stats, clean, dk, qk = ext().distill_fwd(logits, teacher_ids.contiguous(), teacher_logprobs.contiguous(),
+                                                      DIVERGENCES[divergence], float(beta), tail == "drop",
+                                                      float(temperature), None, error_flag(logits.device))
+    ext().distill_bwd(logits, out, float(temperature), None, stats, clean, dk, qk, None, None)
+    return loss, out
