@@ -24,7 +24,7 @@
 namespace libra {
 namespace vocab {
 
-constexpr int kDistThreads = 512;
+constexpr int kDistThreads = 256;
 constexpr int kDistMax = 256;  // slots of a teacher's table
 constexpr double kRestFloor = 5.9604644775390625e-08;  // 2^-24, what fp32 logprobs leave open near a sum of one
 
@@ -56,130 +56,188 @@ struct DistArgs {
 
 struct DistShared {
   MaxSum red[kDistThreads / 32];
-  double sum[kDistThreads / 32];
+  MaxSum part;  // this CTA's unlisted (m, s)
+  int twice;    // one of this CTA's tokens is listed twice
   int ids[kDistMax];
+  double e[kDistMax], p[kDistMax], h[kDistMax];
 };
 
-// Sum over the block in a fixed order; every thread gets it.
-__device__ __forceinline__ double block_sum(double v, double* sh) {
+__device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  double s = 0.0;
-  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) s += sh[w];
-  __syncthreads();
-  return s;
+  return v;
 }
 
-// The slots of a row that count: a token inside the vocabulary, a logprob above -inf, the first occurrence of its
-// token.  Sets their bits (bit of token j: j - head + 8) and returns this thread's token or -1.
-__device__ __forceinline__ int row_slots(const DistArgs& a, int row, int V, int head, uint32_t* bits, DistShared& sh,
-                                         float& lp) {
+// Reads the row's slots and sets, in the bitmap of this CTA's slice, the bits of its tokens: bit of token j is
+// j - head - 8 o0 + 8.  A slot counts if its token is inside the vocabulary and its logprob above -inf; second
+// occurrences of a token are only noticed here (`twice`), since they are rare.
+__device__ __forceinline__ void row_slots(const DistArgs& a, int row, int V, const RowSpan& sp, const Slice& sl,
+                                          uint32_t* bits, DistShared& sh) {
+  const int words = (sl.o1 - sl.o0 + 2 + 3) >> 2;
+  for (int i = threadIdx.x; i < words; i += kDistThreads) bits[i] = 0u;
+  if (threadIdx.x == 0) sh.twice = 0;
   const int k = threadIdx.x;
   int id = -1;
-  lp = 0.f;
   if (k < a.K) {
     const int64_t t = a.ids[(int64_t)row * a.K + k];
-    lp = a.lps[(int64_t)row * a.K + k];
-    if (t >= 0 && t < V && lp > -INFINITY) id = (int)t;
+    if (t >= 0 && t < V && a.lps[(int64_t)row * a.K + k] > -INFINITY) id = (int)t;
     sh.ids[k] = id;
   }
-  bool twice = false;
+  __syncthreads();
   if (id >= 0) {
-    const int bit = id - head + 8;
-    twice = (atomicOr(&bits[bit >> 5], 1u << (bit & 31)) >> (bit & 31)) & 1u;
+    const int rel = id - sp.head, o = rel >> 3;
+    if ((rel < 0 && sl.first) || (rel >= 0 && o >= sl.o0 && (o < sl.o1 || sl.last))) {
+      const int bit = rel - 8 * sl.o0 + 8;
+      if ((atomicOr(&bits[bit >> 5], 1u << (bit & 31)) >> (bit & 31)) & 1u) sh.twice = 1;
+    }
   }
-  if (__syncthreads_or(twice)) {
-    for (int j = 0; j < k && id >= 0; ++j)
-      if (j < a.K && sh.ids[j] == id) id = -1;
+  __syncthreads();
+}
+
+// One octet into a running (m, s), without the tokens whose bits are set.
+__device__ __forceinline__ void add_octet(MaxSum& a, float (&v)[8], uint32_t listed, float c) {
+  if (listed) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if ((listed >> e) & 1u) v[e] = -INFINITY;
   }
-  return id;
+  const float lm = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+  if (lm > a.m) {
+    a.s *= ex2((a.m - lm) * c);
+    a.m = lm;
+  }
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = ex2((v[e] - a.m) * c);
+  a.s += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+}
+
+// Head and tail of the row, one element a thread.
+template <typename T>
+__device__ __forceinline__ void add_ends(MaxSum& a, const T* z, const RowSpan& sp, const Slice& sl,
+                                         const uint32_t* bits, float c) {
+  const int t = threadIdx.x;
+  const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bits);
+  if (sl.first && t < sp.head && !((bytes[0] >> (8 - sp.head + t)) & 1)) add_one(a, to_f(z[t]), c);
+  if (sl.last && t < sp.tail && !((bytes[sl.o1 - sl.o0 + 1] >> t) & 1))
+    add_one(a, to_f(z[sp.head + 8 * (int64_t)sp.octs + t]), c);
 }
 
 // Everything of a row that follows from the unlisted tokens' (m, s): loss, logprob, stats and the slots' gradients.
+// Run by one warp, a lane for every 32nd slot.
 template <typename T>
-__device__ void row_loss(const DistArgs& a, int row, int V, const T* z, int id, float lpf, MaxSum rest,
-                         DistShared& sh) {
-  const int k = threadIdx.x;
+__device__ void row_loss(const DistArgs& a, int row, int V, const T* z, MaxSum rest, bool twice, DistShared& sh) {
+  const int lane = threadIdx.x & 31, K = a.K;
   const double rT = 1.0 / a.T;
-  const double zk = id >= 0 ? (double)to_f(z[id]) : 0.0;
+  const float* lps = a.lps + (int64_t)row * K;
+  if (twice) {  // the first slot of a token counts
+    for (int k = lane; k < K; k += 32) {
+      int id = sh.ids[k];
+      for (int j = 0; j < k && id >= 0; ++j)
+        if (a.ids[(int64_t)row * K + j] == id && lps[j] > -INFINITY) id = -1;
+      sh.h[k] = (double)id;
+    }
+    __syncwarp();
+    for (int k = lane; k < K; k += 32) sh.ids[k] = (int)sh.h[k];
+    __syncwarp();
+  }
   // common maximum of the listed and unlisted logits
-  float mk = id >= 0 ? to_f(z[id]) : -FLT_MAX;
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) mk = fmaxf(mk, __shfl_xor_sync(0xffffffffu, mk, off));
-  if ((k & 31) == 0) sh.red[k >> 5].m = mk;
-  __syncthreads();
   float mf = rest.m;
-  for (int w = 0; w < kDistThreads / 32; ++w) mf = fmaxf(mf, sh.red[w].m);
+  bool any = false;
+  for (int k = lane; k < K; k += 32) {
+    const int id = sh.ids[k];
+    const float v = id >= 0 ? to_f(z[id]) : -INFINITY;
+    any |= id >= 0;
+    sh.e[k] = (double)v;
+    mf = fmaxf(mf, v);
+  }
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) mf = fmaxf(mf, __shfl_xor_sync(0xffffffffu, mf, off));
+  any = __any_sync(0xffffffffu, any);
   const double m = (double)mf;
-  const bool any = __syncthreads_or(id >= 0);
+  double s = 0.0, mass = 0.0;
+  for (int k = lane; k < K; k += 32) {
+    const bool on = sh.ids[k] >= 0;
+    const double x = on ? (sh.e[k] - m) * rT : 0.0;  // log q + log s
+    sh.h[k] = x;
+    sh.e[k] = on ? exp(x) : 0.0;
+    sh.p[k] = on ? exp((double)lps[k]) : 0.0;
+    s += sh.e[k];
+    mass += sh.p[k];
+  }
   const double s_rest = (double)rest.s;
   const double shift = ((double)rest.m - m) * rT;  // of the unlisted sum to the common maximum
   const double e_rest = s_rest == 0.0 ? 0.0 : s_rest * exp(shift);
-  const double ek = id >= 0 ? exp((zk - m) * rT) : 0.0;
-  const double s = block_sum(ek, sh.sum) + e_rest;
+  s = warp_sum(s) + e_rest;
+  mass = warp_sum(mass);
   const double log_s = log(s);
   const bool has_rest = !(s_rest == 0.0);
+  const bool valid = any && !(s == 0.0) && !(a.drop && mass == 0.0);
   const double q_rest = e_rest / s;
   const double lq_rest = has_rest ? shift + log(s_rest) - log_s : 0.0;
-  double lp = (double)lpf;
-  double p = id >= 0 ? exp(lp) : 0.0;
-  const double mass = block_sum(p, sh.sum);
-  const bool valid = any && !(s == 0.0) && !(a.drop && mass == 0.0);
-  double p_rest = 0.0;
+  double p_rest = 0.0, by = 1.0, log_by = 0.0;
   if (a.drop) {
-    const double by = mass > 0.0 ? mass : 1.0;
-    lp -= log(by);
-    p /= by;
+    if (mass > 0.0) {
+      by = 1.0 / mass;
+      log_by = log(mass);
+    }
   } else if (has_rest) {
     p_rest = fmax(1.0 - mass, kRestFloor);
   }
   const double total = a.drop ? 1.0 : mass + p_rest;
   const double lp_rest = p_rest > 0.0 ? log(p_rest) : 0.0;
-  const double lq = id >= 0 ? (zk - m) * rT - log_s : 0.0;
-  const double q = ek / s;
-  double loss = 0.0, dk = 0.0, d_rest = 0.0;  // d_rest: q_r times the unlisted tokens' coefficient
-  if (a.div == kForward) {
-    const double t = id >= 0 && p > 0.0 ? p * (lp - lq) : 0.0;
-    loss = block_sum(t, sh.sum) + (p_rest > 0.0 ? p_rest * (lp_rest - lq_rest) : 0.0);
-    dk = q * total - p;
-    d_rest = q_rest * total - p_rest;
-  } else {
-    double h = 0.0, h_rest = 0.0, kp = 0.0, kp_rest = 0.0;
-    if (a.div == kReverse) {
-      if (id >= 0 && !(q == 0.0)) h = lq - lp;
-      if (has_rest) h_rest = lq_rest - lp_rest;
-    } else {
-      const double b = a.beta;
-      if (id >= 0) {
+  const double rs = 1.0 / s, b = a.beta;
+  double loss = 0.0, mean = 0.0, d_rest, h_rest = 0.0;  // d_rest: q_r times the unlisted tokens' coefficient
+  const int64_t base = (int64_t)row * K;
+  for (int k = lane; k < K; k += 32) {
+    const bool on = sh.ids[k] >= 0;
+    const double p = sh.p[k] * by, q = sh.e[k] * rs;
+    const double lp = (double)lps[k] - log_by, lq = sh.h[k] - log_s;
+    double h = 0.0;
+    if (on) {
+      if (a.div == kForward) {
+        if (p > 0.0) loss += p * (lp - lq);
+        h = q * total - p;  // here already the gradient
+      } else if (a.div == kReverse) {
+        if (!(q == 0.0)) h = lq - lp;
+        mean += q * h;
+      } else {
         const double lm = log(b * p + (1.0 - b) * q);
         if (!(q == 0.0)) h = (1.0 - b) * (lq - lm);
-        if (p > 0.0) kp = b * p * (lp - lm);
-      }
-      if (has_rest) {
-        const double lm = log(b * p_rest + (1.0 - b) * q_rest);
-        h_rest = (1.0 - b) * (lq_rest - lm);
-        if (p_rest > 0.0) kp_rest = b * p_rest * (lp_rest - lm);
+        if (p > 0.0) loss += b * p * (lp - lm);
+        mean += q * h;
       }
     }
-    const double mean = block_sum(q * h, sh.sum) + q_rest * h_rest;
-    loss = mean + block_sum(kp, sh.sum) + kp_rest;
-    dk = q * (h - mean);
+    sh.h[k] = h;
+    sh.e[k] = q;
+  }
+  loss = warp_sum(loss);
+  if (a.div == kForward) {
+    if (p_rest > 0.0) loss += p_rest * (lp_rest - lq_rest);
+    d_rest = q_rest * total - p_rest;
+  } else {
+    if (has_rest) {
+      if (a.div == kReverse) {
+        h_rest = lq_rest - lp_rest;
+      } else {
+        const double lm = log(b * p_rest + (1.0 - b) * q_rest);
+        h_rest = (1.0 - b) * (lq_rest - lm);
+        if (p_rest > 0.0) loss += b * p_rest * (lp_rest - lm);
+      }
+    }
+    mean = warp_sum(mean) + q_rest * h_rest;
+    loss += mean;
     d_rest = q_rest * (h_rest - mean);
   }
-  if (k < a.K) {
-    const int64_t at = (int64_t)row * a.K + k;
-    a.clean[at] = id;
-    a.dk[at] = id >= 0 && valid ? (float)dk : 0.f;
-    a.qk[at] = s == 0.0 ? 0.f : (float)q;
+  for (int k = lane; k < K; k += 32) {
+    const bool on = sh.ids[k] >= 0 && valid;
+    const double d = a.div == kForward ? sh.h[k] : sh.e[k] * (sh.h[k] - mean);
+    a.clean[base + k] = sh.ids[k];
+    a.dk[base + k] = on ? (float)d : 0.f;
+    a.qk[base + k] = s == 0.0 ? 0.f : (float)sh.e[k];
   }
-  if (k == 0) {
+  if (lane == 0) {
     a.loss[row] = valid ? (float)loss : 0.f;
-    float* st = a.stats + 4 * (int64_t)row;
-    st[0] = rest.m;
-    st[1] = valid && has_rest ? (float)(d_rest / s_rest) : 0.f;
-    st[2] = has_rest ? (float)(q_rest / s_rest) : 0.f;
     int flags = valid ? kLossRow : 0;
     if (a.targets) {
       const int64_t t = a.targets[row];
@@ -189,71 +247,139 @@ __device__ void row_loss(const DistArgs& a, int row, int V, const T* z, int id, 
       a.logp[row] = lt;
       if (lt != -INFINITY) flags |= kProbRow;
     }
-    st[3] = (float)flags;
+    *reinterpret_cast<float4*>(a.stats + 4 * (int64_t)row) =
+        make_float4(rest.m, valid && has_rest ? (float)(d_rest / s_rest) : 0.f,
+                    has_rest ? (float)(q_rest / s_rest) : 0.f, (float)flags);
   }
 }
 
+// One cluster of `n` CTAs a row: each CTA sums its slice, rank 0 joins the parts and finishes the row.
 template <typename T>
-__global__ void __launch_bounds__(kDistThreads) distill_fwd_kernel(const T* logits, int64_t ld, int V, DistArgs a) {
+__global__ void __launch_bounds__(kDistThreads, 4) distill_fwd_kernel(const T* logits, int64_t ld, int V, int n,
+                                                                      DistArgs a) {
   extern __shared__ uint32_t dist_bits[];
   __shared__ DistShared sh;
-  const int row = blockIdx.x;
+  const int row = blockIdx.x / n, rank = blockIdx.x % n;
   const T* z = logits + (int64_t)row * ld;
   const RowSpan sp = row_span(z, V);
-  const int words = (V + 15 + 31) >> 5;
-  for (int i = threadIdx.x; i < words; i += kDistThreads) dist_bits[i] = 0u;
-  __syncthreads();
-  float lp;
-  const int id = row_slots(a, row, V, sp.head, dist_bits, sh, lp);
+  const Slice sl = row_slice(sp, rank, n);
+  row_slots(a, row, V, sp, sl, dist_bits, sh);
+  const uint8_t* bytes = reinterpret_cast<const uint8_t*>(dist_bits) + 1 - sl.o0;
   const float c = (float)(1.4426950408889634 / a.T);
   MaxSum r = {-FLT_MAX, 0.f};
-  for (int j = threadIdx.x; j < V; j += kDistThreads) {
-    const int bit = j - sp.head + 8;
-    if (!((dist_bits[bit >> 5] >> (bit & 31)) & 1u)) add_one(r, to_f(z[j]), c);
+  add_ends(r, z, sp, sl, dist_bits, c);
+  constexpr int kU = sizeof(T) == 2 ? 4 : 2;  // 64 bytes in flight a thread
+  const T* body = z + sp.head;
+  int o = sl.o0 + threadIdx.x;
+  for (; o + (kU - 1) * kDistThreads < sl.o1; o += kU * kDistThreads) {
+    Oct<T> v[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) v[u].load_once(body + 8 * (int64_t)(o + u * kDistThreads));
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      float f[8];
+      v[u].get(f);
+      add_octet(r, f, bytes[o + u * kDistThreads], c);
+    }
+  }
+  for (; o < sl.o1; o += kDistThreads) {
+    Oct<T> v;
+    v.load_once(body + 8 * (int64_t)o);
+    float f[8];
+    v.get(f);
+    add_octet(r, f, bytes[o], c);
   }
   r = block_merge<kDistThreads>(r, c, sh.red);
-  row_loss(a, row, V, z, id, lp, r, sh);
+  if (threadIdx.x == 0) sh.part = r;
+  if (n > 1) cluster_sync_all();
+  if (rank == 0 && threadIdx.x < 32) {
+    int twice = sh.twice;
+    for (int i = 1; i < n; ++i) {
+      r = merge(r, MaxSum{ld_cluster(&sh.part.m, i), ld_cluster(&sh.part.s, i)}, c);
+      twice |= ld_cluster(&sh.twice, i);
+    }
+    row_loss(a, row, V, z, r, twice != 0, sh);
+  }
+  if (n > 1) cluster_sync_all();  // a CTA's shared memory outlives its readers
 }
 
-// dz = (g dL/dx + g_lp dlogp/dx) / T.  out may be the logits.  A row without gradient is written as zeros.
+// dz = (g dL/dx + g_lp dlogp/dx) / T over one of gridDim.y slices of a row.  out may be the logits.  A row without
+// gradient is written as zeros.
 template <typename T>
 __global__ void __launch_bounds__(kDistThreads) distill_bwd_kernel(const T* logits, int64_t ld, T* out, int64_t out_ld,
-                                                                   int V, int K, const int64_t* targets, float T_,
+                                                                   int V, int K, const int64_t* targets, double Td,
                                                                    const float* stats, const int* clean,
                                                                    const float* dk, const float* qk, const float* g,
                                                                    const float* g_lp) {
   const int row = blockIdx.x;
   const T* z = logits + (int64_t)row * ld;
-  T* o = out + (int64_t)row * out_ld;
-  const float* st = stats + 4 * (int64_t)row;
-  const float rT = 1.f / T_, c = kLog2e / T_;
-  const int flags = (int)st[3];
-  const float gk = flags & kLossRow ? (g ? g[row] : 1.f) : 0.f;
-  const float gl = g_lp && (flags & kProbRow) ? g_lp[row] : 0.f;
-  const int64_t target = g_lp && (flags & kProbRow) ? targets[row] : -1;
-  if (!(flags & kLossRow) && target < 0) {
-    for (int j = threadIdx.x; j < V; j += kDistThreads) from_f(o + j, 0.f);
-    return;
-  }
-  const float coef = (gk * st[1] - gl * st[2]) * rT, m = st[0];
-  // the table's tokens and the target, whose values replace the common form
+  T* out_row = out + (int64_t)row * out_ld;
+  const float4 st = *reinterpret_cast<const float4*>(stats + 4 * (int64_t)row);
+  const float rT = (float)(1.0 / Td), c = (float)(1.4426950408889634 / Td);
+  const int flags = (int)st.w;
+  const bool lp = g_lp && (flags & kProbRow);
+  const float gk = flags & kLossRow ? (g ? g[row] : 1.f) : 0.f, gl = lp ? g_lp[row] : 0.f;
+  const int64_t target = lp ? targets[row] : -1;
+  const bool zero = !(flags & kLossRow) && !lp;
+  const float coef = (gk * st.y - gl * st.z) * rT, m = st.x;
+  const RowSpan sp = row_span(z, V);
+  const Slice sl = row_slice(sp, blockIdx.y, gridDim.y);
+  const int lo = sl.first ? 0 : sp.head + 8 * sl.o0, hi = sl.last ? V : sp.head + 8 * sl.o1;
+  // the listed tokens and the target, whose values replace the common form
   const int k = threadIdx.x;
   int id = -1;
-  float val = 0.f;
+  float val = 0.f, t_val = 0.f;
   if (k < K) {
     const int64_t at = (int64_t)row * K + k;
     id = clean[at];
     val = (gk * dk[at] - gl * qk[at] + (id == target ? gl : 0.f)) * rT;
   }
-  const bool listed = __syncthreads_or(id >= 0 && id == target);
-  if (k == K && !listed && target >= 0 && target < V) {
-    id = (int)target;
-    val = coef * ex2((to_f(z[id]) - m) * c) + gl * rT;
+  const bool in_slice = target >= lo && target < hi;
+  if (k == 0 && in_slice) t_val = coef * ex2((to_f(z[target]) - m) * c) + gl * rT;
+  const bool listed = __syncthreads_or(id >= 0 && id == target);  // (and every read of a special precedes the writes)
+  const bool vec = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(out_row)) & 15u) == 0;
+  if (zero) {
+    for (int j = lo + k; j < hi; j += kDistThreads) from_f(out_row + j, 0.f);
+    return;
+  }
+  if (vec) {
+    if (sl.first && k < sp.head) from_f(out_row + k, coef * ex2((to_f(z[k]) - m) * c));
+    const int te = sp.head + 8 * sp.octs + k;
+    if (sl.last && k < sp.tail) from_f(out_row + te, coef * ex2((to_f(z[te]) - m) * c));
+    constexpr int kU = sizeof(T) == 2 ? 4 : 2;
+    const T* body = z + sp.head;
+    T* dst = out_row + sp.head;
+    int o = sl.o0 + k;
+    for (; o < sl.o1; o += kU * kDistThreads) {
+      Oct<T> v[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (o + u * kDistThreads < sl.o1) v[u].load_once(body + 8 * (int64_t)(o + u * kDistThreads));
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        if (o + u * kDistThreads < sl.o1) {
+          float f[8];
+          v[u].get(f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = coef * ex2((f[e] - m) * c);
+          store_oct(dst + 8 * (int64_t)(o + u * kDistThreads), f);
+        }
+      }
+    }
+  } else {  // the two rows are not aligned alike
+    for (int j = lo + k; j < hi; j += kDistThreads) from_f(out_row + j, coef * ex2((to_f(z[j]) - m) * c));
   }
   __syncthreads();
-  for (int j = threadIdx.x; j < V; j += kDistThreads) from_f(o + j, coef * ex2((to_f(z[j]) - m) * c));
-  __syncthreads();
-  if (id >= 0) from_f(o + id, val);
+  if (id >= lo && id < hi) from_f(out_row + id, val);
+  if (k == 0 && in_slice && !listed) from_f(out_row + target, t_val);
+}
+
+// CTAs a row: enough for three on every SM, at most 8 (a portable cluster), none below 2048 octets' worth of row.
+static int row_split(int N, int V) {
+  static const int want = 3 * 148;
+  int n = 1;
+  while (n < 8 && N * n < want && V / (2 * n) >= 4096) n *= 2;
+  return n;
 }
 
 static void check_distill(const torch::Tensor& logits, const torch::Tensor& ids, const torch::Tensor& lps, int64_t div,
@@ -302,12 +428,10 @@ std::vector<torch::Tensor> distill_fwd(torch::Tensor logits, torch::Tensor ids, 
   a.qk = qk.data_ptr<float>();
   a.err = err.data_ptr<int>();
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  const size_t smem = (size_t)((V + 15 + 31) >> 5) * 4;
+  const int n = row_split(N, V);
+  const size_t smem = (size_t)((V / 8 / n + 1 + 2 + 3) / 4) * 4;
   auto go = [&](auto kern, auto* p) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    LIBRA_CHECK(e == cudaSuccess, "distill_loss: %s", cudaGetErrorString(e));
-    kern<<<N, kDistThreads, smem, st>>>(p, logits.stride(0), V, a);
-    LIBRA_LAUNCH_CHECK();
+    launch_cluster(kern, dim3((unsigned)(N * (int64_t)n)), kDistThreads, smem, n, st, p, logits.stride(0), V, n, a);
   };
   if (logits.scalar_type() == at::kFloat)
     go(distill_fwd_kernel<float>, (const float*)logits.data_ptr());
@@ -339,11 +463,10 @@ void distill_bwd(torch::Tensor logits, torch::Tensor out, double T, c10::optiona
   const c10::cuda::CUDAGuard guard(logits.device());
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   auto go = [&](auto kern, auto* p, auto* o) {
-    kern<<<N, kDistThreads, 0, st>>>(p, logits.stride(0), o, out.stride(0), V, K,
-                                     targets.has_value() ? targets->data_ptr<int64_t>() : nullptr, (float)T,
-                                     stats.data_ptr<float>(), clean.data_ptr<int>(), dk.data_ptr<float>(),
-                                     qk.data_ptr<float>(), g.has_value() ? g->data_ptr<float>() : nullptr,
-                                     g_lp.has_value() ? g_lp->data_ptr<float>() : nullptr);
+    kern<<<dim3(N, row_split(N, V)), kDistThreads, 0, st>>>(
+        p, logits.stride(0), o, out.stride(0), V, K, targets.has_value() ? targets->data_ptr<int64_t>() : nullptr, T,
+        stats.data_ptr<float>(), clean.data_ptr<int>(), dk.data_ptr<float>(), qk.data_ptr<float>(),
+        g.has_value() ? g->data_ptr<float>() : nullptr, g_lp.has_value() ? g_lp->data_ptr<float>() : nullptr);
     LIBRA_LAUNCH_CHECK();
   };
   if (logits.scalar_type() == at::kFloat)

@@ -16,6 +16,7 @@
 #include <torch/extension.h>
 
 #include <cfloat>
+#include <utility>
 
 #include "common.cuh"
 
@@ -142,6 +143,51 @@ __device__ __forceinline__ MaxSum block_merge(MaxSum a, float c, MaxSum* sh) {
   for (int i = 1; i < kThreads / 32; ++i) a = merge(a, sh[i], c);
   __syncthreads();
   return a;
+}
+
+// The share of a row that CTA `rank` of `n` takes: octets [o0, o1); rank 0 also has the head, the last one the tail.
+struct Slice {
+  int o0, o1;
+  bool first, last;
+};
+__device__ __forceinline__ Slice row_slice(const RowSpan& sp, int rank, int n) {
+  return {(int)((int64_t)sp.octs * rank / n), (int)((int64_t)sp.octs * (rank + 1) / n), rank == 0, rank == n - 1};
+}
+
+// Another CTA's shared memory (same cluster), after a cluster barrier.
+__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ int ld_cluster(const int* p, uint32_t rank) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+
+// Launch with `cluster` CTAs of grid.x to a cluster (1: an ordinary launch).
+template <typename... KArgs, typename... Args>
+inline void launch_cluster(void (*kern)(KArgs...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st,
+                           Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    LIBRA_CHECK(e == cudaSuccess, "libra_b200: shared memory: %s", cudaGetErrorString(e));
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+  LIBRA_CHECK(e == cudaSuccess, "libra_b200: kernel launch failed: %s", cudaGetErrorString(e));
 }
 
 // Host checks shared by the three operators.

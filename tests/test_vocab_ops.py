@@ -417,7 +417,9 @@ def test_distill_strides(device, layout, dtype):
     _check_distill(z, ids, lps, "js", 0.5)
     _check_distill(z, ids, lps, "js", 0.5, one_pass=True)
     if layout != "transposed":
-        loss, grad = ops.distill_loss_grad(z.clone(), ids, lps)
+        # in place: the bits of a call out of place on rows that start as they do (a row's alignment orders its sum,
+        # so rows aligned otherwise agree within the limits above only)
+        loss, grad = ops.distill_loss_grad(z, ids, lps)
         w = _view(z.clone(), layout)
         loss2, out = ops.distill_loss_grad(w, ids, lps, out=w)
         assert out is w and torch.equal(loss, loss2) and torch.equal(grad, w)
