@@ -117,9 +117,10 @@ std::vector<torch::Tensor> top_logprobs(torch::Tensor logits, int64_t k, c10::op
 std::vector<torch::Tensor> distill_fwd(torch::Tensor logits, torch::Tensor ids, torch::Tensor lps, int64_t div,
                                        double beta, bool drop, double T, c10::optional<torch::Tensor> targets,
                                        torch::Tensor err);
-void distill_bwd(torch::Tensor logits, torch::Tensor out, double T, c10::optional<torch::Tensor> targets,
-                 torch::Tensor stats, torch::Tensor clean, torch::Tensor dk, torch::Tensor qk,
-                 c10::optional<torch::Tensor> g, c10::optional<torch::Tensor> g_lp);
+torch::Tensor distill_onepass(torch::Tensor logits, torch::Tensor ids, torch::Tensor lps, int64_t div, double beta,
+                              bool drop, double T, torch::Tensor out, torch::Tensor err);
+void distill_bwd(torch::Tensor logits, torch::Tensor out, double T, int64_t K, c10::optional<torch::Tensor> targets,
+                 torch::Tensor saved, c10::optional<torch::Tensor> g, c10::optional<torch::Tensor> g_lp);
 }  // namespace vocab
 }  // namespace libra
 
@@ -183,6 +184,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "repetition / presence / frequency penalties, biases and grammar masks on rows of logits");
   m.def("top_logprobs", &libra::vocab::top_logprobs, "k largest logits of every row with their logprobs");
   m.def("distill_fwd", &libra::vocab::distill_fwd, "distillation loss from a teacher's top logprobs");
+  m.def("distill_onepass", &libra::vocab::distill_onepass, "distillation loss and unit gradient in one pass");
   m.def("distill_bwd", &libra::vocab::distill_bwd, "gradient of distill_fwd with respect to the logits");
   m.def("flash_fwd", &libra::attn::flash_fwd, "tcgen05 varlen GQA attention forward", py::arg("q"), py::arg("k"),
         py::arg("v"), py::arg("cu_seqlens"), py::arg("tiles"), py::arg("scale"), py::arg("causal"), py::arg("err"),

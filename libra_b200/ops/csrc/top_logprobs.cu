@@ -60,7 +60,8 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T* logits, int64
   const float c = kLog2e / tm;
   MaxSum a = {-FLT_MAX, 0.f};
   for (int j = threadIdx.x; j < V; j += kTopThreads) add_one(a, to_f(z[j]), c);
-  a = block_merge<kTopThreads>(a, c, sh.red);
+  put_warp(a, c, sh.red);
+  a = join_warps<kTopThreads / 32>(c, sh.red);
   const uint32_t kth = kth_key(z, V, k, sh);
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();

@@ -5,11 +5,14 @@
 // taken as a scalar head up to the next 16-byte boundary, "octets" of eight
 // elements (one 16-byte load of bf16, two of fp32) and a scalar tail.
 //
-// Softmax statistics are a running maximum m and s = sum exp2((z - m) c) with
-// c = log2(e) / T.  m starts at the lowest finite float instead of -inf: the
-// difference z - m is then never inf - inf, so a -inf logit adds exactly 0, a
-// row of the type's lowest value is uniform, and a row with nothing but -inf
-// ends with s = 0.
+// Softmax statistics are a running reference m and s = sum exp2((z - m) c) with
+// c = log2(e) / T.  m is a logit of the row; it follows the maximum only when
+// that is more than 2^kSlack above it in the sum's terms, which happens once or
+// twice a thread, where an exact running maximum would rescale almost every
+// octet of some lane of a warp.  fp32 holds the larger sums as exactly.  m
+// starts at the lowest finite float instead of -inf: the difference z - m is
+// then never inf - inf, so a -inf logit adds exactly 0, a row of the type's
+// lowest value is uniform, and a row with nothing but -inf ends with s = 0.
 #pragma once
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -19,10 +22,12 @@
 #include <utility>
 
 #include "common.cuh"
+#include "tmap.cuh"
 
 namespace libra {
 namespace vocab {
 
+constexpr float kSlack = 20.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct RowSpan {
@@ -51,6 +56,11 @@ struct Oct<__nv_bfloat16> {
   uint4 a;
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void load_once(const __nv_bfloat16* p) { a = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ float max() const {  // of the numbers in it
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&a);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
@@ -70,6 +80,9 @@ struct Oct<float> {
   __device__ __forceinline__ void load_once(const float* p) {
     a = __ldcs(reinterpret_cast<const float4*>(p));
     b = __ldcs(reinterpret_cast<const float4*>(p + 4));
+  }
+  __device__ __forceinline__ float max() const {
+    return fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w)));
   }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
@@ -112,14 +125,42 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
 }
 
+// Two fp32 lanes in one instruction.
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 c, a, b;\n\t"
+      "mov.b64 {%0, %1}, c;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 c, a, b;\n\t"
+      "mov.b64 {%0, %1}, c;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+// exp2((v - m) c) of eight values.
+__device__ __forceinline__ void exp_oct(float (&v)[8], float m, float c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const F2 x = mul2(add2(F2{v[2 * i], v[2 * i + 1]}, F2{-m, -m}), F2{c, c});
+    v[2 * i] = ex2(x.x);
+    v[2 * i + 1] = ex2(x.y);
+  }
+}
+__device__ __forceinline__ F2 sum_oct(const float (&v)[8]) {
+  return add2(add2(F2{v[0], v[1]}, F2{v[2], v[3]}), add2(F2{v[4], v[5]}, F2{v[6], v[7]}));
+}
+
 struct MaxSum {
   float m, s;
 };
-
-__device__ __forceinline__ MaxSum merge(MaxSum a, MaxSum b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  return {m, a.s * ex2((a.m - m) * c) + b.s * ex2((b.m - m) * c)};
-}
 
 __device__ __forceinline__ void add_one(MaxSum& a, float z, float c) {
   const float m = fmaxf(a.m, z);
@@ -127,32 +168,55 @@ __device__ __forceinline__ void add_one(MaxSum& a, float z, float c) {
   a.m = m;
 }
 
-// Over the block; `sh` holds one entry a warp.  Every thread gets the result, and the merge order is fixed.
-template <int kThreads>
-__device__ __forceinline__ MaxSum block_merge(MaxSum a, float c, MaxSum* sh) {
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) {
-    const MaxSum b = {__shfl_xor_sync(0xffffffffu, a.m, off), __shfl_xor_sync(0xffffffffu, a.s, off)};
-    a = merge(a, b, c);
-  }
-  const int w = threadIdx.x >> 5;
-  if ((threadIdx.x & 31) == 0) sh[w] = a;
-  __syncthreads();
-  a = sh[0];
+  for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+__device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
-  for (int i = 1; i < kThreads / 32; ++i) a = merge(a, sh[i], c);
-  __syncthreads();
-  return a;
+  for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+// Largest of the numbers (not NaN) in a warp.
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 
-// The share of a row that CTA `rank` of `n` takes: octets [o0, o1); rank 0 also has the head, the last one the tail.
+// Over a warp; every lane gets the same result.
+__device__ __forceinline__ MaxSum warp_merge(MaxSum a, float c) {
+  const float m = warp_max(a.m);
+  return {m, warp_sum(__fmul_rn(a.s, ex2((a.m - m) * c)))};
+}
+
+// Over the block, as far as the warps' results in `sh`, which any warp joins with join_warps.
+__device__ __forceinline__ void put_warp(MaxSum a, float c, MaxSum* sh) {
+  a = warp_merge(a, c);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
+  __syncthreads();
+}
+template <int kWarps>
+__device__ __forceinline__ MaxSum join_warps(float c, const MaxSum* sh) {
+  const int lane = threadIdx.x & 31;
+  return warp_merge(lane < kWarps ? sh[lane] : MaxSum{-FLT_MAX, 0.f}, c);
+}
+
+// The share of a row that CTA `rank` of 2^lg takes: octets [o0, o1); rank 0 also has the head, the last one the tail
+// and the octets that an even split leaves over (fewer than 2^lg).
 struct Slice {
   int o0, o1;
   bool first, last;
 };
-__device__ __forceinline__ Slice row_slice(const RowSpan& sp, int rank, int n) {
-  return {(int)((int64_t)sp.octs * rank / n), (int)((int64_t)sp.octs * (rank + 1) / n), rank == 0, rank == n - 1};
+__device__ __forceinline__ Slice row_slice(const RowSpan& sp, int rank, int lg) {
+  const int per = sp.octs >> lg;
+  const bool last = rank == (1 << lg) - 1;
+  return {rank * per, last ? sp.octs : (rank + 1) * per, rank == 0, last};
 }
+// Most octets of a slice.
+inline int slice_octs(int V, int n) { return V / 8 / n + n - 1; }
+inline int log2_of(int n) { return n <= 1 ? 0 : 1 + log2_of(n / 2); }
 
 // Another CTA's shared memory (same cluster), after a cluster barrier.
 __device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
@@ -166,25 +230,54 @@ __device__ __forceinline__ int ld_cluster(const int* p, uint32_t rank) {
   return v;
 }
 
-// Launch with `cluster` CTAs of grid.x to a cluster (1: an ordinary launch).
+__device__ __forceinline__ double ld_cluster(const double* p, uint32_t rank) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// 16 bytes global -> shared without a register; a thread that reads only what it copied itself needs no barrier.
+__device__ __forceinline__ void copy16_async(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+
+// Launch of `ctas` CTAs, `cluster` of them to a cluster (1: an ordinary launch).  pdl: the kernel may start while the
+// one before it on the stream runs, and waits for it itself (pdl_wait).
 template <typename... KArgs, typename... Args>
-inline void launch_cluster(void (*kern)(KArgs...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st,
-                           Args&&... args) {
+inline void launch_rows(void (*kern)(KArgs...), int64_t ctas, int threads, size_t smem, int cluster, bool pdl,
+                        cudaStream_t st, Args&&... args) {
+  LIBRA_CHECK(ctas < (1ll << 31), "libra_b200: too many rows for one launch");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
+  cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
+  if (pdl) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
-  if (smem > 48 * 1024) {
+  if (smem > 32 * 1024) {  // with the kernel's static part this may pass the default 48 KB
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     LIBRA_CHECK(e == cudaSuccess, "libra_b200: shared memory: %s", cudaGetErrorString(e));
+  }
+  if (cluster > 8) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    LIBRA_CHECK(e == cudaSuccess, "libra_b200: cluster size: %s", cudaGetErrorString(e));
   }
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
   LIBRA_CHECK(e == cudaSuccess, "libra_b200: kernel launch failed: %s", cudaGetErrorString(e));

@@ -127,10 +127,10 @@ class _DistillLoss(torch.autograd.Function):
     def forward(ctx, logits, ids, lps, div, beta, drop, temperature, targets):
         from . import error_flag, ext
 
-        loss, logp, stats, clean, dk, qk = ext().distill_fwd(logits, ids, lps, div, beta, drop, temperature, targets,
-                                                             error_flag(logits.device))
-        ctx.save_for_backward(logits, targets, stats, clean, dk, qk)
-        ctx.temperature = temperature
+        loss, logp, saved = ext().distill_fwd(logits, ids, lps, div, beta, drop, temperature, targets,
+                                              error_flag(logits.device))
+        ctx.save_for_backward(logits, targets, saved)
+        ctx.temperature, ctx.slots = temperature, ids.shape[1]
         ctx.set_materialize_grads(False)
         return loss, (logp if targets is not None else None)
 
@@ -139,12 +139,12 @@ class _DistillLoss(torch.autograd.Function):
     def backward(ctx, g, g_lp):
         from . import ext
 
-        logits, targets, stats, clean, dk, qk = ctx.saved_tensors
+        logits, targets, saved = ctx.saved_tensors
         if g is None and g_lp is None:
             return (None,) * 8
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         g = torch.zeros(logits.shape[0], device=logits.device) if g is None else g.contiguous()
-        ext().distill_bwd(logits, grad, ctx.temperature, targets, stats, clean, dk, qk, g,
+        ext().distill_bwd(logits, grad, ctx.temperature, ctx.slots, targets, saved, g,
                           None if g_lp is None else g_lp.contiguous())
         return (grad,) + (None,) * 7
 
@@ -199,8 +199,7 @@ def distill_loss_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
 
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    loss, _, stats, clean, dk, qk = ext().distill_fwd(logits, teacher_ids.contiguous(), teacher_logprobs.contiguous(),
-                                                      DIVERGENCES[divergence], float(beta), tail == "drop",
-                                                      float(temperature), None, error_flag(logits.device))
-    ext().distill_bwd(logits, out, float(temperature), None, stats, clean, dk, qk, None, None)
+    loss = ext().distill_onepass(logits, teacher_ids.contiguous(), teacher_logprobs.contiguous(),
+                                 DIVERGENCES[divergence], float(beta), tail == "drop", float(temperature), out,
+                                 error_flag(logits.device))
     return loss, out
