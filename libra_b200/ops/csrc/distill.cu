@@ -122,14 +122,7 @@ __device__ __forceinline__ void add_octet(MaxSum& a, float& top, const Oct<T>& r
       if ((listed >> e) & 1u) v[e] = -INFINITY;
     lm = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
   }
-  if (lm > top) {
-    a.s *= ex2((a.m - lm) * c);
-    a.m = lm;
-    top = lm + slack;
-  }
-  exp_oct(v, a.m, c);
-  const F2 s = sum_oct(v);
-  a.s += s.x + s.y;
+  add_values(a, top, v, lm, c, slack);
 }
 
 // Head and tail of the row, one element a thread.

@@ -4,33 +4,83 @@
 //   lse = log sum_j exp(z_j / T),   logprob_i = z_i / T - lse
 //
 // The order is taken on the raw logits, so scaling cannot make new ties.
+//
+// One pass over the row gives the softmax sum and the candidates.  Every
+// thread keeps the maxima of four classes of its octets; the k-th largest of
+// those 1024 maxima of disjoint classes is a lower bound of the k-th largest
+// logit.  The bound is taken after the first round of loads and again a little
+// later; an octet whose maximum reaches it is noted (a few hundred of 19
+// thousand), and only noted octets are looked at again, against the final
+// bound.  What remains, little more than k values, is ranked by counting.
+// Slices whose values defeat the bound (long ties, ascending rows, NaN) take
+// an exact radix select over the slice instead.
+//
+// Rows are split over a cluster when there are few: every CTA then finds the
+// sorted top of its slice and looks up its entries' ranks in the other lists.
 #include "vocab_rows.cuh"
 
 namespace libra {
 namespace vocab {
 
-constexpr int kTopThreads = 512;
+constexpr int kTopThreads = 256;
+constexpr int kTopWarps = kTopThreads / 32;
 constexpr int kTopMax = 256;
+constexpr int kClasses = 4;     // of octets a thread; 1024 maxima a block
+constexpr int kNoted = 4096;    // octets
+constexpr int kChosen = 1024;   // values at or above the final bound
+constexpr uint32_t kInfKey = 0x007fffffu;  // order_key(-inf)
 
 struct TopShared {
-  MaxSum red[kTopThreads / 32];
+  unsigned long long chosen[kChosen];  // key << 32 | ~index: larger is better
+  unsigned long long list[kTopMax];    // sorted top of the slice, without -inf
+  int noted[kNoted];
   unsigned hist[256];
-  unsigned long long best[kTopMax];  // key << 32 | ~index: larger is better
-  int n, bin, left;
-  int wsum[kTopThreads / 32];
+  int count[16];
+  MaxSum red[kTopWarps];
+  MaxSum part;
+  int n_noted, n_chosen, n_list, bin, left;
+  int wsum[kTopWarps];
 };
 
-// Key of the k-th largest element: radix select from the most significant byte.
+__device__ __forceinline__ unsigned long long entry_of(float v, int j) {
+  return ((unsigned long long)order_key(v) << 32) | (uint32_t)~j;
+}
+
+// Largest bound b with at least k of the block's class maxima at or above it (to the upper 16 bits of its key, which
+// are all of a bf16 value's); the lowest finite float if fewer than k are above -inf.
+__device__ __forceinline__ float kth_bound(const float (&cls)[kClasses], int k, TopShared& sh) {
+  uint32_t key[kClasses], prefix = 0u;
+#pragma unroll
+  for (int i = 0; i < kClasses; ++i) key[i] = order_key(cls[i]);
+  if (threadIdx.x < 16) sh.count[threadIdx.x] = 0;
+  __syncthreads();
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t trial = prefix | (1u << bit);
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < kClasses; ++i) c += key[i] >= trial;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if ((threadIdx.x & 31) == 0 && c) atomicAdd(&sh.count[bit - 16], c);
+    __syncthreads();
+    if (sh.count[bit - 16] >= k) prefix = trial;
+  }
+  __syncthreads();
+  return prefix <= kInfKey ? -FLT_MAX : key_value(prefix);
+}
+
+// The slice's exact top (at most k) into sh.chosen, by radix select on the key from its most significant byte and the
+// lowest indices among the ties with the k-th.  [lo, hi): the slice's tokens.
 template <typename T>
-__device__ uint32_t kth_key(const T* z, int V, int k, TopShared& sh) {
-  uint32_t prefix = 0u, mask = 0u;
+__device__ int exact_top(const T* z, int lo, int hi, int k, TopShared& sh) {
+  k = min(k, hi - lo);
+  uint32_t kth = 0u, mask = 0u;
   int left = k;
   for (int shift = 24; shift >= 0; shift -= 8) {
     for (int i = threadIdx.x; i < 256; i += kTopThreads) sh.hist[i] = 0u;
     __syncthreads();
-    for (int j = threadIdx.x; j < V; j += kTopThreads) {
+    for (int j = lo + threadIdx.x; j < hi; j += kTopThreads) {
       const uint32_t key = order_key(to_f(z[j]));
-      if ((key & mask) == prefix) atomicAdd(&sh.hist[(key >> shift) & 255u], 1u);
+      if ((key & mask) == kth) atomicAdd(&sh.hist[(key >> shift) & 255u], 1u);
     }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -40,66 +90,201 @@ __device__ uint32_t kth_key(const T* z, int V, int k, TopShared& sh) {
       sh.left = left - above;
     }
     __syncthreads();
-    prefix |= (uint32_t)sh.bin << shift;
+    kth |= (uint32_t)sh.bin << shift;
     mask |= 255u << shift;
     left = sh.left;
     __syncthreads();
   }
-  return prefix;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kTopThreads) top_kernel(const T* logits, int64_t ld, int V, int k,
-                                                          const float* temps, float temp, int64_t* out_ids,
-                                                          float* out_lp, float* out_lse) {
-  __shared__ TopShared sh;
-  const int row = blockIdx.x;
-  const T* z = logits + (int64_t)row * ld;
-  float tm = temps ? temps[row] : temp;
-  if (!(tm > 0.f)) tm = 1.f;
-  const float c = kLog2e / tm;
-  MaxSum a = {-FLT_MAX, 0.f};
-  for (int j = threadIdx.x; j < V; j += kTopThreads) add_one(a, to_f(z[j]), c);
-  put_warp(a, c, sh.red);
-  a = join_warps<kTopThreads / 32>(c, sh.red);
-  const uint32_t kth = kth_key(z, V, k, sh);
-  if (threadIdx.x == 0) sh.n = 0;
+  if (threadIdx.x == 0) sh.n_chosen = 0;
   __syncthreads();
-  for (int j = threadIdx.x; j < V; j += kTopThreads) {
-    const uint32_t key = order_key(to_f(z[j]));
-    if (key > kth) sh.best[atomicAdd(&sh.n, 1)] = ((unsigned long long)key << 32) | (uint32_t)~j;
+  for (int j = lo + threadIdx.x; j < hi; j += kTopThreads) {
+    const float v = to_f(z[j]);
+    if (order_key(v) > kth) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = entry_of(v, j);
   }
   __syncthreads();
-  int have = sh.n;
-  __syncthreads();
-  // the remaining places go to the lowest indices among the ties with the k-th key
-  for (int j0 = 0; j0 < V && have < k; j0 += kTopThreads) {
+  int have = sh.n_chosen;
+  for (int j0 = lo; j0 < hi && have < k && kth > kInfKey; j0 += kTopThreads) {
     const int j = j0 + threadIdx.x;
-    const bool tie = j < V && order_key(to_f(z[j])) == kth;
+    const float v = j < hi ? to_f(z[j]) : 0.f;
+    const bool tie = j < hi && order_key(v) == kth;
     const unsigned ballot = __ballot_sync(0xffffffffu, tie);
     if ((threadIdx.x & 31) == 0) sh.wsum[threadIdx.x >> 5] = __popc(ballot);
     __syncthreads();
     int before = 0, total = 0;
-    for (int w = 0; w < kTopThreads / 32; ++w) {
+    for (int w = 0; w < kTopWarps; ++w) {
       if (w < (int)(threadIdx.x >> 5)) before += sh.wsum[w];
       total += sh.wsum[w];
     }
     const int at = have + before + __popc(ballot & ((1u << (threadIdx.x & 31)) - 1u));
-    if (tie && at < k) sh.best[at] = ((unsigned long long)kth << 32) | (uint32_t)~j;
+    if (tie && at < k) sh.chosen[at] = entry_of(v, j);
     have += total;
     __syncthreads();
   }
-  const float log_s = logf(a.s);
-  const bool none = a.s == 0.f;  // nothing but -inf
-  for (int i = threadIdx.x; i < k; i += kTopThreads) {
-    const unsigned long long me = sh.best[i];
-    int rank = 0;
-    for (int j = 0; j < k; ++j) rank += sh.best[j] > me;
-    out_ids[(int64_t)row * k + rank] = (int64_t)(uint32_t)~(uint32_t)me;
-    const float v = key_value((uint32_t)(me >> 32));
-    out_lp[(int64_t)row * k + rank] = none ? -INFINITY : (v - a.m) / tm - log_s;
+  return min(have, k);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTopThreads, 4) top_kernel(const T* logits, int64_t ld, int V, int lg, int k,
+                                                             const float* temps, float temp, int64_t* out_ids,
+                                                             float* out_lp, float* out_lse) {
+  extern __shared__ __align__(16) unsigned char top_smem[];
+  TopShared& sh = *reinterpret_cast<TopShared*>(top_smem);
+  const int n = 1 << lg, row = blockIdx.x >> lg, rank = blockIdx.x & (n - 1), t = threadIdx.x;
+  const T* z = logits + (int64_t)row * ld;
+  const RowSpan sp = row_span(z, V);
+  const Slice sl = row_slice(sp, rank, lg);
+  float tm = temps ? temps[row] : temp;
+  if (!(tm > 0.f)) tm = 1.f;
+  const float c = kLog2e / tm, slack = kSlack / c;
+  if (t == 0) sh.n_noted = sh.n_chosen = 0;
+  constexpr int kU = kClasses;
+  const T* body = z + sp.head;
+  Oct<T> v[kU];
+  float cls[kClasses];
+#pragma unroll
+  for (int u = 0; u < kU; ++u) cls[u] = -INFINITY;
+  int o = sl.o0 + t;
+#pragma unroll
+  for (int u = 0; u < kU; ++u)
+    if (o + u * kTopThreads < sl.o1) {
+      v[u].load_once(body + 8 * (int64_t)(o + u * kTopThreads));
+      cls[u] = v[u].max();
+    }
+  float bound = kth_bound(cls, k, sh);
+  MaxSum r = {-FLT_MAX, 0.f};
+  float top = -FLT_MAX;
+  int round = 0;
+  const int rounds = (sl.o1 - sl.o0 + kU * kTopThreads - 1) / (kU * kTopThreads);
+  for (; round < rounds; ++round, o += kU * kTopThreads) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (o + u * kTopThreads < sl.o1) {
+        const float lm = v[u].max();
+        cls[u] = fmaxf(cls[u], lm);
+        if (lm >= bound) {
+          const int at = atomicAdd(&sh.n_noted, 1);
+          if (at < kNoted) sh.noted[at] = o + u * kTopThreads;
+        }
+        float f[8];
+        v[u].get(f);
+        add_values(r, top, f, lm, c, slack);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+      if (o + (u + kU) * kTopThreads < sl.o1) v[u].load_once(body + 8 * (int64_t)(o + (u + kU) * kTopThreads));
+    if (round == 2 && rounds > 4) bound = fmaxf(bound, kth_bound(cls, k, sh));
   }
-  if (threadIdx.x == 0) out_lse[row] = none ? -INFINITY : a.m / tm + log_s;
+  const int te = sp.head + 8 * sp.octs + t;
+  const float ends[2] = {sl.first && t < sp.head ? to_f(z[t]) : -INFINITY,
+                         sl.last && t < sp.tail ? to_f(z[te]) : -INFINITY};
+  if (sl.first && t < sp.head) add_one(r, ends[0], c);
+  if (sl.last && t < sp.tail) add_one(r, ends[1], c);
+  put_warp(r, c, sh.red);
+  r = join_warps<kTopWarps>(c, sh.red);
+  if (t == 0) sh.part = r;
+  if (rounds > 1) bound = fmaxf(bound, kth_bound(cls, k, sh));
+  const int noted = sh.n_noted;
+  if (noted <= kNoted) {
+    for (int i = t; i < noted; i += kTopThreads) {
+      Oct<T> w;
+      const int at = sh.noted[i];
+      w.load(body + 8 * (int64_t)at);
+      float f[8];
+      w.get(f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (f[e] >= bound) {
+          const int p = atomicAdd(&sh.n_chosen, 1);
+          if (p < kChosen) sh.chosen[p] = entry_of(f[e], sp.head + 8 * at + e);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (ends[e] >= bound) {
+        const int p = atomicAdd(&sh.n_chosen, 1);
+        if (p < kChosen) sh.chosen[p] = entry_of(ends[e], e ? te : t);
+      }
+  }
+  __syncthreads();
+  int chosen = sh.n_chosen;
+  if (noted > kNoted || chosen > kChosen || r.s != r.s) {
+    __syncthreads();
+    chosen = exact_top(z, sl.first ? 0 : sp.head + 8 * sl.o0, sl.last ? V : sp.head + 8 * sl.o1, k, sh);
+    __syncthreads();
+  }
+  for (int i = t; i < chosen; i += kTopThreads) {
+    const unsigned long long me = sh.chosen[i];
+    int at = 0;
+    for (int j = 0; j < chosen; ++j) at += sh.chosen[j] > me;
+    if (at < k) sh.list[at] = me;
+  }
+  if (t == 0) sh.n_list = min(chosen, k);
+  if (n > 1)
+    cluster_sync_all();
+  else
+    __syncthreads();
+  if (n > 1) {
+    const int lane = t & 31;
+    r = warp_merge(lane < n ? MaxSum{ld_cluster(&sh.part.m, lane), ld_cluster(&sh.part.s, lane)}
+                            : MaxSum{-FLT_MAX, 0.f}, c);
+  }
+  const float log_s = logf(r.s);
+  const bool none = r.s == 0.f;  // nothing but -inf
+  int total = sh.n_list;
+  int lens[16];
+  if (n > 1) {
+    total = 0;
+    for (int i = 0; i < n; ++i) {
+      lens[i] = ld_cluster(&sh.n_list, i);
+      total += lens[i];
+    }
+  }
+  for (int i = t; i < sh.n_list; i += kTopThreads) {
+    const unsigned long long me = sh.list[i];
+    int place = i;
+    if (n > 1) {
+      for (int q = 0; q < n && place < k; ++q) {
+        if (q == rank) continue;
+        int lo = 0, hi = lens[q];  // entries before lo are larger, those from hi on are not
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (ld_cluster(&sh.list[mid], q) > me)
+            lo = mid + 1;
+          else
+            hi = mid;
+        }
+        place += lo;
+      }
+    }
+    if (place < k) {
+      out_ids[(int64_t)row * k + place] = (int64_t)(uint32_t)~(uint32_t)me;
+      out_lp[(int64_t)row * k + place] = (key_value((uint32_t)(me >> 32)) - r.m) / tm - log_s;
+    }
+  }
+  if (rank == 0 && t == 0) out_lse[row] = none ? -INFINITY : r.m / tm + log_s;
+  if (rank == 0 && total < k) {  // the remaining places go to the first -inf of the row
+    for (int j0 = 0; j0 < V && total < k; j0 += kTopThreads) {
+      const int j = j0 + t;
+      const bool hit = j < V && to_f(z[j]) == -INFINITY;
+      const unsigned ballot = __ballot_sync(0xffffffffu, hit);
+      if ((t & 31) == 0) sh.wsum[t >> 5] = __popc(ballot);
+      __syncthreads();
+      int before = 0, sum = 0;
+      for (int w = 0; w < kTopWarps; ++w) {
+        if (w < (t >> 5)) before += sh.wsum[w];
+        sum += sh.wsum[w];
+      }
+      const int at = total + before + __popc(ballot & ((1u << (t & 31)) - 1u));
+      if (hit && at < k) {
+        out_ids[(int64_t)row * k + at] = j;
+        out_lp[(int64_t)row * k + at] = r.s != r.s ? r.s : -INFINITY;
+      }
+      total += sum;
+      __syncthreads();
+    }
+  }
+  if (n > 1) cluster_sync_all();  // a CTA's list outlives its readers
 }
 
 // logits [N, V] bf16 / fp32 -> ids [N, k] int64, logprobs [N, k] fp32 (descending), lse [N] fp32.
@@ -119,15 +304,18 @@ std::vector<torch::Tensor> top_logprobs(torch::Tensor logits, int64_t k, c10::op
   if (N == 0) return {ids, lp, lse};
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   const float* tp = temps.has_value() ? temps->data_ptr<float>() : nullptr;
+  // CTAs a row: enough for three on every SM, at most 8, none for fewer than 4096 tokens
+  int n = 1;
+  while (n < 8 && N * n < 3 * 148 && V / (2 * n) >= 4096) n *= 2;
+  auto go = [&](auto kern, auto* p) {
+    launch_rows(kern, (int64_t)N * n, kTopThreads, sizeof(TopShared), n, false, st, p, logits.stride(0), V, log2_of(n),
+                (int)k, tp, (float)temperature, ids.data_ptr<int64_t>(), lp.data_ptr<float>(),
+                lse.data_ptr<float>());
+  };
   if (logits.scalar_type() == at::kFloat)
-    top_kernel<float><<<N, kTopThreads, 0, st>>>(logits.data_ptr<float>(), logits.stride(0), V, (int)k, tp,
-                                                 (float)temperature, ids.data_ptr<int64_t>(), lp.data_ptr<float>(),
-                                                 lse.data_ptr<float>());
+    go(top_kernel<float>, (const float*)logits.data_ptr());
   else
-    top_kernel<__nv_bfloat16><<<N, kTopThreads, 0, st>>>(
-        (const __nv_bfloat16*)logits.data_ptr(), logits.stride(0), V, (int)k, tp, (float)temperature,
-        ids.data_ptr<int64_t>(), lp.data_ptr<float>(), lse.data_ptr<float>());
-  LIBRA_LAUNCH_CHECK();
+    go(top_kernel<__nv_bfloat16>, (const __nv_bfloat16*)logits.data_ptr());
   return {ids, lp, lse};
 }
 

@@ -162,6 +162,18 @@ struct MaxSum {
   float m, s;
 };
 
+// An octet's values into a thread's running (m, s): `lm` is their maximum, `top` is m + kSlack / c.
+__device__ __forceinline__ void add_values(MaxSum& a, float& top, float (&v)[8], float lm, float c, float slack) {
+  if (lm > top) {
+    a.s *= ex2((a.m - lm) * c);
+    a.m = lm;
+    top = lm + slack;
+  }
+  exp_oct(v, a.m, c);
+  const F2 s = sum_oct(v);
+  a.s += s.x + s.y;
+}
+
 __device__ __forceinline__ void add_one(MaxSum& a, float z, float c) {
   const float m = fmaxf(a.m, z);
   a.s = a.s * ex2((a.m - m) * c) + ex2((z - m) * c);
@@ -230,6 +242,11 @@ __device__ __forceinline__ int ld_cluster(const int* p, uint32_t rank) {
   return v;
 }
 
+__device__ __forceinline__ unsigned long long ld_cluster(const unsigned long long* p, uint32_t rank) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
 __device__ __forceinline__ double ld_cluster(const double* p, uint32_t rank) {
   double v;
   asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
