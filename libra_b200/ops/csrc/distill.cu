@@ -333,15 +333,20 @@ __global__ void __launch_bounds__(kFwdThreads, 4) distill_sum_kernel(const T* lo
   const uint8_t* bytes = reinterpret_cast<const uint8_t*>(dist_bits) + 1 - sl.o0;
   MaxSum r = {-FLT_MAX, 0.f};
   float top = -FLT_MAX;
-  while (o < sl.o1) {
+  const int step = kU * kFwdThreads;
+  for (; o + step - kFwdThreads < sl.o1; o += step) {
+    Oct<T> w[kU];  // the next round's loads fly while this one is summed
 #pragma unroll
     for (int u = 0; u < kU; ++u)
-      if (o + u * kFwdThreads < sl.o1) add_octet(r, top, v[u], bytes[o + u * kFwdThreads], c, slack);
-    o += kU * kFwdThreads;
+      if (o + step + u * kFwdThreads < sl.o1) w[u].load_once(body + 8 * (int64_t)(o + step + u * kFwdThreads));
 #pragma unroll
-    for (int u = 0; u < kU; ++u)
-      if (o + u * kFwdThreads < sl.o1) v[u].load_once(body + 8 * (int64_t)(o + u * kFwdThreads));
+    for (int u = 0; u < kU; ++u) add_octet(r, top, v[u], bytes[o + u * kFwdThreads], c, slack);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) v[u] = w[u];
   }
+#pragma unroll
+  for (int u = 0; u < kU; ++u)
+    if (o + u * kFwdThreads < sl.o1) add_octet(r, top, v[u], bytes[o + u * kFwdThreads], c, slack);
   add_ends(r, z, sp, sl, dist_bits, c);
   put_warp(r, c, red);
   if (t < 32) {
@@ -580,10 +585,11 @@ __global__ void __launch_bounds__(kOneThreads, kOneCtas) distill_onepass_kernel(
   cluster_wait();  // a CTA's part outlives its readers
 }
 
-// CTAs a row: enough for three on every SM, at most 2^5, none for fewer than 4096 tokens.
+// CTAs a row: enough for two waves of four on every SM (777 x 50257 fp32, forward and backward: 119 us with one CTA a
+// row, which leaves the second wave a third full, 103 us with four), at most `most`, none for fewer than 4096 tokens.
 static int row_split(int N, int V, int most) {
   int n = 1;
-  while (n < most && N * n < 3 * 148 && V / (2 * n) >= 4096) n *= 2;
+  while (n < most && N * n < 8 * 148 && V / (2 * n) >= 4096) n *= 2;
   return n;
 }
 

@@ -6,12 +6,13 @@
 // The order is taken on the raw logits, so scaling cannot make new ties.
 //
 // One pass over the row gives the softmax sum and the candidates.  Every
-// thread keeps the maxima of four classes of its octets; the k-th largest of
-// those 1024 maxima of disjoint classes is a lower bound of the k-th largest
-// logit.  The bound is taken after the first round of loads and again a little
-// later; an octet whose maximum reaches it is noted (a few hundred of 19
+// thread keeps the maxima of four classes of its octets.  Where each of w warps
+// has k / w maxima of disjoint classes at or above b, k logits are, and b is a
+// lower bound of the k-th largest; a warp finds its own by bisection without a
+// barrier.  The bound is taken after the first round of loads and again a
+// little later; an octet whose maximum reaches it is noted (a few hundred of 19
 // thousand), and only noted octets are looked at again, against the final
-// bound.  What remains, little more than k values, is ranked by counting.
+// bound.  What remains, a little more than k values, is ranked by counting.
 // Slices whose values defeat the bound (long ties, ascending rows, NaN) take
 // an exact radix select over the slice instead.
 //
@@ -33,9 +34,12 @@ constexpr uint32_t kInfKey = 0x007fffffu;  // order_key(-inf)
 struct TopShared {
   unsigned long long chosen[kChosen];  // key << 32 | ~index: larger is better
   unsigned long long list[kTopMax];    // sorted top of the slice, without -inf
-  int noted[kNoted];
+  union {
+    int noted[kNoted];
+    unsigned long long others[kTopMax * 8];  // the cluster's lists, later
+  };
   unsigned hist[256];
-  int count[16];
+  float bound[kTopWarps];
   MaxSum red[kTopWarps];
   MaxSum part;
   int n_noted, n_chosen, n_list, bin, left;
@@ -46,26 +50,32 @@ __device__ __forceinline__ unsigned long long entry_of(float v, int j) {
   return ((unsigned long long)order_key(v) << 32) | (uint32_t)~j;
 }
 
-// Largest bound b with at least k of the block's class maxima at or above it (to the upper 16 bits of its key, which
-// are all of a bf16 value's); the lowest finite float if fewer than k are above -inf.
-__device__ __forceinline__ float kth_bound(const float (&cls)[kClasses], int k, TopShared& sh) {
-  uint32_t key[kClasses], prefix = 0u;
+// A bound b with at least k of the block's class maxima at or above it: the least over the first `warps` warps (those
+// that have octets) of the largest one with k / warps of the warp's maxima at or above it, to the upper 16 bits of its
+// key, which are all of a bf16 value's.  The lowest finite float if there is none above -inf.
+__device__ __forceinline__ float kth_bound(const float (&cls)[kClasses], int k, int warps, TopShared& sh) {
+  const int quota = (k + warps - 1) / warps;
+  uint32_t key[kClasses], most = 0u, prefix = 0u;
 #pragma unroll
-  for (int i = 0; i < kClasses; ++i) key[i] = order_key(cls[i]);
-  if (threadIdx.x < 16) sh.count[threadIdx.x] = 0;
-  __syncthreads();
-  for (int bit = 31; bit >= 16; --bit) {
+  for (int i = 0; i < kClasses; ++i) {
+    key[i] = order_key(cls[i]) >> 16;
+    most = max(most, key[i]);
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  for (int bit = 31 - __clz(most | 1u); bit >= 0; --bit) {
     const uint32_t trial = prefix | (1u << bit);
     int c = 0;
 #pragma unroll
     for (int i = 0; i < kClasses; ++i) c += key[i] >= trial;
-    c = __reduce_add_sync(0xffffffffu, c);
-    if ((threadIdx.x & 31) == 0 && c) atomicAdd(&sh.count[bit - 16], c);
-    __syncthreads();
-    if (sh.count[bit - 16] >= k) prefix = trial;
+    if (__reduce_add_sync(0xffffffffu, c) >= quota) prefix = trial;
   }
+  const int w = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0) sh.bound[w] = prefix <= (kInfKey >> 16) ? -FLT_MAX : key_value(prefix << 16);
   __syncthreads();
-  return prefix <= kInfKey ? -FLT_MAX : key_value(prefix);
+  float b = sh.bound[0];
+  for (int i = 1; i < warps; ++i) b = fminf(b, sh.bound[i]);
+  __syncthreads();
+  return b;
 }
 
 // The slice's exact top (at most k) into sh.chosen, by radix select on the key from its most significant byte and the
@@ -150,7 +160,8 @@ __global__ void __launch_bounds__(kTopThreads, 4) top_kernel(const T* logits, in
       v[u].load_once(body + 8 * (int64_t)(o + u * kTopThreads));
       cls[u] = v[u].max();
     }
-  float bound = kth_bound(cls, k, sh);
+  const int warps = max(1, min(kTopWarps, (sl.o1 - sl.o0 + 31) >> 5));
+  float bound = kth_bound(cls, k, warps, sh);
   MaxSum r = {-FLT_MAX, 0.f};
   float top = -FLT_MAX;
   int round = 0;
@@ -173,7 +184,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) top_kernel(const T* logits, in
 #pragma unroll
     for (int u = 0; u < kU; ++u)
       if (o + (u + kU) * kTopThreads < sl.o1) v[u].load_once(body + 8 * (int64_t)(o + (u + kU) * kTopThreads));
-    if (round == 2 && rounds > 4) bound = fmaxf(bound, kth_bound(cls, k, sh));
+    if (round == 2 && rounds > 4) bound = fmaxf(bound, kth_bound(cls, k, warps, sh));
   }
   const int te = sp.head + 8 * sp.octs + t;
   const float ends[2] = {sl.first && t < sp.head ? to_f(z[t]) : -INFINITY,
@@ -183,7 +194,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) top_kernel(const T* logits, in
   put_warp(r, c, sh.red);
   r = join_warps<kTopWarps>(c, sh.red);
   if (t == 0) sh.part = r;
-  if (rounds > 1) bound = fmaxf(bound, kth_bound(cls, k, sh));
+  if (rounds > 1) bound = fmaxf(bound, kth_bound(cls, k, warps, sh));
   const int noted = sh.n_noted;
   if (noted <= kNoted) {
     for (int i = t; i < noted; i += kTopThreads) {
@@ -232,30 +243,31 @@ __global__ void __launch_bounds__(kTopThreads, 4) top_kernel(const T* logits, in
   const float log_s = logf(r.s);
   const bool none = r.s == 0.f;  // nothing but -inf
   int total = sh.n_list;
-  int lens[16];
+  int len = 0;  // of the list of CTA `lane`
   if (n > 1) {
-    total = 0;
-    for (int i = 0; i < n; ++i) {
-      lens[i] = ld_cluster(&sh.n_list, i);
-      total += lens[i];
+    len = (t & 31) < n ? ld_cluster(&sh.n_list, t & 31) : 0;
+    total = __reduce_add_sync(0xffffffffu, len);
+    for (int q = 0; q < n; ++q) {
+      const int have = __shfl_sync(0xffffffffu, len, q);
+      for (int i = t; i < have; i += kTopThreads) sh.others[q * kTopMax + i] = ld_cluster(&sh.list[i], q);
     }
+    __syncthreads();
   }
-  for (int i = t; i < sh.n_list; i += kTopThreads) {
-    const unsigned long long me = sh.list[i];
-    int place = i;
-    if (n > 1) {
-      for (int q = 0; q < n && place < k; ++q) {
-        if (q == rank) continue;
-        int lo = 0, hi = lens[q];  // entries before lo are larger, those from hi on are not
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (ld_cluster(&sh.list[mid], q) > me)
-            lo = mid + 1;
-          else
-            hi = mid;
-        }
-        place += lo;
+  for (int i0 = 0; i0 < sh.n_list; i0 += kTopThreads) {
+    const int i = i0 + t;
+    const unsigned long long me = i < sh.n_list ? sh.list[i] : 0ull;
+    int place = i < sh.n_list ? i : k;
+    for (int q = 0; q < n && n > 1; ++q) {
+      int lo = 0, hi = __shfl_sync(0xffffffffu, len, q);
+      if (q == rank) continue;
+      while (lo < hi) {  // entries before lo are larger, those from hi on are not
+        const int mid = (lo + hi) >> 1;
+        if (sh.others[q * kTopMax + mid] > me)
+          lo = mid + 1;
+        else
+          hi = mid;
       }
+      place += lo;
     }
     if (place < k) {
       out_ids[(int64_t)row * k + place] = (int64_t)(uint32_t)~(uint32_t)me;
