@@ -7,14 +7,23 @@
 //   out = z3, or -inf where the grammar's bit of v is 0
 //
 // in fp32, rounded once to the output's type.
+//
+// A CTA owns a tile of a row's tokens and keeps their occurrences in shared
+// memory: it scans the row's whole history (from L2, where the row's other
+// tiles find it too) and counts what falls into its tile, then streams the
+// tile once.  An octet without occurrences, biases or masked tokens is only
+// converted.  Tokens with biases are left out of the stream and written
+// afterwards from their own logit, so the call can work in place and still
+// round once.
+#include <algorithm>
+#include <type_traits>
+
 #include "vocab_rows.cuh"
 
 namespace libra {
 namespace vocab {
 
-constexpr int kCtlThreads = 256;
-constexpr int kCtlTile = 8192;  // tokens of one CTA
-constexpr uint32_t kSeen = 0x80000000u;
+constexpr int kCtlThreads = 512;
 
 struct CtlArgs {
   const int* hist;          // [H, hist_w]
@@ -35,80 +44,196 @@ struct CtlArgs {
   int* err;
 };
 
-template <typename TI, typename TO>
-__global__ void __launch_bounds__(kCtlThreads) control_kernel(const TI* logits, int64_t ld, TO* out, int64_t out_ld,
-                                                              int V, CtlArgs a) {
-  extern __shared__ uint32_t ctl_smem[];
-  uint32_t* cnt = ctl_smem;                                    // [kCtlTile]
-  float* bias = reinterpret_cast<float*>(ctl_smem + kCtlTile);  // [kCtlTile]
-  const int b = blockIdx.y;
-  const int v0 = blockIdx.x * kCtlTile;
-  const int n = min(kCtlTile, V - v0);
+// Counters of a tile's tokens: occurrences behind the prompt, and a bit for tokens of the prompt.  16 bits a token while
+// the history cannot overflow them (64 KB for 32768 tokens: three CTAs on an SM), else 32.
+template <int kBits>
+struct Counts {
+  static constexpr uint32_t kSeen = 1u << (kBits - 1), kCount = kSeen - 1;
+  static constexpr int kPer = 32 / kBits;
+  uint32_t* w;
+  __device__ __forceinline__ int shift(int i) const { return kBits == 32 ? 0 : (i & 1) * 16; }
+  __device__ __forceinline__ uint32_t& word(int i) const { return w[i / kPer]; }
+  __device__ __forceinline__ void add(int i) const { atomicAdd(&word(i), 1u << shift(i)); }
+  __device__ __forceinline__ void see(int i) const { atomicOr(&word(i), kSeen << shift(i)); }
+  __device__ __forceinline__ uint32_t get(int i) const {
+    return kBits == 32 ? word(i) : (word(i) >> shift(i)) & 0xffffu;
+  }
+  // of an octet that starts at a multiple of 8; false if all are zero
+  __device__ __forceinline__ bool octet(int i, uint32_t (&c)[8]) const {
+    uint4 a = *reinterpret_cast<const uint4*>(&word(i));
+    if (kBits == 32) {
+      const uint4 b = *reinterpret_cast<const uint4*>(&word(i + 4));
+      c[0] = a.x; c[1] = a.y; c[2] = a.z; c[3] = a.w;
+      c[4] = b.x; c[5] = b.y; c[6] = b.z; c[7] = b.w;
+      return (a.x | a.y | a.z | a.w | b.x | b.y | b.z | b.w) != 0u;
+    }
+    const uint32_t v[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = (v[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+    return (a.x | a.y | a.z | a.w) != 0u;
+  }
+};
+
+template <int kBits>
+__device__ __forceinline__ float penalize(float x, uint32_t c, float rep, float pres, float freq) {
+  if (c) {
+    x = x > 0.f ? x / rep : x * rep;
+    const uint32_t k = c & Counts<kBits>::kCount;
+    if (k) x = x - freq * (float)k - pres;
+  }
+  return x;
+}
+
+// Bits of tokens j .. j + 7.
+__device__ __forceinline__ uint32_t mask_bits(const int* mask, int j, int V) {
+  const int w = j >> 5;
+  const uint32_t lo = (uint32_t)__ldg(mask + w);
+  const int s = j & 31;
+  if (s <= 24) return (lo >> s) & 0xffu;
+  const uint32_t hi = (w + 1) * 32 < V ? (uint32_t)__ldg(mask + w + 1) : 0u;
+  return __funnelshift_r(lo, hi, s) & 0xffu;
+}
+
+template <typename TI, typename TO, int kBits>
+__global__ void __launch_bounds__(kCtlThreads, 3) control_kernel(const TI* logits, int64_t ld, TO* out, int64_t out_ld,
+                                                              int V, int tiles, int tile_octs, CtlArgs a) {
+  using C = Counts<kBits>;
+  extern __shared__ __align__(16) uint32_t ctl_smem[];
+  __shared__ int twice;
+  const C cnt{ctl_smem};
+  uint32_t* biases = ctl_smem + (8 * tile_octs + 32) / C::kPer;  // a bit a token
+  const int b = blockIdx.x / tiles, tile = blockIdx.x % tiles, t = threadIdx.x;
+  const TI* z = logits + (int64_t)b * ld;
+  TO* dst = out + (int64_t)b * out_ld;
+  const RowSpan sp = row_span(z, V);
+  const int o0 = tile * tile_octs, o1 = min(sp.octs, o0 + tile_octs);
+  const bool first = tile == 0, last = tile == tiles - 1;
+  // tokens [lo, hi) of the row; token j has counter j - base, and octets start at multiples of 8 of it
+  const int base = sp.head + 8 * o0 - 8;
+  const int lo = first ? 0 : sp.head + 8 * o0, hi = last ? V : sp.head + 8 * o1;
   const float rep = a.rep ? a.rep[b] : 1.f, pres = a.pres ? a.pres[b] : 0.f, freq = a.freq ? a.freq[b] : 0.f;
   bool bad = false;
-  for (int i = threadIdx.x; i < kCtlTile; i += kCtlThreads) {
-    cnt[i] = 0u;
-    bias[i] = 0.f;
-  }
-  __syncthreads();
+  int len = 0, prompt = 0;
+  const int* h = nullptr;
   if (a.hist && (rep != 1.f || pres != 0.f || freq != 0.f)) {
     const int hr = a.hist_rows ? a.hist_rows[b] : b;
-    int len = a.hist_lens[b];
-    if (hr < 0 || hr >= a.hist_rows_n || len < 0 || len > a.hist_w) bad = true;
-    if (hr < 0 || hr >= a.hist_rows_n) len = 0;
-    len = min(len, a.hist_w);
-    const int prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
-    const int* h = a.hist + (int64_t)max(hr, 0) * a.hist_ld;
-    for (int i = threadIdx.x; i < len; i += kCtlThreads) {
-      const unsigned t = (unsigned)(h[i] - v0);
-      if (h[i] >= 0 && t < (unsigned)n) {
-        if (i < prompt)
-          atomicOr(&cnt[t], kSeen);
-        else
-          atomicAdd(&cnt[t], 1u);
-      }
-    }
+    len = a.hist_lens[b];
+    const bool in = hr >= 0 && hr < a.hist_rows_n;
+    bad = !in || len < 0 || len > a.hist_w;
+    len = in ? min(len, a.hist_w) : 0;
+    prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
+    h = a.hist + (int64_t)(in ? hr : 0) * a.hist_ld;
   }
+  int b0 = 0, b1 = 0;
   if (a.bias_offs) {
-    int lo = a.bias_offs[b], hi = a.bias_offs[b + 1];
-    if (lo < 0 || hi < lo || hi > a.bias_n) {
+    b0 = a.bias_offs[b];
+    b1 = a.bias_offs[b + 1];
+    if (b0 < 0 || b1 < b0 || b1 > a.bias_n) {
       bad = true;
-      lo = hi = 0;
-    }
-    // a token's entries are summed in list order by the thread of its first entry
-    for (int e = lo + threadIdx.x; e < hi; e += kCtlThreads) {
-      const int id = a.bias_ids[e];
-      if (id < v0 || id >= v0 + n) continue;
-      bool first = true;
-      for (int j = lo; j < e && first; ++j) first = a.bias_ids[j] != id;
-      if (!first) continue;
-      float s = 0.f;
-      for (int j = e; j < hi; ++j)
-        if (a.bias_ids[j] == id) s += a.bias_vals[j];
-      bias[id - v0] = s;
+      b0 = b1 = 0;
     }
   }
   const int* mask = nullptr;
   if (a.mask) {
     const int mr = a.mask_rows ? a.mask_rows[b] : b;
-    if (mr >= a.mask_n) bad = true;
+    bad = bad || mr >= a.mask_n;
     if (mr >= 0 && mr < a.mask_n) mask = a.mask + (int64_t)mr * a.mask_ld;
   }
-  if (bad && a.err && threadIdx.x == 0) atomicCAS(a.err, 0, kBadArgument);
-  __syncthreads();
-  const TI* z = logits + (int64_t)b * ld + v0;
-  TO* o = out + (int64_t)b * out_ld + v0;
-  for (int i = threadIdx.x; i < n; i += kCtlThreads) {
-    float x = to_f(z[i]);
-    const uint32_t c = cnt[i];
-    if (c) {
-      x = x > 0.f ? x / rep : x * rep;
-      const uint32_t k = c & ~kSeen;
-      if (k) x = x - freq * (float)k - pres;
+  if (bad && t == 0) atomicCAS(a.err, 0, kBadArgument);
+  const bool counted = len > 0, biased = b1 > b0;
+  if (counted || biased) {
+    const int quads = counted ? (hi - base + C::kPer * 4 - 1) / (C::kPer * 4) : 0;
+    for (int i = t; i < quads; i += kCtlThreads) reinterpret_cast<uint4*>(ctl_smem)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = t; i < (hi - base + 31) / 32 && biased; i += kCtlThreads) biases[i] = 0u;
+    if (t == 0) twice = 0;
+    __syncthreads();
+#pragma unroll 8
+    for (int i = t; i < len; i += kCtlThreads) {
+      const int id = h[i];
+      if (id >= lo && id < hi) {
+        if (i < prompt)
+          cnt.see(id - base);
+        else
+          cnt.add(id - base);
+      }
     }
-    x += bias[i];
-    if (mask && !((mask[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1)) x = -INFINITY;
-    from_f(o + i, x);
+    for (int e = b0 + t; e < b1; e += kCtlThreads) {
+      const int id = a.bias_ids[e];
+      if (id < lo || id >= hi) continue;
+      const int i = id - base;
+      if ((atomicOr(&biases[i >> 5], 1u << (i & 31)) >> (i & 31)) & 1u) twice = 1;
+    }
+    __syncthreads();
+  } else if (!mask && (const void*)z == (const void*)dst) {
+    return;  // in place, and nothing to do
+  }
+  // head and tail of the row: a token a thread
+  if ((first && t < sp.head) || (last && t >= 32 && t - 32 < sp.tail)) {
+    const int j = t < 32 ? t : sp.head + 8 * sp.octs + t - 32;
+    const uint32_t c = counted ? cnt.get(j - base) : 0u;
+    float x = penalize<kBits>(to_f(z[j]), c, rep, pres, freq);
+    if (mask && !((mask[j >> 5] >> (j & 31)) & 1)) x = -INFINITY;
+    if (!biased || !((biases[(j - base) >> 5] >> ((j - base) & 31)) & 1)) from_f(dst + j, x);
+  }
+  const uint8_t* bias_bytes = reinterpret_cast<const uint8_t*>(biases) + 1;
+  const TI* body = z + sp.head;
+  TO* obody = dst + sp.head;
+  const bool vec = aligned16(obody);
+  constexpr int kU = sizeof(TI) == 2 ? 4 : 2;
+  for (int o = o0 + t; o < o1; o += kU * kCtlThreads) {
+    Oct<TI> v[kU];
+    uint32_t allow[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int p = o + u * kCtlThreads;
+      allow[u] = 0xffu;
+      if (p < o1) {
+        if (mask) allow[u] = mask_bits(mask, sp.head + 8 * p, V);
+        if (allow[u]) v[u].load_once(body + 8 * (int64_t)p);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int p = o + u * kCtlThreads;
+      if (p >= o1) continue;
+      float f[8];
+      v[u].get(f);
+      uint32_t c[8];
+      if (counted && cnt.octet(8 * (p - o0) + 8, c)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = penalize<kBits>(f[e], c[e], rep, pres, freq);
+      }
+      const uint32_t skip = biased ? bias_bytes[p - o0] : 0u;
+      if (allow[u] != 0xffu) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!((allow[u] >> e) & 1u)) f[e] = -INFINITY;
+      }
+      TO* at = obody + 8 * (int64_t)p;
+      if (vec && !skip) {
+        store_oct(at, f);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!((skip >> e) & 1u)) from_f(at + e, f[e]);
+      }
+    }
+  }
+  // biased tokens, from their own logits; one listed twice is written by its first entry, the sum in list order
+  for (int e = b0 + t; e < b1; e += kCtlThreads) {
+    const int id = a.bias_ids[e];
+    if (id < lo || id >= hi) continue;
+    float s = a.bias_vals[e];
+    if (twice) {
+      bool again = false;
+      for (int i = b0; i < e && !again; ++i) again = a.bias_ids[i] == id;
+      if (again) continue;
+      for (int i = e + 1; i < b1; ++i)
+        if (a.bias_ids[i] == id) s += a.bias_vals[i];
+    }
+    float x = penalize<kBits>(to_f(z[id]), counted ? cnt.get(id - base) : 0u, rep, pres, freq) + s;
+    if (mask && !((mask[id >> 5] >> (id & 31)) & 1)) x = -INFINITY;
+    from_f(dst + id, x);
   }
 }
 
@@ -177,26 +302,34 @@ void control_logits(torch::Tensor logits, c10::optional<torch::Tensor> history,
     a.mask_rows = (const int*)opt(mask_rows, at::kInt, B, "mask_rows");
   }
   LIBRA_CHECK(err.device() == logits.device() && err.scalar_type() == at::kInt, "control_logits: error word");
-  LIBRA_CHECK(B < 65536, "control_logits: at most 65535 rows");
   if (B == 0 || V == 0) return;
   a.err = err.data_ptr<int>();
   const c10::cuda::CUDAGuard guard(logits.device());
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  const dim3 grid((V + kCtlTile - 1) / kCtlTile, B);
-  const size_t smem = kCtlTile * 8;
-  auto go = [&](auto kern, auto* in, auto* o) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    LIBRA_CHECK(e == cudaSuccess, "control_logits: %s", cudaGetErrorString(e));
-    kern<<<grid, kCtlThreads, smem, st>>>(in, logits.stride(0), o, out.stride(0), V, a);
-    LIBRA_LAUNCH_CHECK();
+  // tiles of 32768 tokens, since every tile scans the history once (256 x 151936 fp32 with 16384 tokens of history: 82 us,
+  // 89 us with tiles of 16384, 118 us with 256 threads), smaller ones while that leaves SMs without three CTAs
+  int tile = 32768;
+  while (tile > 2048 && (int64_t)B * ((V + tile - 1) / tile) < 3 * 148) tile /= 2;
+  const int tiles = std::max(1, (V / 8 + tile / 8 - 1) / (tile / 8));
+  const bool wide = a.hist && a.hist_w >= (1 << 15);  // 16-bit counters hold 2^15 - 1 occurrences
+  const size_t smem = (size_t)(tile + 32) * (wide ? 4 : 2) + (tile + 32) / 8;
+  auto go = [&](auto* in, auto* o) {
+    using I = std::remove_const_t<std::remove_pointer_t<decltype(in)>>;
+    using O = std::remove_pointer_t<decltype(o)>;
+    if (wide)
+      launch_rows(control_kernel<I, O, 32>, (int64_t)B * tiles, kCtlThreads, smem, 1, false, st, in, logits.stride(0),
+                  o, out.stride(0), V, tiles, tile / 8, a);
+    else
+      launch_rows(control_kernel<I, O, 16>, (int64_t)B * tiles, kCtlThreads, smem, 1, false, st, in, logits.stride(0),
+                  o, out.stride(0), V, tiles, tile / 8, a);
   };
   using bf = __nv_bfloat16;
   const bool fi = logits.scalar_type() == at::kFloat, fo = out.scalar_type() == at::kFloat;
   void *pi = logits.data_ptr(), *po = out.data_ptr();
-  if (fi && fo) go(control_kernel<float, float>, (const float*)pi, (float*)po);
-  if (fi && !fo) go(control_kernel<float, bf>, (const float*)pi, (bf*)po);
-  if (!fi && fo) go(control_kernel<bf, float>, (const bf*)pi, (float*)po);
-  if (!fi && !fo) go(control_kernel<bf, bf>, (const bf*)pi, (bf*)po);
+  if (fi && fo) go((const float*)pi, (float*)po);
+  if (fi && !fo) go((const float*)pi, (bf*)po);
+  if (!fi && fo) go((const bf*)pi, (float*)po);
+  if (!fi && !fo) go((const bf*)pi, (bf*)po);
 }
 
 }  // namespace vocab
