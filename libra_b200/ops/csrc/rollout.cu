@@ -25,6 +25,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <cfloat>
+
 #include "common.cuh"
 #include "tmap.cuh"
 
@@ -355,7 +357,8 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(
   const uint64_t seed = (uint64_t)seeds[row];
   const uint64_t pos = (uint64_t)positions[row];
   const uint2 key = make_uint2((uint32_t)seed, (uint32_t)(seed >> 32));
-  SampleAcc a{-INFINITY, 0.f, -INFINITY, 0x7fffffff, 0.f};
+  // the running maximum starts finite: a masked (-inf) logit then adds exp(-inf) = 0, not exp(-inf + inf)
+  SampleAcc a{-FLT_MAX, 0.f, -INFINITY, 0x7fffffff, 0.f};
   const int V4 = V / 4;
   for (int i = threadIdx.x; i < V4; i += kSampleThreads) {
     float v[4];
@@ -597,7 +600,7 @@ __global__ void __launch_bounds__(kFiltThreads) sample_filtered_kernel(
   const float inv = greedy ? 1.f : 1.f / Tm;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // pass 1: max and sum of exp of the scaled logits
-  float m = -INFINITY, s = 0.f;
+  float m = -FLT_MAX, s = 0.f;  // finite, see sample_kernel
   for (int j = threadIdx.x; j < V; j += kFiltThreads) {
     const float v = load1(x + j) * inv;
     if (v > m) {
@@ -682,7 +685,7 @@ __global__ void __launch_bounds__(kFiltThreads) sample_filtered_kernel(
     SampleAcc t = wacc[0];
     for (int w = 1; w < kFiltThreads / 32; ++w)
       if (wacc[w].best > t.best || (wacc[w].best == t.best && wacc[w].idx < t.idx)) t = wacc[w];
-    const bool ok = t.idx >= 0 && t.idx < V;
+    const bool ok = t.idx >= 0 && t.idx < V && t.val > -INFINITY;  // not a row of nothing but masked logits
     out_tok[row] = ok ? t.idx : 0;
     out_lp[row] = ok ? t.val - m - logf(s) : -INFINITY;
   }
