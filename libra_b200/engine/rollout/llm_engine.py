@@ -22,16 +22,18 @@ from __future__ import annotations
 
 import asyncio
 import itertools
+import math
 import threading
 import time
 import uuid
 from collections import deque
 from dataclasses import dataclass, field
-from typing import Deque, Dict, List, Optional
+from typing import Deque, Dict, List, Optional, Tuple
 
 import torch
 
 from libra_b200 import ops
+from libra_b200.engine.rollout.controls import LogitControls
 from libra_b200.engine.rollout.kv_cache import PagedKVCache
 from libra_b200.engine.rollout.runner import InferenceRunner, WorkItem
 from libra_b200.engine.rollout.sampler import SamplingParams, sample
@@ -47,6 +49,8 @@ class GenerationResult:
     output_logprobs: List[float]
     finish_reason: str
     metrics: Dict[str, float] = field(default_factory=dict)
+    # (token, logprob) pairs of every output position, most likely first (``SamplingParams.top_logprobs``)
+    output_top_logprobs: List[List[Tuple[int, float]]] = field(default_factory=list)
 
 
 @dataclass
@@ -56,6 +60,7 @@ class _Request:
     params: SamplingParams
     out: List[int] = field(default_factory=list)
     logprobs: List[float] = field(default_factory=list)
+    top: List[List[Tuple[int, float]]] = field(default_factory=list)
     cached: int = 0           # tokens whose KV is in the cache
     future: Optional[asyncio.Future] = None
     loop: Optional[asyncio.AbstractEventLoop] = None
@@ -140,6 +145,7 @@ class LLMEngine:
         self._kv_ops: List[tuple] = []  # KV-cache calls the followers must replay, in order
         self.tp_reload_hook = None  # follower side: callable(request) -> (params, version)
         self.block_size = block_size
+        self._controls = LogitControls(cfg.vocab_size, max_running, self.device)
         self._graphs = None          # DecodeGraphs, built at the first pure-decode step
         self._graphs_ok = (self.device.type == "cuda" and tp_size == 1 and not cfg.is_moe and cfg.head_dim == 128)
         self._seed_rng = torch.Generator().manual_seed(int(uuid.uuid4().int & 0x7FFFFFFF))
@@ -197,9 +203,18 @@ class LLMEngine:
                 return
 
     # ------------------------------------------------------------------ request API
+    def check_params(self, params: SamplingParams) -> None:
+        """Raise ValueError for sampling arguments that this engine's vocabulary rules out."""
+        if params.allowed_token_ids is not None and not any(
+                0 <= int(t) < self.cfg.vocab_size for t in params.allowed_token_ids):
+            raise ValueError("allowed_token_ids: none of them is in the vocabulary")
+        if params.top_logprobs > self.cfg.vocab_size:
+            raise ValueError(f"top_logprobs: the vocabulary has {self.cfg.vocab_size} tokens")
+
     def add_request(self, prompt_tokens: List[int], params: SamplingParams, request_id: str = "",
                     future=None, loop=None, callback=None) -> str:
         rid = request_id or f"{self.instance_id}-{next(self._ids)}"
+        self.check_params(params)
         gen = None
         if params.seed is not None:
             gen = torch.Generator(device=self.device)
@@ -271,6 +286,7 @@ class LLMEngine:
             self.waiting.clear()
         for r in reqs:
             self._kv_call("free", r.request_id)
+            self._controls.release(r.request_id)
             if r.future is not None and r.loop is not None:
                 r.loop.call_soon_threadsafe(lambda f=r.future: f.done() or f.set_exception(RuntimeError(str(exc))))
 
@@ -499,16 +515,25 @@ class LLMEngine:
         admitted = self._admit()
         decode = [r for r in self.running if r.cached == r.n_tokens - 1]
         if (not admitted and decode and self._graphs_ok and len(decode) <= self.max_running
-                and all(r.params.top_p >= 1.0 and r.params.top_k <= 0 for r in decode)
+                and all(r.params.top_p >= 1.0 and r.params.top_k <= 0 and not r.params.controlled
+                        and not r.params.top_logprobs for r in decode)
                 and self._graph_runner() is not None):
             return self._decode_step_graph(decode, t0)
-        batch = admitted + decode
+        batch = self._prepare_controls(admitted + decode)
         if not batch:
             return 0
+        alive = {id(r) for r in batch}
+        admitted = [r for r in admitted if id(r) in alive]
+        decode = [r for r in decode if id(r) in alive]
         items = [WorkItem(r.request_id, r.tokens, r.cached) for r in batch]
         self._publish(items)
         with nvtx.nvtx_range("prefill" if admitted else "decode"):
             logits = self.runner.step(items)
+        sent = self._controls.h2d
+        controlled = any(r.params.controlled for r in batch)
+        logits = self._controls.apply(logits, batch) if controlled else logits.contiguous()
+        n_top = max(r.params.top_logprobs for r in batch)
+        top = None
         if logits.device.type == "cuda":
             # the fused samplers (same Philox stream as the captured decode steps); their per-request inputs
             # go up through pinned staging, so the host does not wait for the step's kernels here
@@ -520,19 +545,28 @@ class LLMEngine:
             pos = _to_device([r.n_tokens - 1 for r in batch], torch.long, dev)
             toks = torch.empty(len(batch), dtype=torch.long, device=dev)
             lps = torch.empty(len(batch), dtype=torch.float32, device=dev)
+            if n_top:  # before the sampler, which clears fp32 logits
+                top = ops.top_logprobs(logits, n_top, temps)
             if all(r.params.top_p >= 1.0 and r.params.top_k <= 0 for r in batch):
-                ops.sample_tokens(logits.contiguous(), temps, seeds, pos, toks, lps)
+                ops.sample_tokens(logits, temps, seeds, pos, toks, lps)
             else:
                 top_p = _to_device([r.params.top_p for r in batch], torch.float32, dev)
                 top_k = _to_device([r.params.top_k for r in batch], torch.long, dev)
-                ops.sample_tokens_filtered(logits.contiguous(), temps, top_p, top_k, seeds, pos, toks, lps)
+                ops.sample_tokens_filtered(logits, temps, top_p, top_k, seeds, pos, toks, lps)
         else:
             temps = torch.tensor([r.params.temperature for r in batch], dtype=torch.float32)
             top_p = torch.tensor([r.params.top_p for r in batch], device=logits.device, dtype=torch.float32)
             top_k = torch.tensor([r.params.top_k for r in batch], device=logits.device, dtype=torch.long)
             gens = [r.generator for r in batch] if any(r.generator is not None for r in batch) else None
+            if n_top:
+                top = ops.top_logprobs(logits, n_top, temps)
             toks, lps = sample(logits, temps, top_p, top_k, gens)
         toks, lps = toks.tolist(), lps.tolist()
+        if top is not None:
+            top = [[(t, v) for t, v in zip(i, p) if v > -math.inf]  # not the tokens that a mask excludes
+                   for i, p in zip(top[0].tolist(), top[1].tolist())]
+            self._eager_io["d2h"] += 12 * n_top * len(batch)
+        self._eager_io["h2d"] += self._controls.h2d - sent
         n_new = sum(r.n_tokens - r.cached for r in batch)
         self._eager_io["h2d"] += 28 * n_new + 32 * len(batch)  # tokens, positions, slots, rows, sampler inputs
         self._eager_io["d2h"] += 12 * len(batch)
@@ -540,10 +574,12 @@ class LLMEngine:
         self.stats["prefill_tokens"] += sum(len(r.tokens) - r.cached for r in admitted)
         self.stats["decode_tokens"] += len(decode)
         still = []
-        for r, t, lp in zip(batch, toks, lps):
+        for n, (r, t, lp) in enumerate(zip(batch, toks, lps)):
             r.cached = len(r.tokens)
             r.out.append(int(t))
             r.logprobs.append(float(lp))
+            if r.params.top_logprobs:
+                r.top.append(top[n][:r.params.top_logprobs])
             if not r.t_first:
                 r.t_first = now
             reason = self._stop_reason(r, int(t))
@@ -557,6 +593,17 @@ class LLMEngine:
         self.stats["busy_s"] += time.perf_counter() - t0
         return len(batch)
 
+    def _prepare_controls(self, batch: List[_Request]) -> List[_Request]:
+        """The masks of the batch's next tokens; requests whose grammar allows none finish here."""
+        ended = {id(r): reason for r in batch if r.params.controlled and (reason := self._controls.prepare(r))}
+        if not ended:
+            return batch
+        for r in batch:
+            if id(r) in ended:
+                self._finish(r, ended[id(r)])
+        self.running = [r for r in self.running if id(r) not in ended]
+        return [r for r in batch if id(r) not in ended]
+
     def _stop_reason(self, r: _Request, tok: int) -> str:
         if tok in r.params.stop_token_ids or (self.eos_token_id is not None and tok == self.eos_token_id):
             return "stop"
@@ -568,10 +615,11 @@ class LLMEngine:
 
     def _finish(self, r: _Request, reason: str) -> None:
         self._kv_call("free", r.request_id)
+        self._controls.release(r.request_id)
         self.stats["finished"] += 1
         res = GenerationResult(r.request_id, r.prompt, list(r.out), list(r.logprobs), reason,
                                {"ttft_s": (r.t_first - r.t_arrive) if r.t_first else 0.0,
-                                "latency_s": time.perf_counter() - r.t_arrive, "cached_tokens": 0})
+                                "latency_s": time.perf_counter() - r.t_arrive, "cached_tokens": 0}, list(r.top))
         if r.callback is not None:
             r.callback(res)
         if r.future is not None and r.loop is not None:

@@ -1,11 +1,16 @@
 """Token sampling: temperature, top-k and top-p (nucleus), with the sampled
 token's logprob under the temperature-scaled distribution (what the rollout
-returns as ``token_logprobs``; reference ``engine/rollout_engine.py:255``)."""
+returns as ``token_logprobs``; reference ``engine/rollout_engine.py:255``).
+
+Penalties, biases, allowed tokens and a grammar change the logits before all
+of that (``ops.control_logits``), so a controlled request's logprobs, top
+logprobs included, are those of the distribution it was sampled from."""
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
-from typing import List, Optional
+from typing import Any, Dict, List, Optional
 
 import torch
 
@@ -19,6 +24,52 @@ class SamplingParams:
     stop_token_ids: List[int] = field(default_factory=list)
     seed: Optional[int] = None
     logprobs: bool = True
+    repetition_penalty: float = 1.0     # divides positive logits of tokens already present, multiplies others
+    presence_penalty: float = 0.0       # subtracted once from tokens of the output so far
+    frequency_penalty: float = 0.0      # and once per occurrence there
+    logit_bias: Optional[Dict[int, float]] = None
+    allowed_token_ids: Optional[List[int]] = None
+    grammar: Optional[Any] = None       # engine.rollout.controls.Grammar
+    top_logprobs: int = 0               # most likely tokens to report beside each sampled one
+
+    def __post_init__(self):
+        if not (self.repetition_penalty > 0 and math.isfinite(self.repetition_penalty)):
+            raise ValueError(f"repetition_penalty must be above 0, got {self.repetition_penalty}")
+        for name in ("presence_penalty", "frequency_penalty"):
+            if not math.isfinite(getattr(self, name)):
+                raise ValueError(f"{name} must be finite, got {getattr(self, name)}")
+        if self.logit_bias:
+            self.logit_bias = {int(k): float(v) for k, v in self.logit_bias.items()}
+            if not all(math.isfinite(v) and 0 <= k < 2 ** 31 for k, v in self.logit_bias.items()):
+                raise ValueError("logit_bias maps token ids to finite numbers")
+        if self.allowed_token_ids is not None and not len(self.allowed_token_ids):
+            raise ValueError("allowed_token_ids must not be empty")
+        if not 0 <= int(self.top_logprobs) <= 256:
+            raise ValueError(f"top_logprobs must lie in [0, 256], got {self.top_logprobs}")
+
+    @property
+    def penalized(self) -> bool:
+        return self.repetition_penalty != 1.0 or self.presence_penalty != 0.0 or self.frequency_penalty != 0.0
+
+    @property
+    def controlled(self) -> bool:
+        return (self.penalized or bool(self.logit_bias) or self.allowed_token_ids is not None
+                or self.grammar is not None)
+
+
+# what a caller may pass through the rollout engines and the HTTP route besides the named arguments
+EXTRA_SAMPLING_KEYS = ("repetition_penalty", "presence_penalty", "frequency_penalty", "logit_bias",
+                       "allowed_token_ids", "top_logprobs")
+
+
+def extra_sampling(kw: Dict[str, Any]) -> Dict[str, Any]:
+    """The given ones of ``EXTRA_SAMPLING_KEYS``, as ``SamplingParams`` takes them."""
+    cast = {"logit_bias": lambda v: {int(k): float(x) for k, x in v.items()},
+            "allowed_token_ids": lambda v: [int(t) for t in v], "top_logprobs": int}
+    try:
+        return {k: cast.get(k, float)(kw[k]) for k in EXTRA_SAMPLING_KEYS if kw.get(k) is not None}
+    except (TypeError, AttributeError) as exc:
+        raise ValueError(f"bad sampling argument: {exc}") from exc
 
 
 def sample(logits: torch.Tensor, temperature: torch.Tensor, top_p: torch.Tensor, top_k: torch.Tensor,

@@ -23,7 +23,7 @@ import logging
 import time
 from typing import Any, Dict, List, Optional, Sequence, Union
 
-from libra_b200.engine.rollout.sampler import SamplingParams
+from libra_b200.engine.rollout.sampler import SamplingParams, extra_sampling
 
 log = logging.getLogger(__name__)
 Prompt = Union[str, Sequence[int]]
@@ -43,7 +43,8 @@ class LocalRolloutEngine:
 
     async def generate(self, prompt: Prompt, max_new_tokens: int = 1024, temperature: float = 1.0,
                        top_p: float = 1.0, n: int = 1, input_tokens: int = 0, seed: Optional[int] = None,
-                       top_k: int = -1, stop_token_ids: Optional[List[int]] = None, **_) -> Dict[str, Any]:
+                       top_k: int = -1, stop_token_ids: Optional[List[int]] = None, grammar=None,
+                       **kw) -> Dict[str, Any]:
         ids = _ids(self.tokenizer, prompt)
         stops = list(stop_token_ids or [])
         eos = getattr(self.tokenizer, "eos_token_id", None)
@@ -51,8 +52,8 @@ class LocalRolloutEngine:
             stops.append(int(eos))
         res = await self.engine.generate(ids, SamplingParams(max_tokens=max_new_tokens, temperature=temperature,
                                                              top_p=top_p, top_k=top_k, stop_token_ids=stops,
-                                                             seed=seed))
-        return {"text": self.tokenizer.decode(res.output_tokens), "tokens": [str(t) for t in res.output_tokens],
+                                                             seed=seed, grammar=grammar, **extra_sampling(kw)))
+        return {**({"top_logprobs": res.output_top_logprobs} if kw.get("top_logprobs") else {}),"text": self.tokenizer.decode(res.output_tokens), "tokens": [str(t) for t in res.output_tokens],
                 "token_ids": list(res.output_tokens), "prompt_token_ids": ids, "logprobs": list(res.output_logprobs),
                 "finish_reason": res.finish_reason, "metrics": res.metrics, "policy_version": self.engine.version}
 
@@ -96,9 +97,12 @@ class HTTPRolloutEngine:
                    "max_tokens": max_new_tokens, "temperature": temperature, "top_p": top_p, "n": n, "logprobs": 1}
         if seed is not None:
             payload["seed"] = int(seed)
+        if kw.get("grammar") is not None:
+            raise ValueError("a grammar object needs an in-process rollout engine")
         for k in ("top_k", "stop_token_ids"):
             if kw.get(k) is not None:
                 payload[k] = kw[k]
+        payload.update(extra_sampling(kw))
         session = await self._client()
         async with session.post(self.completions_url, json=payload) as resp:
             if resp.status != 200:
@@ -116,7 +120,9 @@ class HTTPRolloutEngine:
         lp = c.get("logprobs") or {}
         if not isinstance(lp, dict):
             lp = {}
-        return {"text": c.get("text", "") or "", "tokens": lp.get("tokens") or [],
+        top = lp.get("top_logprobs")
+        return {**({"top_logprobs": [[(int(t), float(v)) for t, v in row] for row in top]} if top else {}),
+                "text": c.get("text", "") or "", "tokens": lp.get("tokens") or [],
                 "token_ids": c.get("token_ids") or [], "prompt_token_ids": c.get("prompt_token_ids") or [],
                 "logprobs": lp.get("token_logprobs") or [], "finish_reason": c.get("finish_reason", "length")}
 

@@ -4,9 +4,13 @@ Routes (the reference serves the same ones from a patched vLLM API server,
 ``scripts/vllm_hot_reload_api_server.py:41-96``):
 
 * ``POST /v1/completions`` - ``prompt`` as text or token ids, ``max_tokens``,
-  ``temperature``, ``top_p``, ``top_k``, ``seed``, ``logprobs``; the choice
+  ``temperature``, ``top_p``, ``top_k``, ``seed``, ``logprobs``,
+  ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``,
+  ``logit_bias``, ``allowed_token_ids``, ``top_logprobs``; the choice
   carries ``text``, ``token_ids``, ``prompt_token_ids``,
-  ``logprobs.tokens/token_logprobs`` and ``finish_reason``.
+  ``logprobs.tokens/token_logprobs`` (and ``logprobs.top_logprobs``, a list of
+  [token id, logprob] pairs per position, when asked for) and
+  ``finish_reason``.  A bad sampling argument answers 400.
 * ``GET /health``, ``GET /v1/models``, ``GET /metrics``.
 * ``POST /reload_weights`` ``{"checkpoint_path": dir, "version": v}`` - load a
   checkpoint written by the trainer (disk weight sync), under a lock, then drop
@@ -36,7 +40,7 @@ from typing import Any, Dict, Optional
 
 from aiohttp import web
 
-from libra_b200.engine.rollout.sampler import SamplingParams
+from libra_b200.engine.rollout.sampler import SamplingParams, extra_sampling
 
 
 def build_app(engine, tokenizer, model_name: str = "libra", weight_loader=None) -> web.Application:
@@ -64,9 +68,14 @@ def build_app(engine, tokenizer, model_name: str = "libra", weight_loader=None) 
         eos = getattr(tokenizer, "eos_token_id", None)
         if eos is not None and eos not in stops and not body.get("ignore_eos", False):
             stops.append(int(eos))
-        params = SamplingParams(max_tokens=int(body.get("max_tokens", 16)), temperature=float(body.get("temperature", 1.0)),
-                                top_p=float(body.get("top_p", 1.0)), top_k=int(body.get("top_k", -1)),
-                                stop_token_ids=stops, seed=body.get("seed"))
+        try:
+            params = SamplingParams(max_tokens=int(body.get("max_tokens", 16)),
+                                    temperature=float(body.get("temperature", 1.0)),
+                                    top_p=float(body.get("top_p", 1.0)), top_k=int(body.get("top_k", -1)),
+                                    stop_token_ids=stops, seed=body.get("seed"), **extra_sampling(body))
+            engine.check_params(params)
+        except ValueError as exc:
+            return web.json_response({"error": str(exc)}, status=400)
         n = max(1, int(body.get("n", 1)))
         results = await asyncio.gather(*(engine.generate(ids, params) for _ in range(n)))
         choices = []
@@ -75,6 +84,8 @@ def build_app(engine, tokenizer, model_name: str = "libra", weight_loader=None) 
                       "prompt_token_ids": ids, "finish_reason": r.finish_reason}
             if body.get("logprobs") is not None:
                 choice["logprobs"] = {"tokens": [str(t) for t in r.output_tokens], "token_logprobs": r.output_logprobs}
+            if params.top_logprobs:
+                choice.setdefault("logprobs", {})["top_logprobs"] = r.output_top_logprobs
             choices.append(choice)
         comp = sum(len(r.output_tokens) for r in results)
         return web.json_response({"id": f"cmpl-{uuid.uuid4().hex[:12]}", "object": "text_completion",
