@@ -545,6 +545,9 @@ class AsyncRLConfig:
     micro_batch_size: int = 4
     kl_coef: float = 0.001
     clip_epsilon: float = 0.2
+    # weight and divergence (forward, reverse, js) of the distillation loss for trajectories with a teacher's top logprobs
+    distill_coef: float = 0.0
+    distill_divergence: str = "forward"
     gamma: float = 1.0
     max_new_tokens: int = 1024
     r2e_max_turns: int = 3

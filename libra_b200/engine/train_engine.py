@@ -81,7 +81,8 @@ class B200TrainEngine:
                  max_grad_norm: float = 1.0, tp_size: int = 1, model_path: str = "",
                  max_tokens_per_micro_batch: int = 16384, max_tokens_per_recompute_batch: int = 65536,
                  ep_size: int = 1, sequence_parallel: bool = False, precision_aware_optimizer: bool = False,
-                 optimizer_cpu_offload: bool = False, optimizer_offload_fraction: float = 0.0, pp_size: int = 1):
+                 optimizer_cpu_offload: bool = False, optimizer_offload_fraction: float = 0.0, pp_size: int = 1,
+                 distill_coef: float = 0.0, distill_divergence: str = "forward"):
         self.cfg: Qwen3Config = get_config(model)
         self.model_path = model_path
         self.optim = OptimConfig(lr=learning_rate, max_grad_norm=max_grad_norm)
@@ -98,6 +99,15 @@ class B200TrainEngine:
         self.tp_size = tp_size
         # pipeline parallelism: this rank holds a contiguous range of layers (1F1B over NCCL p2p)
         self.pp_size = max(1, int(pp_size))
+        # weight of the distillation loss in grpo_update, for trajectories that carry a teacher's top logprobs
+        # ("teacher_ids" / "teacher_logprobs", see score_teacher)
+        self.distill_coef, self.distill_divergence = float(distill_coef), str(distill_divergence)
+        if self.distill_divergence not in ("forward", "reverse", "js"):
+            raise ValueError(f"distill_divergence must be forward, reverse or js, got {distill_divergence!r}")
+        if self.distill_coef < 0.0:
+            raise ValueError(f"distill_coef must not be negative, got {distill_coef}")
+        if self.distill_coef > 0.0:
+            self._check_whole_vocabulary("distill_coef")
         self.sequence_parallel = bool(sequence_parallel) and tp_size > 1
         # precision-aware optimizer (MCore use_precision_aware_optimizer): Adam moments stored in bf16
         # (updated in fp32 inside the kernel), fp32 master weights; 8 instead of 12 bytes per parameter
@@ -552,7 +562,39 @@ class B200TrainEngine:
                              dtype=torch.float32)
             extra["w"] = w.index_select(0, sidx)
             extra["rewards"] = torch.tensor([float(t["rewards"].reshape(-1)[0]) for t in trajectories])
+        elif traj_weights is not None:
+            extra["w"] = torch.tensor(traj_weights, dtype=torch.float32).index_select(0, batch.seq_index.long())
+        if ((self.distill_coef > 0.0 or not with_old_logprobs) and traj_weights is not None
+                and any("teacher_ids" in t for t in trajectories)):
+            extra["teacher_ids"], extra["teacher_logprobs"] = self._teacher_tables(trajectories, batch)
         return {"batch": batch, **extra}
+
+    def _check_whole_vocabulary(self, what: str) -> None:
+        if self.tp_size > 1 or self.pp_size > 1:
+            raise ValueError(f"{what} needs tp_size=1 and pp_size=1 (the whole LM head on every rank)")
+
+    def _teacher_tables(self, trajectories: List[Dict[str, Any]], batch: PackedBatch):
+        """Teacher tables [actions, K] of a packed batch; trajectories without one get empty slots."""
+        k = max(t["teacher_ids"].shape[-1] for t in trajectories if "teacher_ids" in t)
+        ids, lps = [], []
+        for t in trajectories:
+            n = int(t["input_ids"].numel())
+            i = torch.full((n, k), -1, dtype=torch.long)
+            p = torch.zeros(n, k)
+            if "teacher_ids" in t:
+                src = t["teacher_ids"].reshape(-1, t["teacher_ids"].shape[-1])
+                if src.shape[0] != n or t["teacher_logprobs"].numel() != src.numel():
+                    raise ValueError(f"teacher tables of {src.shape[0]} positions for {n} tokens")
+                i[:, :src.shape[1]] = src
+                p[:, :src.shape[1]] = t["teacher_logprobs"].reshape(src.shape).float()
+            ids.append(i)
+            lps.append(p)
+        pad = batch.num_tokens - sum(t.shape[0] for t in ids)
+        if pad > 0:
+            ids.append(torch.full((pad, k), -1, dtype=torch.long))
+            lps.append(torch.zeros(pad, k))
+        rows = batch.action_rows + 1  # the table of an action token stands at its own position
+        return torch.cat(ids).index_select(0, rows), torch.cat(lps).index_select(0, rows)
 
     def loss_weights(self, trajectories: List[Dict[str, Any]]) -> List[float]:
         """Per-trajectory token weight reproducing the reference loss aggregation:
@@ -659,6 +701,66 @@ class B200TrainEngine:
                 updated[rows[sel] - cu[i]] = lp[sel]
                 traj["logprobs"] = updated.view(1, L)
 
+    @torch.no_grad()
+    def score_teacher(self, trajectories: List[Dict[str, Any]], k: int) -> None:
+        """Write the k most likely tokens of this engine's policy at every action token into the trajectories
+        ("teacher_ids" int64 and "teacher_logprobs" fp32 [1, L, k], host tensors; empty slots elsewhere), for
+        another engine's ``distill_update`` or ``grpo_update``."""
+        self._check_whole_vocabulary("score_teacher")
+        results = []
+        for chunk, host in self.prepare_recompute(trajectories):
+            ids, lps = self.model.action_top_logprobs(self.to_device(host)["batch"], k, self.temperature)
+            results.append((chunk, host["batch"], ids.to("cpu", non_blocking=True), lps.to("cpu", non_blocking=True)))
+            self.io_bytes["d2h"] += 12 * ids.numel()
+        if self.device.type == "cuda":
+            torch.cuda.current_stream(self.device).synchronize()
+        for chunk, batch, ids, lps in results:
+            cu, rows = batch.cu_seqlens.tolist(), batch.action_rows + 1
+            for i, traj in enumerate(chunk):
+                n = cu[i + 1] - cu[i]
+                sel = (rows >= cu[i]) & (rows < cu[i + 1])
+                tid = torch.full((n, k), -1, dtype=torch.long)
+                tlp = torch.zeros(n, k)
+                tid[rows[sel] - cu[i]] = ids[sel]
+                tlp[rows[sel] - cu[i]] = lps[sel]
+                traj["teacher_ids"], traj["teacher_logprobs"] = tid.view(1, n, k), tlp.view(1, n, k)
+
+    def distill_update(self, trajectories: List[Dict[str, Any]]) -> Dict[str, float]:
+        """One optimizer step on the distillation loss alone (weighted as ``loss_weights``); every trajectory
+        needs a teacher's tables but neither logprobs nor rewards."""
+        self._check_whole_vocabulary("distill_update")
+        missing = sum("teacher_ids" not in t for t in trajectories)
+        if missing:
+            raise ValueError(f"distill_update: {missing} trajectories have no teacher_ids (see score_teacher)")
+        w = self.loss_weights(trajectories)
+        chunks = self._align_chunks(self.chunk_by_tokens(trajectories, self.max_tokens_per_micro_batch))
+        return self.update_packed([self.to_device(self.pack([trajectories[i] for i in idx], False,
+                                                            [w[i] for i in idx])) for idx in chunks])
+
+    def _loss_backward(self, mb: Dict[str, Any], acc: torch.Tensor, kd: torch.Tensor) -> None:
+        """Loss and backward pass of one device chunk: GRPO, GRPO with the weighted distillation loss from the
+        same LM head product, or (a chunk without old logprobs) distillation alone."""
+        m, batch = self.model, mb["batch"]
+        if "old_logp" not in mb:
+            loss = (m.action_distill(batch, mb["teacher_ids"], mb["teacher_logprobs"], self.temperature,
+                                     divergence=self.distill_divergence) * mb["w"]).sum()
+            loss.backward()
+            acc[0] += loss.detach()
+            kd += loss.detach()
+            return
+        if self.distill_coef > 0.0 and "teacher_ids" in mb:
+            div, logp = m.action_distill(batch, mb["teacher_ids"], mb["teacher_logprobs"], self.temperature,
+                                         with_logprobs=True, divergence=self.distill_divergence)
+            div = (div * mb["w"]).sum()
+        else:
+            logp, div = m.action_logprobs(batch, self.temperature), None
+        loss, pg, kl = self.loss(logp, mb["old_logp"], mb["adv"], mb.get("w"))
+        if div is not None:
+            loss = loss + self.distill_coef * div
+            kd += div.detach()
+        loss.backward()
+        acc += torch.stack([loss.detach(), pg.detach(), kl.detach()])
+
     def grpo_update(self, trajectories: List[Dict[str, Any]], ppo_epochs: int = 1) -> Dict[str, float]:
         """One optimizer step per PPO epoch over the whole batch (host inputs)."""
         epoch_stats = []
@@ -673,14 +775,14 @@ class B200TrainEngine:
         """Forward/backward over device-resident weighted chunks + optimizer step."""
         self.flat_grad.zero_()
         acc = torch.zeros(3, dtype=torch.float32, device=self.device)
+        kd = torch.zeros(1, dtype=torch.float32, device=self.device)
+        distilled = any("teacher_ids" in mb and (self.distill_coef > 0.0 or "old_logp" not in mb)
+                        for mb in device_micro_batches)
         if self.pp_size > 1:
             self._pp_forward_backward(device_micro_batches, acc)
         for mb in device_micro_batches if self.pp_size == 1 else []:
             with nvtx.nvtx_range("forward_backward"):
-                logp = self.model.action_logprobs(mb["batch"], self.temperature)
-                loss, pg, kl = self.loss(logp, mb["old_logp"], mb["adv"], mb.get("w"))
-                loss.backward()
-            acc += torch.stack([loss.detach(), pg.detach(), kl.detach()])
+                self._loss_backward(mb, acc, kd)
         with nvtx.nvtx_range("grad_reduce"):
             self._apply_elastic_inter_replica_gradients()
             for g in self._tp_partial:  # per-head norm weights see only this rank's heads
@@ -693,7 +795,7 @@ class B200TrainEngine:
             return {"loss_sum": acc}
         rewards = [mb["rewards"] for mb in device_micro_batches if "rewards" in mb]
         r = torch.cat(rewards) if rewards else torch.zeros(0, device=self.device)
-        parts = [acc, r.sum().reshape(1).float(), self.sq_norm]
+        parts = [acc, r.sum().reshape(1).float(), self.sq_norm] + ([kd] if distilled else [])
         if self.device.type == "cuda":
             # the error word rides along with the stats read: a bounded wait that gave up inside this step
             # (the fused parameter gather waits on its peers) surfaces here, before the next forward
@@ -706,6 +808,8 @@ class B200TrainEngine:
         out = {"loss": vals[0], "pg_loss": vals[1], "kl": vals[2], "reward_sum": vals[3],
                "n_samples": float(r.numel()), "n_updates": 1.0, "reward_mean": vals[3] / max(r.numel(), 1),
                "grad_norm": math.sqrt(max(vals[4], 0.0))}
+        if distilled:
+            out["distill_loss"] = vals[5]
         return self._reduce_stats(out)
 
     # ------------------------------------------------------------------ gradients/optimizer
@@ -897,11 +1001,13 @@ class B200TrainEngine:
         if self.dp_size <= 1 or not dist.is_initialized():
             return stats
         vec = torch.tensor([stats["loss"], stats["pg_loss"], stats["kl"], stats["reward_sum"], stats["n_samples"],
-                            stats["n_updates"], stats["grad_norm"]], dtype=torch.float32, device=self.device)
+                            stats["n_updates"], stats["grad_norm"], stats.get("distill_loss", 0.0)],
+                           dtype=torch.float32, device=self.device)
         dist.all_reduce(vec, group=self.dp_group)
         n = self.dp_size
         v = vec.tolist()
-        return {"loss": v[0] / n, "pg_loss": v[1] / n, "kl": v[2] / n, "reward_sum": v[3], "n_samples": v[4],
+        more = {"distill_loss": v[7] / n} if "distill_loss" in stats else {}
+        return {**more, "loss": v[0] / n, "pg_loss": v[1] / n, "kl": v[2] / n, "reward_sum": v[3], "n_samples": v[4],
                 "n_updates": v[5], "reward_mean": v[3] / max(v[4], 1.0), "grad_norm": v[6] / n}
 
     def release_optimizer_state(self) -> None:
@@ -1103,7 +1209,8 @@ def _merge_stats(stats: List[Dict[str, float]]) -> Dict[str, float]:
     samples = sum(float(s.get("n_samples", 0.0)) for s in stats)
     rsum = sum(float(s.get("reward_sum", 0.0)) for s in stats)
     wavg = lambda key: sum(float(s.get(key, 0.0)) * float(s.get("n_updates", 1.0)) for s in stats) / max(updates, 1.0)  # noqa: E731
-    return {"loss": wavg("loss"), "pg_loss": wavg("pg_loss"), "kl": wavg("kl"), "reward_sum": rsum,
+    more = {"distill_loss": wavg("distill_loss")} if any("distill_loss" in s for s in stats) else {}
+    return {**more, "loss": wavg("loss"), "pg_loss": wavg("pg_loss"), "kl": wavg("kl"), "reward_sum": rsum,
             "reward_mean": rsum / max(samples, 1.0), "n_samples": samples, "n_updates": updates,
             "grad_norm": wavg("grad_norm")}
 
@@ -1138,4 +1245,6 @@ def create_train_engine(config) -> B200TrainEngine:
                            optimizer_cpu_offload=bool(getattr(config, "megatron_optimizer_cpu_offload", False)),
                            optimizer_offload_fraction=float(getattr(config, "megatron_optimizer_offload_fraction",
                                                                     0.0)),
-                           pp_size=int(getattr(config, "train_pp_size", 1) or 1))
+                           pp_size=int(getattr(config, "train_pp_size", 1) or 1),
+                           distill_coef=float(getattr(config, "distill_coef", 0.0) or 0.0),
+                           distill_divergence=str(getattr(config, "distill_divergence", "forward") or "forward"))

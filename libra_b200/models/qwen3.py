@@ -463,6 +463,25 @@ class Qwen3Model(nn.Module):
         return vocab_parallel_logprob(rows, self.lm_head_weight, batch.action_targets, temperature, self.tp_group,
                                       self.tp_rank, entropy_out)
 
+    def _whole_head_rows(self, batch: PackedBatch, what: str) -> torch.Tensor:
+        if self.tp_size > 1:
+            raise ValueError(f"{what} needs the whole vocabulary on one rank (tp_size=1)")
+        return self.hidden_states(batch).index_select(0, batch.action_rows)
+
+    def action_distill(self, batch: PackedBatch, teacher_ids, teacher_logprobs, temperature: float = 1.0,
+                       with_logprobs: bool = False, **kw):
+        """Divergence of every action token's distribution from the teacher's top logprobs
+        (``ops.lm_head_distill``); with the tokens' logprobs from the same pass if asked for."""
+        rows = self._whole_head_rows(batch, "distillation")
+        return ops.lm_head_distill(rows, self.lm_head_weight, teacher_ids, teacher_logprobs, temperature=temperature,
+                                   targets=batch.action_targets if with_logprobs else None, **kw)
+
+    @torch.no_grad()
+    def action_top_logprobs(self, batch: PackedBatch, k: int, temperature: float = 1.0):
+        """The k most likely tokens and their logprobs at every action token (a teacher's table)."""
+        return ops.lm_head_top_logprobs(self._whole_head_rows(batch, "top logprobs"), self.lm_head_weight, k,
+                                        temperature)
+
     def logits(self, batch: PackedBatch) -> torch.Tensor:
         """Full logits [T, V] (inference/sampling helper)."""
         h = self.hidden_states(batch)

@@ -720,11 +720,12 @@ def grad_sq_norm(grad, out):
     return out
 
 
-from .vocab import control_logits, distill_loss, distill_loss_grad, top_logprobs  # noqa: E402
+from .vocab import (control_logits, distill_loss, distill_loss_grad, lm_head_distill,  # noqa: E402
+                    lm_head_top_logprobs, top_logprobs)
 
 __all__ = [
     "ext", "extension_available", "check_kernel_errors", "gemm", "linear", "rmsnorm", "qk_norm_rope", "swiglu",
     "varlen_causal_attention", "lm_head_logprob", "adamw_step", "grad_sq_norm", "ref", "linear_swiglu",
     "paged_decode", "sample_tokens", "grouped_linear", "grouped_swiglu", "control_logits", "top_logprobs",
-    "distill_loss", "distill_loss_grad",
+    "distill_loss", "distill_loss_grad", "lm_head_distill", "lm_head_top_logprobs",
 ]

@@ -203,3 +203,121 @@ def distill_loss_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
                                  DIVERGENCES[divergence], float(beta), tail == "drop", float(temperature), out,
                                  error_flag(logits.device))
     return loss, out
+
+
+class _LMHeadDistill(torch.autograd.Function):
+    """distill_loss of h W^T / T, chunk by chunk, without an fp32 logits tensor.
+
+    Without targets every chunk's bf16 logits are rewritten by their unit
+    gradients as soon as they are scored (one pass over them), and the upstream
+    gradients of the rows scale the [R, H] operands of the two products instead
+    of the [R, V] gradients.  With targets the two upstream gradients mix per
+    token, so the logits are kept and rewritten in the backward pass."""
+
+    @staticmethod
+    def forward(ctx, h, w, ids, lps, kind, targets):
+        from . import LOGPROB_CHUNK_ROWS, error_flag, ext, gemm
+
+        C, err = ext(), error_flag(h.device)
+        div, beta, drop, temperature = kind
+        R = h.shape[0]
+        loss = torch.empty(R, dtype=torch.float32, device=h.device)
+        logp = None if targets is None else torch.empty(R, dtype=torch.float32, device=h.device)
+        need = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        ctx.kept, ctx.rows = [], LOGPROB_CHUNK_ROWS
+        for s in range(0, R, ctx.rows):
+            e = min(R, s + ctx.rows)
+            logits = gemm(h[s:e], w)
+            saved = None
+            if need and targets is None:
+                loss[s:e] = C.distill_onepass(logits, ids[s:e], lps[s:e], div, beta, drop, temperature, logits, err)
+            else:
+                loss[s:e], lp, saved = C.distill_fwd(logits, ids[s:e], lps[s:e], div, beta, drop, temperature,
+                                                     None if targets is None else targets[s:e], err)
+                if logp is not None:
+                    logp[s:e] = lp
+            if need:
+                ctx.kept.append((logits, saved))
+        ctx.save_for_backward(h, w, targets)
+        ctx.temperature, ctx.slots = temperature, ids.shape[1]
+        ctx.set_materialize_grads(False)
+        return loss, logp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, g_lp):
+        from . import EPI_ACC_F32, EPI_F32, ext, gemm
+
+        h, w, targets = ctx.saved_tensors
+        if g is None and g_lp is None:
+            return (None,) * 6
+        R = h.shape[0]
+        if R and not ctx.kept:
+            raise RuntimeError("lm_head_distill: its backward pass runs once (the logits are gone)")
+        g = torch.zeros(R, device=h.device) if g is None else g.contiguous()
+        if targets is not None:
+            g_lp = torch.zeros(R, device=h.device) if g_lp is None else g_lp.contiguous()
+        dh = torch.empty_like(h) if ctx.needs_input_grad[0] else None
+        main = getattr(w, "main_grad", None)
+        dw = main
+        if ctx.needs_input_grad[1] and main is None:
+            dw = torch.zeros(w.shape, dtype=torch.float32, device=w.device)
+        kept, ctx.kept = ctx.kept, []
+        for n, s in enumerate(range(0, R, ctx.rows)):
+            e = min(R, s + ctx.rows)
+            logits, saved = kept[n]
+            kept[n] = None
+            x = h[s:e]
+            if targets is None:  # logits are unit gradients already
+                if dh is not None:
+                    dh[s:e] = gemm(logits, w, b_mn=True, epi=EPI_F32) * g[s:e].unsqueeze(1)
+                x = (x.float() * g[s:e].unsqueeze(1)).to(h.dtype)
+            else:
+                ext().distill_bwd(logits, logits, ctx.temperature, ctx.slots, targets[s:e], saved, g[s:e], g_lp[s:e])
+                if dh is not None:
+                    gemm(logits, w, b_mn=True, out=dh[s:e])
+            if ctx.needs_input_grad[1]:
+                gemm(logits, x, a_mn=True, b_mn=True, out=dw, epi=EPI_ACC_F32)
+        return dh, (None if main is not None or dw is None else dw.to(w.dtype)), None, None, None, None
+
+
+def lm_head_distill(h: torch.Tensor, w: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, *,
+                    divergence: str = "forward", beta: float = 0.5, tail: str = "bucket", temperature: float = 1.0,
+                    targets: Optional[torch.Tensor] = None):
+    """``distill_loss`` of the LM head ``w`` [V, H] on hidden rows ``h`` [R, H]
+    (the logits are rounded to bf16, as in ``lm_head_logprob``), differentiable
+    with respect to both; the weight's gradient accumulates into its
+    ``main_grad`` when it has one.  With ``targets`` int64 [R] the result is
+    (loss, logprob of the targets), GRPO's logprobs and the distillation loss
+    from one LM head product.  The backward pass runs once."""
+    _check_distill("lm_head_distill", h, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature)
+    if h.dim() != 2 or w.dim() != 2 or h.shape[1] != w.shape[1]:
+        raise ValueError(f"lm_head_distill: h [R, H] and w [V, H], got {tuple(h.shape)} and {tuple(w.shape)}")
+    if h.device.type != "cuda":
+        logits = torch.nn.functional.linear(h.float(), w.float())
+        loss, logp = ref.distill_loss(logits, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature,
+                                      targets)
+    else:
+        kind = (DIVERGENCES[divergence], float(beta), tail == "drop", float(temperature))
+        loss, logp = _LMHeadDistill.apply(h.contiguous(), w, teacher_ids.contiguous(), teacher_logprobs.contiguous(),
+                                          kind, None if targets is None else targets.contiguous())
+    return loss if targets is None else (loss, logp)
+
+
+@torch.no_grad()
+def lm_head_top_logprobs(h: torch.Tensor, w: torch.Tensor, k: int, temperature: float = 1.0
+                         ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``top_logprobs`` of the LM head ``w`` on hidden rows ``h``, chunk by
+    chunk: token ids int64 [R, k] and logprobs fp32 [R, k], a teacher's side of
+    ``lm_head_distill``."""
+    from . import LOGPROB_CHUNK_ROWS, linear
+
+    k = int(k)
+    if not 1 <= k <= min(MAX_TOP, w.shape[0]):
+        raise ValueError(f"lm_head_top_logprobs: k must lie in [1, {min(MAX_TOP, w.shape[0])}], got {k}")
+    ids = torch.empty(h.shape[0], k, dtype=torch.long, device=h.device)
+    lps = torch.empty(h.shape[0], k, dtype=torch.float32, device=h.device)
+    for s in range(0, h.shape[0], LOGPROB_CHUNK_ROWS):
+        e = min(h.shape[0], s + LOGPROB_CHUNK_ROWS)
+        ids[s:e], lps[s:e], _ = top_logprobs(linear(h[s:e], w), k, temperature)
+    return ids, lps
