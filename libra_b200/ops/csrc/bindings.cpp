@@ -117,6 +117,9 @@ std::vector<torch::Tensor> top_logprobs(torch::Tensor logits, int64_t k, c10::op
 std::vector<torch::Tensor> distill_fwd(torch::Tensor logits, torch::Tensor ids, torch::Tensor lps, int64_t div,
                                        double beta, bool drop, double T, c10::optional<torch::Tensor> targets,
                                        torch::Tensor err);
+std::vector<torch::Tensor> distill_loss(torch::Tensor logits, torch::Tensor ids, torch::Tensor lps, int64_t div,
+                                        double beta, bool drop, double T, c10::optional<torch::Tensor> targets,
+                                        torch::Tensor err);
 torch::Tensor distill_onepass(torch::Tensor logits, torch::Tensor ids, torch::Tensor lps, int64_t div, double beta,
                               bool drop, double T, torch::Tensor out, torch::Tensor err);
 void distill_bwd(torch::Tensor logits, torch::Tensor out, double T, int64_t K, c10::optional<torch::Tensor> targets,
@@ -184,6 +187,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "repetition / presence / frequency penalties, biases and grammar masks on rows of logits");
   m.def("top_logprobs", &libra::vocab::top_logprobs, "k largest logits of every row with their logprobs");
   m.def("distill_fwd", &libra::vocab::distill_fwd, "distillation loss from a teacher's top logprobs");
+  m.def("distill_loss", &libra::vocab::distill_loss, "distill_fwd with autograd through distill_bwd");
   m.def("distill_onepass", &libra::vocab::distill_onepass, "distillation loss and unit gradient in one pass");
   m.def("distill_bwd", &libra::vocab::distill_bwd, "gradient of distill_fwd with respect to the logits");
   m.def("flash_fwd", &libra::attn::flash_fwd, "tcgen05 varlen GQA attention forward", py::arg("q"), py::arg("k"),

@@ -122,33 +122,6 @@ def _check_distill(op: str, logits, ids, lps, divergence, beta, tail, temperatur
         raise ValueError(f"{op}: 1 to {MAX_TOP} teacher tokens a row, got {ids.shape[1]}")
 
 
-class _DistillLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, lps, div, beta, drop, temperature, targets):
-        from . import error_flag, ext
-
-        loss, logp, saved = ext().distill_fwd(logits, ids, lps, div, beta, drop, temperature, targets,
-                                              error_flag(logits.device))
-        ctx.save_for_backward(logits, targets, saved)
-        ctx.temperature, ctx.slots = temperature, ids.shape[1]
-        ctx.set_materialize_grads(False)
-        return loss, (logp if targets is not None else None)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, g_lp):
-        from . import ext
-
-        logits, targets, saved = ctx.saved_tensors
-        if g is None and g_lp is None:
-            return (None,) * 8
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        g = torch.zeros(logits.shape[0], device=logits.device) if g is None else g.contiguous()
-        ext().distill_bwd(logits, grad, ctx.temperature, ctx.slots, targets, saved, g,
-                          None if g_lp is None else g_lp.contiguous())
-        return (grad,) + (None,) * 7
-
-
 def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, *,
                  divergence: str = "forward", beta: float = 0.5, tail: str = "bucket", temperature: float = 1.0,
                  targets: Optional[torch.Tensor] = None):
@@ -174,9 +147,12 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logpro
         loss, logp = ref.distill_loss(logits, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature,
                                       targets)
     else:
-        loss, logp = _DistillLoss.apply(logits, teacher_ids.contiguous(), teacher_logprobs.contiguous(),
+        from . import error_flag, ext
+
+        loss, logp = ext().distill_loss(logits, teacher_ids.contiguous(), teacher_logprobs.contiguous(),
                                         DIVERGENCES[divergence], float(beta), tail == "drop", float(temperature),
-                                        None if targets is None else targets.contiguous())
+                                        None if targets is None else targets.contiguous(),
+                                        error_flag(logits.device))
     return loss if targets is None else (loss, logp)
 
 

@@ -578,6 +578,20 @@ def test_distill_kernel_refusals():
 
 
 @pytest.mark.gpu
+def test_distill_refuses_second_derivatives_and_changed_logits():
+    z = _rand((2, 64), 0, torch.float32, "cuda").requires_grad_(True)
+    ids, lps = _teacher(z.detach(), 3, 2, 1.0)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(ops.distill_loss(z, ids, lps).sum(), z, create_graph=True)
+    y = z * 1.0
+    loss = ops.distill_loss(y, ids, lps).sum()
+    y.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    assert not ops.distill_loss(z.detach(), ids, lps).requires_grad
+
+
+@pytest.mark.gpu
 def test_distill_reports_targets_outside_the_vocabulary():
     dev = torch.device("cuda", torch.cuda.current_device())
     z = _rand((3, 500), 0, torch.float32, dev).requires_grad_(True)
