@@ -74,14 +74,21 @@ struct Counts {
   }
 };
 
+struct Penalty {
+  float rep, inv, pres, freq;  // inv = 1 / rep
+};
+
+// Without branches: some lane of a warp has an occurrence in almost every octet of the frequent tokens.  A product with
+// 1 / r instead of the quotient adds one rounding (2^-24), and takes a fifth of a division's instructions.
 template <int kBits>
-__device__ __forceinline__ float penalize(float x, uint32_t c, float rep, float pres, float freq) {
-  if (c) {
-    x = x > 0.f ? x / rep : x * rep;
-    const uint32_t k = c & Counts<kBits>::kCount;
-    if (k) x = x - freq * (float)k - pres;
-  }
-  return x;
+__device__ __forceinline__ float penalize(float x, uint32_t c, const Penalty& p) {
+  const uint32_t k = c & Counts<kBits>::kCount;
+  // 2^23 + k is a float whose low bits are k
+  const float n = kBits == 16 ? __uint_as_float(0x4b000000u | k) - 8388608.f : (float)k;
+  const float s = x > 0.f ? p.inv : p.rep;
+  x *= c ? s : 1.f;
+  const float less = fmaf(p.freq, n, p.pres);
+  return x - (k ? less : 0.f);
 }
 
 // Bits of tokens j .. j + 7.
@@ -111,11 +118,12 @@ __global__ void __launch_bounds__(kCtlThreads, 3) control_kernel(const TI* logit
   // tokens [lo, hi) of the row; token j has counter j - base, and octets start at multiples of 8 of it
   const int base = sp.head + 8 * o0 - 8;
   const int lo = first ? 0 : sp.head + 8 * o0, hi = last ? V : sp.head + 8 * o1;
-  const float rep = a.rep ? a.rep[b] : 1.f, pres = a.pres ? a.pres[b] : 0.f, freq = a.freq ? a.freq[b] : 0.f;
+  const float rep = a.rep ? a.rep[b] : 1.f;
+  const Penalty pen = {rep, 1.f / rep, a.pres ? a.pres[b] : 0.f, a.freq ? a.freq[b] : 0.f};
   bool bad = false;
   int len = 0, prompt = 0;
   const int* h = nullptr;
-  if (a.hist && (rep != 1.f || pres != 0.f || freq != 0.f)) {
+  if (a.hist && (rep != 1.f || pen.pres != 0.f || pen.freq != 0.f)) {
     const int hr = a.hist_rows ? a.hist_rows[b] : b;
     len = a.hist_lens[b];
     const bool in = hr >= 0 && hr < a.hist_rows_n;
@@ -171,7 +179,7 @@ __global__ void __launch_bounds__(kCtlThreads, 3) control_kernel(const TI* logit
   if ((first && t < sp.head) || (last && t >= 32 && t - 32 < sp.tail)) {
     const int j = t < 32 ? t : sp.head + 8 * sp.octs + t - 32;
     const uint32_t c = counted ? cnt.get(j - base) : 0u;
-    float x = penalize<kBits>(to_f(z[j]), c, rep, pres, freq);
+    float x = penalize<kBits>(to_f(z[j]), c, pen);
     if (mask && !((mask[j >> 5] >> (j & 31)) & 1)) x = -INFINITY;
     if (!biased || !((biases[(j - base) >> 5] >> ((j - base) & 31)) & 1)) from_f(dst + j, x);
   }
@@ -201,7 +209,7 @@ __global__ void __launch_bounds__(kCtlThreads, 3) control_kernel(const TI* logit
       uint32_t c[8];
       if (counted && cnt.octet(8 * (p - o0) + 8, c)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = penalize<kBits>(f[e], c[e], rep, pres, freq);
+        for (int e = 0; e < 8; ++e) f[e] = penalize<kBits>(f[e], c[e], pen);
       }
       const uint32_t skip = biased ? bias_bytes[p - o0] : 0u;
       if (allow[u] != 0xffu) {
@@ -231,7 +239,7 @@ __global__ void __launch_bounds__(kCtlThreads, 3) control_kernel(const TI* logit
       for (int i = e + 1; i < b1; ++i)
         if (a.bias_ids[i] == id) s += a.bias_vals[i];
     }
-    float x = penalize<kBits>(to_f(z[id]), counted ? cnt.get(id - base) : 0u, rep, pres, freq) + s;
+    float x = penalize<kBits>(to_f(z[id]), counted ? cnt.get(id - base) : 0u, pen) + s;
     if (mask && !((mask[id >> 5] >> (id & 31)) & 1)) x = -INFINITY;
     from_f(dst + id, x);
   }
@@ -306,8 +314,8 @@ void control_logits(torch::Tensor logits, c10::optional<torch::Tensor> history,
   a.err = err.data_ptr<int>();
   const c10::cuda::CUDAGuard guard(logits.device());
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  // tiles of 32768 tokens, since every tile scans the history once (256 x 151936 fp32 with 16384 tokens of history: 82 us,
-  // 89 us with tiles of 16384, 118 us with 256 threads), smaller ones while that leaves SMs without three CTAs
+  // tiles of 32768 tokens, since every tile scans the history once (256 x 151936 fp32 with 16384 tokens of history: 80 us,
+  // 84 us with tiles of 16384), smaller ones while that leaves SMs without three CTAs
   int tile = 32768;
   while (tile > 2048 && (int64_t)B * ((V + tile - 1) / tile) < 3 * 148) tile /= 2;
   const int tiles = std::max(1, (V / 8 + tile / 8 - 1) / (tile / 8));
