@@ -96,7 +96,7 @@ class LogitControls:
         width = 4096 if self.table is None else self.table.shape[1]
         while width < need:
             width *= 2
-        if 16384 < need < 32768:
+        if 16384 < need <= 32760:
             width = 32760  # the kernel counts histories below 32768 in 16 bits
         if self.table is None or width != self.table.shape[1]:
             new = torch.zeros(self.max_rows, width, dtype=torch.int32, device=self.device)

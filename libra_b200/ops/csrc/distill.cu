@@ -38,7 +38,7 @@ enum Divergence : int { kForward = 0, kReverse = 1, kJs = 2 };
 //   [0] reference m of the unlisted logits
 //   [1] A: unlisted dL/dx_j = A exp((z_j - m) / T)
 //   [2] B: softmax of an unlisted token = B exp((z_j - m) / T)
-//   [3] kLossRow if the loss is not identically 0, plus kProbRow if the target's logprob is finite
+//   [3] kLossRow if the loss is not identically 0, plus kProbRow if the target's logprob has a gradient
 
 // Sums over a row's table.  With mk the largest listed logit and x_k = (z_k - mk) / T:
 struct __align__(16) TableSums {
@@ -383,10 +383,9 @@ __global__ void __launch_bounds__(kTableWarps * 32) distill_row_kernel(const T* 
       const int64_t g = a.targets[row];
       const bool in = g >= 0 && g < V;
       if (!in) atomicCAS(a.err, 0, kBadArgument);
-      const float lt = in && log_s != -INFINITY
-                           ? (float)(((double)to_f(logits[(int64_t)row * ld + g]) - m) / a.T - log_s) : -INFINITY;
-      a.logp[row] = lt;
-      if (lt != -INFINITY) flags |= kProbRow;
+      const bool defined = in && log_s != -INFINITY;  // the row has a distribution
+      a.logp[row] = defined ? (float)(((double)to_f(logits[(int64_t)row * ld + g]) - m) / a.T - log_s) : -INFINITY;
+      if (defined) flags |= kProbRow;
     }
     *reinterpret_cast<float4*>(a.stats + 4 * (int64_t)row) = make_float4(f.m, f.A, f.B, (float)flags);
   }
@@ -476,7 +475,7 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logit
 
 // Unit gradient in one pass: a cluster holds the whole row in shared memory, each CTA its slice, so the logits are read
 // once.  A thread copies, sums and rewrites the same octets, which needs no barrier.  Behind the one cluster barrier
-// that the slices' sums wait for, every CTA finishes the row for itself (a few scalars by the last warp).  out may be
+// that the slices' sums wait for, every CTA finishes the row for itself (a few scalars by the first warp).  out may be
 // the logits: the tables were read before.
 template <typename T>
 __global__ void __launch_bounds__(kOneThreads, kOneCtas) distill_onepass_kernel(const T* logits, int64_t ld, T* out,
@@ -535,7 +534,7 @@ __global__ void __launch_bounds__(kOneThreads, kOneCtas) distill_onepass_kernel(
     r = join_warps<kOneThreads / 32>(c, red);
     if (t == 0) part = r;
   }
-  cluster_sync_all();
+  cluster_meet();
   if (t < 32) {
     r = warp_merge(t < n ? MaxSum{ld_cluster(&part.m, t), ld_cluster(&part.s, t)} : MaxSum{-FLT_MAX, 0.f}, c);
     const RowFin f = finish_grads(a, row, u, r, c);
@@ -603,15 +602,15 @@ static void check_distill(const torch::Tensor& logits, const torch::Tensor& ids,
   LIBRA_CHECK(lps.sizes() == ids.sizes() && vec_of(lps, logits, at::kFloat, ids.numel()),
               "%s: teacher_logprobs must be contiguous fp32 like teacher_ids", op);
   LIBRA_CHECK(V >= 1 && V <= 1600000, "%s: vocabulary of 1 to 1600000 tokens", op);
-  LIBRA_CHECK(div >= 0 && div <= 2 && beta > 0.0 && beta < 1.0 && T > 0.0, "%s: divergence, beta or temperature", op);
+  LIBRA_CHECK(div >= 0 && div <= 2 && beta > 0.0 && beta < 1.0 && T >= 1e-6 && T <= 1e6,
+              "%s: divergence, beta or temperature", op);
 }
 
-// The tables' memory in one allocation, behind `extra` floats: sums, slices' parts, tokens, exp(x), p, x - log p.
-static torch::Tensor alloc_tables(DistArgs& a, const torch::Tensor& logits, int64_t splits, int64_t extra) {
+// The tables' memory in one allocation: sums, slices' parts, tokens, exp(x), p, x - log p.
+static torch::Tensor alloc_tables(DistArgs& a, const torch::Tensor& logits, int64_t splits) {
   const int64_t NK = (int64_t)a.N * a.K, per = sizeof(TableSums) / 4;
-  extra = (extra + 3) / 4 * 4;
-  auto buf = torch::empty({extra + a.N * (per + 2 * splits) + 4 * NK}, logits.options().dtype(at::kFloat));
-  float* p = buf.data_ptr<float>() + extra;
+  auto buf = torch::empty({a.N * (per + 2 * splits) + 4 * NK}, logits.options().dtype(at::kFloat));
+  float* p = buf.data_ptr<float>();
   a.sums = reinterpret_cast<TableSums*>(p);
   p += a.N * per;
   a.parts = reinterpret_cast<MaxSum*>(p);
@@ -658,7 +657,7 @@ std::vector<torch::Tensor> distill_fwd(torch::Tensor logits, torch::Tensor ids, 
   const int64_t NK = (int64_t)N * K;
   auto saved = torch::empty({4 * (int64_t)N + 3 * NK}, f32);
   if (N == 0) return {loss, logp, saved};
-  auto work = alloc_tables(a, logits, n, 0);
+  auto work = alloc_tables(a, logits, n);
   a.stats = saved.data_ptr<float>();
   a.dk = a.stats + 4 * (int64_t)N;
   a.qk = a.dk + NK;
@@ -709,7 +708,7 @@ torch::Tensor distill_onepass(torch::Tensor logits, torch::Tensor ids, torch::Te
   auto loss = torch::empty({N}, logits.options().dtype(at::kFloat));
   if (N == 0) return loss;
   DistArgs a = make_args(logits, ids, lps, div, beta, drop, T, loss, err);
-  auto work = alloc_tables(a, logits, 1, 0);
+  auto work = alloc_tables(a, logits, 1);
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   const int octs = slice_octs(V, n), bits_at = octs * 8 * size, rows = (N + kTableWarps - 1) / kTableWarps;
   const size_t smem = bits_at + (octs + 2 + 3) / 4 * 4;

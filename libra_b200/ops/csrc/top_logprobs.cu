@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) top_kernel(const T* logits, in
   const Slice sl = row_slice(sp, rank, lg);
   float tm = temps ? temps[row] : temp;
   if (!(tm > 0.f)) tm = 1.f;
-  const float c = kLog2e / tm, slack = kSlack / c;
+  const float c = fminf(kLog2e / tm, FLT_MAX), slack = kSlack / c;  // (a tiny temperature is its limit, one-hot)
   if (t == 0) sh.n_noted = sh.n_chosen = 0;
   constexpr int kU = kClasses;
   const T* body = z + sp.head;
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) top_kernel(const T* logits, in
   }
   if (t == 0) sh.n_list = min(chosen, k);
   if (n > 1)
-    cluster_sync_all();
+    cluster_meet();
   else
     __syncthreads();
   if (n > 1) {
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) top_kernel(const T* logits, in
       __syncthreads();
     }
   }
-  if (n > 1) cluster_sync_all();  // a CTA's list outlives its readers
+  if (n > 1) cluster_meet();  // a CTA's list outlives its readers
 }
 
 // logits [N, V] bf16 / fp32 -> ids [N, k] int64, logprobs [N, k] fp32 (descending), lse [N] fp32.

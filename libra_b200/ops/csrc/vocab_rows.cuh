@@ -252,8 +252,18 @@ __device__ __forceinline__ double ld_cluster(const double* p, uint32_t rank) {
   asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_meet() {
+  cluster_arrive();
+  cluster_wait();
+}
 
 // 16 bytes global -> shared without a register; a thread that reads only what it copied itself needs no barrier.
 __device__ __forceinline__ void copy16_async(void* dst, const void* src) {

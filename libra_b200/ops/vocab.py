@@ -57,7 +57,8 @@ def control_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
       -inf, whatever their logit was; a row may end up with nothing else.
 
     They apply in this order, in fp32, with one rounding to ``out`` (fp32
-    unless given; it may be ``logits`` itself).  Row numbers, lengths and
+    unless given; it may be ``logits`` itself), and are not differentiated
+    through.  Row numbers, lengths and
     offsets that point outside their tables are not followed: they set the
     error word that ``check_kernel_errors`` raises.
     """
@@ -90,7 +91,8 @@ def top_logprobs(logits: torch.Tensor, k: int, temperature: Union[float, torch.T
     logprobs under softmax(logits / temperature) fp32 [N, k] and the row's
     log-sum-exp fp32 [N].  ``temperature``: a number or fp32 [N]; what is not
     above 0 counts as 1.  A row of nothing but -inf has logprobs and
-    log-sum-exp of -inf; NaN ranks above +inf and makes the row's logprobs NaN."""
+    log-sum-exp of -inf; NaN ranks above +inf and makes the row's logprobs NaN.
+    Not differentiated through."""
     logits = _rows(logits, "top_logprobs")
     k = int(k)
     if not 1 <= k <= min(MAX_TOP, logits.shape[1]):
@@ -113,8 +115,8 @@ def _check_distill(op: str, logits, ids, lps, divergence, beta, tail, temperatur
         raise ValueError(f"{op}: the reverse divergence needs the rest bucket (it is infinite without one)")
     if divergence == "js" and not 0.0 < beta < 1.0:
         raise ValueError(f"{op}: beta must lie between 0 and 1, got {beta}")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"{op}: temperature must be above 0, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"{op}: temperature must lie in [1e-6, 1e6], got {temperature}")
     if ids.dim() != 2 or ids.shape != lps.shape or ids.shape[0] != logits.shape[0]:
         raise ValueError(f"{op}: teacher_ids and teacher_logprobs must be [rows, K], got {tuple(ids.shape)} and "
                          f"{tuple(lps.shape)} for {logits.shape[0]} rows")
@@ -140,7 +142,9 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logpro
     probabilities by their sum.  The student is softmax(logits / temperature).
 
     With ``targets`` int64 [N] the result is (loss, logprob of the targets),
-    both from the same pass and both differentiable."""
+    both from the same pass and both differentiable; targets outside the
+    vocabulary have logprob -inf and no gradient, and set the error word that
+    ``check_kernel_errors`` raises (ValueError on the CPU)."""
     logits = _rows(logits, "distill_loss")
     _check_distill("distill_loss", logits, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature)
     if logits.device.type != "cuda":

@@ -289,6 +289,9 @@ def test_top_logprobs_awkward_rows(device, kind, V, k, dtype):
 def test_top_logprobs_row_temperatures_and_refusals(device):
     z = _rand((4, 500), 2, torch.bfloat16, device)
     _check_top(z, 9, torch.tensor([0.5, 2.0, 0.0, 1.0], device=device))
+    z[0, 7] = 50.0  # a single best token: all of the mass in the limit of a tiny temperature
+    _, lp, _ = ops.top_logprobs(z[:1], 2, 1e-30)
+    assert float(lp[0, 0]) == 0.0 and float(lp[0, 1]) < -1e30
     assert [t.shape for t in ops.top_logprobs(z[:0], 3)] == [(0, 3), (0, 3), (0,)]
     for k in (0, 257, 501):
         with pytest.raises(ValueError, match="k must"):
@@ -476,6 +479,21 @@ def test_distill_row_of_nothing_but_minus_infinity(device):
     assert float(loss[1]) == 0.0 and float(logp[1]) == -math.inf
     (grad,) = torch.autograd.grad((loss.sum() + logp[[0, 2]].sum()), x)
     assert not bool(grad[1].any()) and bool(torch.isfinite(grad).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_distill_masked_target_has_the_softmax_gradient(device):
+    z = _rand((2, 400), 2, torch.float32, device)
+    ids, lps = _teacher(z, 5, 3, 1.0)
+    targets = torch.tensor([7, 9], device=device)
+    ids[ids == 7] = -1
+    z[0, 7] = -math.inf
+    x = z.clone().requires_grad_(True)
+    loss, logp = ops.distill_loss(x, ids, lps, targets=targets)
+    assert float(logp[0].detach()) == -math.inf
+    (grad,) = torch.autograd.grad(logp, x, torch.ones_like(logp))
+    want = torch.nn.functional.one_hot(targets, 400) - torch.softmax(z.double(), 1)
+    assert torch.allclose(grad.double(), want, rtol=1e-4, atol=1e-7)
 
 
 @pytest.mark.parametrize("device", DEVICES)
