@@ -247,9 +247,10 @@ __global__ void __launch_bounds__(kTopThreads, 4) top_kernel(const T* logits, in
   if (n > 1) {
     len = (t & 31) < n ? ld_cluster(&sh.n_list, t & 31) : 0;
     total = __reduce_add_sync(0xffffffffu, len);
-    for (int q = 0; q < n; ++q) {
+    for (int i0 = 0; i0 < n * k; i0 += kTopThreads) {  // all lists at once: a remote load takes some 500 cycles
+      const int q = min((i0 + t) / k, n - 1), i = i0 + t - q * k;
       const int have = __shfl_sync(0xffffffffu, len, q);
-      for (int i = t; i < have; i += kTopThreads) sh.others[q * kTopMax + i] = ld_cluster(&sh.list[i], q);
+      if (i < have) sh.others[q * kTopMax + i] = ld_cluster(&sh.list[i], q);
     }
     __syncthreads();
   }
