@@ -155,16 +155,25 @@ __global__ void __launch_bounds__(kCtlThreads, 3) control_kernel(const TI* logit
     for (int i = t; i < (hi - base + 31) / 32 && biased; i += kCtlThreads) biases[i] = 0u;
     if (t == 0) twice = 0;
     __syncthreads();
-#pragma unroll 8
-    for (int i = t; i < len; i += kCtlThreads) {
-      const int id = h[i];
+    const auto count = [&](int i, int id) {
       if (id >= lo && id < hi) {
         if (i < prompt)
           cnt.see(id - base);
         else
           cnt.add(id - base);
       }
+    };
+    const int quads_in = aligned16(h) ? len / 4 : 0;  // four tokens a load
+#pragma unroll 4
+    for (int i = t; i < quads_in; i += kCtlThreads) {
+      const int4 q = __ldg(reinterpret_cast<const int4*>(h) + i);
+      count(4 * i, q.x);
+      count(4 * i + 1, q.y);
+      count(4 * i + 2, q.z);
+      count(4 * i + 3, q.w);
     }
+#pragma unroll 4
+    for (int i = 4 * quads_in + t; i < len; i += kCtlThreads) count(i, h[i]);
     for (int e = b0 + t; e < b1; e += kCtlThreads) {
       const int id = a.bias_ids[e];
       if (id < lo || id >= hi) continue;
