@@ -737,14 +737,14 @@ class B200TrainEngine:
         return self.update_packed([self.to_device(self.pack([trajectories[i] for i in idx], False,
                                                             [w[i] for i in idx])) for idx in chunks])
 
-    def _loss_backward(self, mb: Dict[str, Any], acc: torch.Tensor, kd: torch.Tensor) -> None:
+    def _loss_backward(self, mb: Dict[str, Any], acc: torch.Tensor, kd: torch.Tensor, scale: float = 1.0) -> None:
         """Loss and backward pass of one device chunk: GRPO, GRPO with the weighted distillation loss from the
-        same LM head product, or (a chunk without old logprobs) distillation alone."""
+        same LM head product, or (a chunk without old logprobs) distillation alone.  ``scale``: of the gradient."""
         m, batch = self.model, mb["batch"]
         if "old_logp" not in mb:
             loss = (m.action_distill(batch, mb["teacher_ids"], mb["teacher_logprobs"], self.temperature,
                                      divergence=self.distill_divergence) * mb["w"]).sum()
-            loss.backward()
+            (loss if scale == 1.0 else loss * scale).backward()
             acc[0] += loss.detach()
             kd += loss.detach()
             return
@@ -758,7 +758,7 @@ class B200TrainEngine:
         if div is not None:
             loss = loss + self.distill_coef * div
             kd += div.detach()
-        loss.backward()
+        (loss if scale == 1.0 else loss * scale).backward()
         acc += torch.stack([loss.detach(), pg.detach(), kl.detach()])
 
     def grpo_update(self, trajectories: List[Dict[str, Any]], ppo_epochs: int = 1) -> Dict[str, float]:
@@ -1159,10 +1159,8 @@ class B200TrainEngine:
 
         self.flat_grad.zero_()
         for hb in self.prepare_update(trajectories):
-            mb = self.to_device(hb)
-            logp = self.model.action_logprobs(mb["batch"], self.temperature)
-            loss, _, _ = self.loss(logp, mb["old_logp"], mb["adv"], mb.get("w"))
-            (loss * loss_scale).backward()
+            self._loss_backward(self.to_device(hb), torch.zeros(3, device=self.device),
+                                torch.zeros(1, device=self.device), float(loss_scale))
         return GradientPayload(replica_id, target_core_id, (self.flat_grad,), False, replica_rank,
                                replica_world_size, step, self.current_version, membership_epoch)
 

@@ -323,8 +323,8 @@ void control_logits(torch::Tensor logits, c10::optional<torch::Tensor> history,
   a.err = err.data_ptr<int>();
   const c10::cuda::CUDAGuard guard(logits.device());
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  // tiles of 32768 tokens, since every tile scans the history once (256 x 151936 fp32 with 16384 tokens of history: 80 us,
-  // 84 us with tiles of 16384), smaller ones while that leaves SMs without three CTAs
+  // tiles of 32768 tokens, since every tile scans the history once (256 x 151936 fp32 with 16384 tokens of history: 81 us,
+  // 84 us with tiles of 16384, both before the history was read four tokens a load: 75 us, 0.65 of the floor), smaller ones while that leaves SMs without three CTAs
   int tile = 32768;
   while (tile > 2048 && (int64_t)B * ((V + tile - 1) / tile) < 3 * 148) tile /= 2;
   const int tiles = std::max(1, (V / 8 + tile / 8 - 1) / (tile / 8));

@@ -177,6 +177,18 @@ def test_grpo_update_with_the_distillation_term(device):
     assert float((both.flat_grad - want).norm() / want.norm()) < 4 * U16
 
 
+def test_hybrid_payload_carries_the_distillation_term():
+    teacher = _engine("cpu", seed=1)
+    kw = dict(seed=7, distill_coef=0.5)
+    core, hybrid = _engine("cpu", **kw), _engine("cpu", **kw)
+    trajs = _trajectories(core.cfg.vocab_size)
+    core.recompute_logprobs(trajs)
+    teacher.score_teacher(trajs, 5)
+    core.grpo_update(trajs)
+    hybrid.compute_gradient_payload(trajs, replica_id="h", target_core_id="c", step=0, membership_epoch=0)
+    assert torch.equal(core.flat_grad, hybrid.flat_grad)
+
+
 def test_engine_refuses_distillation_across_ranks():
     from libra_b200.engine.train_engine import B200TrainEngine
 
