@@ -293,8 +293,11 @@ __device__ __forceinline__ double finish_loss(const DistArgs& a, int row, const 
       if (a.div == kReverse) {
         if (!(q == 0.0)) sum += q * d;
       } else {
-        if (p > 0.0) sum -= b * p * log(b + (1.0 - b) * exp(d));
-        if (!(q == 0.0)) sum -= (1.0 - b) * q * log(b * exp(-d) + (1.0 - b));
+        // log(m / p) = log(b + (1-b) e^d) and log(m / q) = log(b e^-d + (1-b)), with the larger power taken out of both:
+        // a q far below p is a subnormal whose e^-d is infinite
+        const double e = exp(-fabs(d)), l = log(d > 0.0 ? b * e + (1.0 - b) : b + (1.0 - b) * e);
+        if (p > 0.0) sum -= b * p * (l + fmax(d, 0.0));
+        if (!(q == 0.0)) sum -= (1.0 - b) * q * (l + fmax(-d, 0.0));
       }
     }
     loss = warp_sum(sum);
