@@ -42,7 +42,7 @@ enum Divergence : int { kForward = 0, kReverse = 1, kJs = 2 };
 
 // Sums over a row's table.  With mk the largest listed logit and x_k = (z_k - mk) / T:
 struct __align__(16) TableSums {
-  double s, mass, dot;  // sum of exp(x), of p, of p (log p - x)
+  double s, mass, dot;  // sum of exp(x), of p, of p (log p - x); tail = drop: of p relative to the row's largest
   double p_rest;        // the teacher's mass outside the table
   float sf, massf, p_restf, lp_rest, by, log_by;  // p is scaled by `by` (tail = drop)
   float mk;
@@ -185,10 +185,19 @@ __global__ void __launch_bounds__(kTableWarps * 32) distill_table_kernel(const T
   }
   mk = warp_max(mk);
   any = __any_sync(0xffffffffu, any);
+  // tail = drop: relative to the row's largest, since only the ratios of the p count and none of them may underflow
+  double lp_max = 0.0;
+  if (a.drop) {
+    float most = -INFINITY;
+    for (int k = lane; k < K; k += 32)
+      if (ids[k] >= 0) most = fmaxf(most, a.lps[base + k]);
+    most = warp_max(most);
+    if (most > -INFINITY) lp_max = (double)most;
+  }
   double s = 0.0, mass = 0.0, dot = 0.0;
   for (int k = lane; k < K; k += 32) {
     const bool on = ids[k] >= 0;
-    const double lp = on ? (double)a.lps[base + k] : 0.0;
+    const double lp = on ? (double)a.lps[base + k] - lp_max : 0.0;
     const double x = on ? ((double)a.ex[base + k] - (double)mk) * rT : 0.0;
     const double ex = on ? exp(x) : 0.0, p = on ? exp(lp) : 0.0;
     a.ex[base + k] = (float)ex;
@@ -203,10 +212,10 @@ __global__ void __launch_bounds__(kTableWarps * 32) distill_table_kernel(const T
   dot = warp_sum(dot);
   if (lane == 0) {
     const double p_rest = a.drop ? 0.0 : fmax(1.0 - mass, kRestFloor);
-    const bool scale = a.drop && mass > 0.0;
+    const bool scale = a.drop && any;  // mass lies in [1, K] then
     a.sums[row] = TableSums{s, mass, dot, p_rest, (float)s, (float)mass, (float)p_rest,
                             a.drop ? 0.f : (float)log(p_rest), scale ? (float)(1.0 / mass) : 1.f,
-                            scale ? (float)log(mass) : 0.f, mk, any && !(a.drop && mass == 0.0)};
+                            scale ? (float)log(mass) : 0.f, mk, any};
   }
 }
 
@@ -279,7 +288,8 @@ __device__ __forceinline__ double finish_loss(const DistArgs& a, int row, const 
   log_s = log(s);
   const double lq_rest = has_rest ? ar + log(s_rest) - log_s : 0.0;
   const double p_rest = has_rest ? u.p_rest : 0.0, lp_rest = p_rest > 0.0 ? log(p_rest) : 0.0;
-  const double by = a.drop && u.mass > 0.0 ? 1.0 / u.mass : 1.0, log_by = a.drop && u.mass > 0.0 ? log(u.mass) : 0.0;
+  const bool scale = a.drop && u.any;
+  const double by = scale ? 1.0 / u.mass : 1.0, log_by = scale ? log(u.mass) : 0.0;
   double loss;
   if (a.div == kForward) {
     loss = by * u.dot + by * u.mass * (log_s - al - log_by);

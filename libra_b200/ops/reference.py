@@ -177,11 +177,13 @@ def distill_loss(logits, ids, lps, divergence: str, beta: float, tail: str, temp
     ninf = torch.full_like(z, float("-inf"))
     lq_rest = torch.logsumexp(torch.where(left.unsqueeze(1), torch.where(others, logq, ninf), torch.zeros_like(z)), 1)
     zero, one = torch.zeros_like(lp), torch.ones_like(lp)
+    if tail == "drop":  # only the ratios of the p count: relative to the row's largest, none of them underflows
+        most = torch.where(ok, lp, ninf[:, :1]).amax(1, keepdim=True)
+        lp = lp - torch.where(most > float("-inf"), most, zero[:, :1])
     p = torch.where(ok, torch.where(ok, lp, zero).exp(), zero)
     mass = p.sum(1)
     valid = ok.any(1) & ~dead
     if tail == "drop":
-        valid = valid & (mass > 0)
         by = torch.where(mass > 0, mass, torch.ones_like(mass)).unsqueeze(1)
         p, lp = p / by, lp - by.log()
         p_rest = torch.zeros_like(mass)

@@ -50,3 +50,25 @@ def test_distill_listed_tokens_that_the_student_all_but_excludes(device, T, div)
     _both_forms(z, ids, lps, lps, div, 0.5, "bucket", T)
     if div == "js":
         _both_forms(z, ids, lps, lps, div, 0.1, "drop", T)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("div", ["forward", "js"])
+def test_distill_drop_of_tables_with_little_mass(device, dtype, div):
+    """tail="drop" divides by the table's mass, however small: adding a constant to a row's logprobs changes nothing."""
+    levels = [0.0, -60.0, -86.0, -90.0, -110.0, -200.0, -700.0, -740.0, -800.0, -1e6]
+    g = torch.Generator().manual_seed(8)
+    z = torch.randn(len(levels), 500, generator=g).to(dtype).to(device)
+    base = torch.tensor([-0.5, -1.0, -3.0, -6.5, -0.5])
+    ids = torch.tensor([3, 40, 77, 499, 3])  # the last slot repeats a token, and does not count
+    at = torch.tensor(levels).unsqueeze(1)
+    for K in (1, 5):
+        row_ids = ids[:K].repeat(len(levels), 1).to(device)
+        lps = (at + base[:K]).to(device)  # (exact in fp32)
+        want = base[:K].repeat(len(levels), 1)
+        _both_forms(z, row_ids, lps, want, div, 0.4, "drop", 0.8)
+    # a second slot that does not count may be the likelier one
+    lps = torch.tensor([[-800.0, 0.0, -801.0]], device=device)
+    row_ids = torch.tensor([[5, 5, 9]], device=device)
+    _both_forms(z[:1], row_ids, lps, torch.tensor([[0.0, 0.0, -1.0]]), div, 0.4, "drop", 0.8)
