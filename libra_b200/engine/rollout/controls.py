@@ -30,7 +30,10 @@ class Grammar(Protocol):
 def allow_tokens(words: torch.Tensor, ids: Sequence[int], vocab_size: int) -> None:
     """Set the bits of ``ids`` (those inside the vocabulary) in a mask row."""
     allowed = torch.zeros(words.numel() * 32, dtype=torch.int64)
-    t = torch.as_tensor(list(ids), dtype=torch.int64)
+    try:
+        t = torch.as_tensor(list(ids), dtype=torch.int64)
+    except (RuntimeError, ValueError, OverflowError):  # an id beyond 64 bits is outside every vocabulary
+        t = torch.as_tensor([int(i) for i in ids if 0 <= i < vocab_size], dtype=torch.int64)
     allowed[t[(t >= 0) & (t < vocab_size)]] = 1
     bits = (allowed.view(-1, 32) << torch.arange(32)).sum(1)
     words |= torch.where(bits >= 2 ** 31, bits - 2 ** 32, bits).to(torch.int32)
@@ -62,28 +65,32 @@ class LogitControls:
     def prepare(self, req) -> str:
         """The mask of a request's next token, on the host before the step runs.
         Returns the finish reason if there is none to take ("grammar", or
-        "grammar_error" where its ``fill_mask`` raised), else ""."""
-        p = req.params
-        if p.grammar is None and p.allowed_token_ids is None:
+        "grammar_error" where building it raised), else ""."""
+        try:
+            words = self._build_mask(req)
+        except Exception as exc:  # noqa: BLE001 - the caller's code and values; only its own request ends
+            print(f"request {req.request_id}: grammar failed: {exc}")
+            return "grammar_error"
+        if words is None:
             return ""
-        rid = req.request_id
+        self._mask[req.request_id] = words
+        return "" if bool(words.any()) else "grammar"
+
+    def _build_mask(self, req) -> Optional[torch.Tensor]:
+        p, rid = req.params, req.request_id
         words = None
         if p.grammar is not None:
             words = torch.zeros(self.words, dtype=torch.int32)
-            try:
-                p.grammar.fill_mask(list(req.out), words)
-            except Exception as exc:  # noqa: BLE001 - the caller's code; only its own request ends
-                print(f"request {rid}: grammar failed: {exc}")
-                return "grammar_error"
+            p.grammar.fill_mask(list(req.out), words)
             if self.V % 32:
                 words[-1] &= (1 << (self.V % 32)) - 1
         if p.allowed_token_ids is not None:
             if rid not in self._static:
-                self._static[rid] = torch.zeros(self.words, dtype=torch.int32)
-                allow_tokens(self._static[rid], p.allowed_token_ids, self.V)
+                static = torch.zeros(self.words, dtype=torch.int32)
+                allow_tokens(static, p.allowed_token_ids, self.V)
+                self._static[rid] = static
             words = self._static[rid] if words is None else words & self._static[rid]
-        self._mask[rid] = words
-        return "" if bool(words.any()) else "grammar"
+        return words
 
     # ------------------------------------------------------------------ histories
     def _up(self, t: torch.Tensor) -> torch.Tensor:

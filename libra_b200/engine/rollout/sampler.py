@@ -42,8 +42,13 @@ class SamplingParams:
             self.logit_bias = {int(k): float(v) for k, v in self.logit_bias.items()}
             if not all(math.isfinite(v) and 0 <= k < 2 ** 31 for k, v in self.logit_bias.items()):
                 raise ValueError("logit_bias maps token ids to finite numbers")
-        if self.allowed_token_ids is not None and not len(self.allowed_token_ids):
-            raise ValueError("allowed_token_ids must not be empty")
+        if self.allowed_token_ids is not None:
+            try:
+                self.allowed_token_ids = [int(t) for t in self.allowed_token_ids]
+            except (TypeError, ValueError, OverflowError) as exc:
+                raise ValueError(f"allowed_token_ids must be token ids: {exc}") from exc
+            if not self.allowed_token_ids:
+                raise ValueError("allowed_token_ids must not be empty")
         if not 0 <= int(self.top_logprobs) <= 256:
             raise ValueError(f"top_logprobs must lie in [0, 256], got {self.top_logprobs}")
 
@@ -68,7 +73,7 @@ def extra_sampling(kw: Dict[str, Any]) -> Dict[str, Any]:
             "allowed_token_ids": lambda v: [int(t) for t in v], "top_logprobs": int}
     try:
         return {k: cast.get(k, float)(kw[k]) for k in EXTRA_SAMPLING_KEYS if kw.get(k) is not None}
-    except (TypeError, AttributeError) as exc:
+    except (TypeError, AttributeError, OverflowError) as exc:
         raise ValueError(f"bad sampling argument: {exc}") from exc
 
 
