@@ -246,8 +246,12 @@ class LLMEngine:
             raise ValueError("generate_sync: one SamplingParams per prompt")
         ids = [self.add_request(p, sp or SamplingParams(), callback=lambda r: results.__setitem__(r.request_id, r))
                for p, sp in zip(prompts, plist)]
-        while len(results) < len(ids):
-            self.step()
+        try:
+            while len(results) < len(ids):
+                self.step()
+        except Exception as exc:
+            self._fail_all(exc)  # as the background loop does: nothing of the batch stays behind
+            raise
         return [results[i] for i in ids]
 
     # ------------------------------------------------------------------ background loop
@@ -519,6 +523,7 @@ class LLMEngine:
                         and not r.params.top_logprobs for r in decode)
                 and self._graph_runner() is not None):
             return self._decode_step_graph(decode, t0)
+        self.running = self.running + admitted  # from here on _fail_all finds them, should the step raise
         batch = self._prepare_controls(admitted + decode)
         if not batch:
             return 0
@@ -588,7 +593,7 @@ class LLMEngine:
             else:
                 still.append(r)
         keep = {id(r) for r in still}
-        self.running = [r for r in self.running if id(r) in keep] + [r for r in admitted if id(r) in keep]
+        self.running = [r for r in self.running if id(r) in keep]
         self.stats["steps"] += 1
         self.stats["busy_s"] += time.perf_counter() - t0
         return len(batch)

@@ -79,3 +79,47 @@ def test_allow_tokens_ignores_ids_of_any_size():
     words = torch.zeros(2, dtype=torch.int32)
     allow_tokens(words, [0, 31, 33, 2 ** 64, -5, 40], 40)
     assert [v for v in range(64) if (int(words[v // 32]) >> (v % 32)) & 1] == [0, 31, 33]
+
+
+@pytest.mark.parametrize("where", ["model", "controls", "sampler"])
+def test_a_step_that_raises_answers_and_frees_the_requests_it_admitted(llm, where, monkeypatch):
+    from libra_b200.engine.rollout import llm_engine
+
+    def broken(*a, **kw):
+        raise RuntimeError("broken step")
+
+    apply = llm._controls.apply
+
+    def apply_then_break(*a):
+        apply(*a)  # (the request has its history row by then)
+        broken()
+
+    penalized = SamplingParams(max_tokens=3, temperature=0.0, frequency_penalty=0.5)
+    for _ in range(llm.max_running + 1):  # more often than there are rows
+        with monkeypatch.context() as m:
+            if where == "model":
+                m.setattr(llm.runner, "step", broken)
+            elif where == "controls":
+                m.setattr(llm._controls, "apply", apply_then_break)
+            else:
+                m.setattr(llm_engine, "sample", broken)
+            with pytest.raises(RuntimeError, match="broken step"):
+                asyncio.run(asyncio.wait_for(llm.generate([1, 2, 3], penalized), 30))
+            llm.pause(30)
+        assert _clean(llm)
+        llm.resume()
+    (res,) = [asyncio.run(asyncio.wait_for(llm.generate([1, 2, 3], penalized), 30))]
+    assert len(res.output_tokens) == 3
+
+
+def test_a_blocking_batch_that_raises_leaves_the_engine_clean(llm, monkeypatch):
+    def broken(*a, **kw):
+        raise RuntimeError("broken step")
+
+    p = SamplingParams(max_tokens=3, temperature=0.0, frequency_penalty=0.5)
+    with monkeypatch.context() as m:
+        m.setattr(llm.runner, "step", broken)
+        with pytest.raises(RuntimeError, match="broken step"):
+            llm.generate_sync([[1, 2], [3, 4]], p)
+    assert _clean(llm)
+    assert [len(r.output_tokens) for r in llm.generate_sync([[1, 2], [3, 4]], p)] == [3, 3]
