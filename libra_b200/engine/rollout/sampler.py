@@ -14,6 +14,12 @@ from typing import Any, Dict, List, Optional
 
 import torch
 
+# The controls are applied in fp32.  Lowering a logit may take it to -inf, which excludes the token, but no control may
+# raise one out of fp32 (its softmax would be NaN): not with 2^31 occurrences, nor divided by a small temperature.
+_MOST_LOWER = 3.4e38
+_MOST_RAISE = 1e20
+_REPETITION_RANGE = (1e-20, 1e20)
+
 
 @dataclass
 class SamplingParams:
@@ -33,15 +39,16 @@ class SamplingParams:
     top_logprobs: int = 0               # most likely tokens to report beside each sampled one
 
     def __post_init__(self):
-        if not (self.repetition_penalty > 0 and math.isfinite(self.repetition_penalty)):
-            raise ValueError(f"repetition_penalty must be above 0, got {self.repetition_penalty}")
+        lo, hi = _REPETITION_RANGE
+        if not lo <= self.repetition_penalty <= hi:
+            raise ValueError(f"repetition_penalty must lie in [{lo}, {hi}], got {self.repetition_penalty}")
         for name in ("presence_penalty", "frequency_penalty"):
-            if not math.isfinite(getattr(self, name)):
-                raise ValueError(f"{name} must be finite, got {getattr(self, name)}")
+            if not -_MOST_RAISE <= getattr(self, name) <= _MOST_LOWER:
+                raise ValueError(f"{name} must lie in [{-_MOST_RAISE}, {_MOST_LOWER}], got {getattr(self, name)}")
         if self.logit_bias:
             self.logit_bias = {int(k): float(v) for k, v in self.logit_bias.items()}
-            if not all(math.isfinite(v) and 0 <= k < 2 ** 31 for k, v in self.logit_bias.items()):
-                raise ValueError("logit_bias maps token ids to finite numbers")
+            if not all(-_MOST_LOWER <= v <= _MOST_RAISE and 0 <= k < 2 ** 31 for k, v in self.logit_bias.items()):
+                raise ValueError(f"logit_bias maps token ids to numbers in [{-_MOST_LOWER}, {_MOST_RAISE}]")
         if self.allowed_token_ids is not None:
             try:
                 self.allowed_token_ids = [int(t) for t in self.allowed_token_ids]
