@@ -56,8 +56,9 @@ class SamplingParams:
                 raise ValueError(f"allowed_token_ids must be token ids: {exc}") from exc
             if not self.allowed_token_ids:
                 raise ValueError("allowed_token_ids must not be empty")
-        if not 0 <= int(self.top_logprobs) <= 256:
-            raise ValueError(f"top_logprobs must lie in [0, 256], got {self.top_logprobs}")
+        if self.top_logprobs not in range(257):
+            raise ValueError(f"top_logprobs must be a whole number in [0, 256], got {self.top_logprobs}")
+        self.top_logprobs = int(self.top_logprobs)
 
     @property
     def penalized(self) -> bool:

@@ -1,6 +1,7 @@
 """Sampling arguments at the ends of what fp32 holds, where the engine uses them."""
 
 import asyncio
+import math
 
 import pytest
 
@@ -44,6 +45,16 @@ def test_controls_at_their_limits_leave_a_distribution(device):
             assert len(r.output_tokens) == 5, kw
             assert all(v == v and v < 1e-3 for v in r.output_logprobs), (kw, r.output_logprobs)
             assert all(v == v for row in r.output_top_logprobs for _, v in row), kw
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_top_logprobs_is_a_whole_number(device):
+    for bad in (2.5, "x", None, math.inf):
+        with pytest.raises(ValueError, match="top_logprobs"):
+            SamplingParams(top_logprobs=bad)
+    llm = _llm(device)
+    (r,) = llm.generate_sync([[1, 2, 3]], SamplingParams(max_tokens=2, temperature=0.0, top_logprobs=2.0))
+    assert [len(row) for row in r.output_top_logprobs] == [2, 2]
 
 
 def test_server_answers_400_for_controls_beyond_fp32():
