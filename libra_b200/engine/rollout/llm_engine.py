@@ -221,7 +221,8 @@ class LLMEngine:
             gen.manual_seed(int(params.seed))
         req = _Request(rid, list(int(t) for t in prompt_tokens), params, future=future, loop=loop, callback=callback,
                        generator=gen)
-        req.seed = int(params.seed) if params.seed is not None else int(
+        # the samplers' key is 64 bits wide, held as a signed number
+        req.seed = (int(params.seed) + 2 ** 63) % 2 ** 64 - 2 ** 63 if params.seed is not None else int(
             torch.randint(0, 2 ** 62, (1,), generator=self._seed_rng))
         with self._lock:
             self.waiting.append(req)

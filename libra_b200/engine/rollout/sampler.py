@@ -39,6 +39,7 @@ class SamplingParams:
     top_logprobs: int = 0               # most likely tokens to report beside each sampled one
 
     def __post_init__(self):
+        self.top_k = max(-1, min(int(self.top_k), 2 ** 31 - 1))  # (no vocabulary is larger: no filter)
         lo, hi = _REPETITION_RANGE
         if not lo <= self.repetition_penalty <= hi:
             raise ValueError(f"repetition_penalty must lie in [{lo}, {hi}], got {self.repetition_penalty}")

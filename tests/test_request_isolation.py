@@ -123,3 +123,19 @@ def test_a_blocking_batch_that_raises_leaves_the_engine_clean(llm, monkeypatch):
             llm.generate_sync([[1, 2], [3, 4]], p)
     assert _clean(llm)
     assert [len(r.output_tokens) for r in llm.generate_sync([[1, 2], [3, 4]], p)] == [3, 3]
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("kw", [dict(top_k=2 ** 70), dict(top_k=-2 ** 70), dict(seed=2 ** 63 + 5), dict(seed=2 ** 64 - 1)])
+def test_seeds_and_top_k_beyond_63_bits(device, kw):
+    from libra_b200.engine.train_engine import B200TrainEngine
+
+    eng = B200TrainEngine("tiny" if device == "cpu" else "tiny-gpu", device=device, seed=3)
+    eng.initialize()
+    llm = LLMEngine(eng.cfg, {k: v.detach() for k, v in eng.params.items()}, kv_blocks=64, block_size=16, max_running=4)
+    plain = SamplingParams(max_tokens=6, temperature=0.0)
+    for extra in ({}, {"presence_penalty": 0.1}):  # through the captured and the eager decode
+        a, b = llm.generate_sync([[1, 2], [3, 4]], [plain, SamplingParams(max_tokens=6, **kw, **extra)])
+        assert len(a.output_tokens) == len(b.output_tokens) == 6
+    llm.add_request([1], SamplingParams(**{"seed": 1, **kw}))
+    assert -2 ** 63 <= llm.waiting[0].seed < 2 ** 63
