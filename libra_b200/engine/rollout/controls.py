@@ -148,7 +148,9 @@ class LogitControls:
             i = self._up(torch.tensor([[self._row.get(r.request_id, 0) for r in reqs],
                                        [r.n_tokens if r.params.penalized else 0 for r in reqs],
                                        [len(r.prompt) for r in reqs]], dtype=torch.int32))
-            kw.update(history=self.table, history_rows=i[0], history_lens=i[1], prompt_lens=i[2], repetition=f[0],
+            # the table as wide as this batch needs it: the kernel takes smaller counters for short histories, and the
+            # table keeps the width of the longest request it ever held
+            kw.update(history=self.table[:, :max(r.n_tokens for r in pen)], history_rows=i[0], history_lens=i[1], prompt_lens=i[2], repetition=f[0],
                       presence=f[1], frequency=f[2])
         if any(p.logit_bias for p in ps):
             offs, ids, vals = [0], [], []
