@@ -26,7 +26,8 @@ namespace vocab {
 constexpr int kCtlThreads = 512;
 
 struct CtlArgs {
-  const int* hist;          // [H, hist_w]
+  bool has_hist, has_mask;  // (a table without rows has no address)
+  const int* hist;          // [H, hist_w] or null
   int64_t hist_ld;
   int hist_rows_n, hist_w;
   const int* hist_rows;     // [B] or null: row b
@@ -123,7 +124,7 @@ __global__ void __launch_bounds__(kCtlThreads, 3) control_kernel(const TI* logit
   bool bad = false;
   int len = 0, prompt = 0;
   const int* h = nullptr;
-  if (a.hist && (rep != 1.f || pen.pres != 0.f || pen.freq != 0.f)) {
+  if (a.has_hist && (rep != 1.f || pen.pres != 0.f || pen.freq != 0.f)) {
     const int hr = a.hist_rows ? a.hist_rows[b] : b;
     len = a.hist_lens[b];
     const bool in = hr >= 0 && hr < a.hist_rows_n;
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(kCtlThreads, 3) control_kernel(const TI* logit
     }
   }
   const int* mask = nullptr;
-  if (a.mask) {
+  if (a.has_mask) {
     const int mr = a.mask_rows ? a.mask_rows[b] : b;
     bad = bad || mr >= a.mask_n;
     if (mr >= 0 && mr < a.mask_n) mask = a.mask + (int64_t)mr * a.mask_ld;
@@ -287,6 +288,7 @@ void control_logits(torch::Tensor logits, c10::optional<torch::Tensor> history,
                 "control_logits: history must be int32 [H, L] on the logits' device, unit inner stride");
     LIBRA_CHECK(history_lens.has_value(), "control_logits: history needs history_lens");
     LIBRA_CHECK(history_rows.has_value() || history->size(0) >= B, "control_logits: history has fewer rows than logits");
+    a.has_hist = true;
     a.hist = history->data_ptr<int>();
     a.hist_ld = history->stride(0);
     a.hist_rows_n = (int)history->size(0);
@@ -313,6 +315,7 @@ void control_logits(torch::Tensor logits, c10::optional<torch::Tensor> history,
                     mask->size(0) < (1ll << 31),
                 "control_logits: mask must be int32 [M, ceil(V / 32)] on the logits' device, unit inner stride");
     LIBRA_CHECK(mask_rows.has_value() || mask->size(0) >= B, "control_logits: mask has fewer rows than logits");
+    a.has_mask = true;
     a.mask = mask->data_ptr<int>();
     a.mask_ld = mask->stride(0);
     a.mask_n = (int)mask->size(0);
@@ -328,7 +331,7 @@ void control_logits(torch::Tensor logits, c10::optional<torch::Tensor> history,
   int tile = 32768;
   while (tile > 2048 && (int64_t)B * ((V + tile - 1) / tile) < 3 * 148) tile /= 2;
   const int tiles = std::max(1, (V / 8 + tile / 8 - 1) / (tile / 8));
-  const bool wide = a.hist && a.hist_w >= (1 << 15);  // 16-bit counters hold 2^15 - 1 occurrences
+  const bool wide = a.has_hist && a.hist_w >= (1 << 15);  // 16-bit counters hold 2^15 - 1 occurrences
   const size_t smem = (size_t)(tile + 32) * (wide ? 4 : 2) + (tile + 32) / 8;
   auto go = [&](auto* in, auto* o) {
     using I = std::remove_const_t<std::remove_pointer_t<decltype(in)>>;

@@ -1,0 +1,40 @@
+"""What the vocabulary-row operators promise about their arguments: bad indices,
+gradients, in-place outputs, arguments that a form does not use."""
+
+import pytest
+import torch
+
+from libra_b200 import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _raises_outside(device, call):
+    """A bad index raises on the CPU; the kernels report it through the error word."""
+    if device == "cpu":
+        with pytest.raises(ValueError, match="outside"):
+            call()
+        return
+    dev = torch.device("cuda", torch.cuda.current_device())
+    ops.check_kernel_errors(dev)
+    call()
+    with pytest.raises(ops.KernelError, match="bad argument"):
+        ops.check_kernel_errors(dev)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_control_logits_with_empty_tables(device):
+    z = torch.randn(2, 100, generator=torch.Generator().manual_seed(1)).to(device)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=device)  # noqa: E731
+    rep = torch.tensor([1.5, 1.5], device=device)
+    no_mask = torch.zeros(0, 4, dtype=torch.int32, device=device)
+    out = ops.control_logits(z, mask=no_mask, mask_rows=i32(-1, -1))
+    assert torch.equal(out, z)
+    _raises_outside(device, lambda: ops.control_logits(z, mask=no_mask, mask_rows=i32(-1, 0)))
+    no_width = torch.zeros(2, 0, dtype=torch.int32, device=device)
+    out = ops.control_logits(z, history=no_width, history_lens=i32(0, 0), repetition=rep)
+    assert torch.equal(out, z)
+    _raises_outside(device, lambda: ops.control_logits(z, history=no_width, history_lens=i32(0, 1), repetition=rep))
+    no_rows = torch.zeros(0, 8, dtype=torch.int32, device=device)
+    _raises_outside(device, lambda: ops.control_logits(z, history=no_rows, history_rows=i32(0, 0),
+                                                       history_lens=i32(1, 1), repetition=rep))
