@@ -30,6 +30,7 @@ def _rows(logits: torch.Tensor, op: str) -> torch.Tensor:
     return logits
 
 
+@torch.no_grad()
 def control_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None,
                    history_lens: Optional[torch.Tensor] = None, prompt_lens: Optional[torch.Tensor] = None,
                    history_rows: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
@@ -84,6 +85,7 @@ def control_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     return out
 
 
+@torch.no_grad()
 def top_logprobs(logits: torch.Tensor, k: int, temperature: Union[float, torch.Tensor] = 1.0
                  ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The ``k`` (1 to 256) largest logits of every row [N, V], in descending

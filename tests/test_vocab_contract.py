@@ -38,3 +38,16 @@ def test_control_logits_with_empty_tables(device):
     no_rows = torch.zeros(0, 8, dtype=torch.int32, device=device)
     _raises_outside(device, lambda: ops.control_logits(z, history=no_rows, history_rows=i32(0, 0),
                                                        history_lens=i32(1, 1), repetition=rep))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_controls_and_top_logprobs_are_not_differentiated_through(device):
+    x = torch.randn(3, 200, generator=torch.Generator().manual_seed(1)).to(device).requires_grad_(True)
+    frequency, presence = torch.ones(3, device=device), torch.ones(3, device=device)
+    hist = torch.ones(3, 2, dtype=torch.int32, device=device)
+    lens = torch.full((3,), 2, dtype=torch.int32, device=device)
+    kw = dict(history=hist, history_lens=lens, frequency=frequency, presence=presence)
+    assert not ops.control_logits(x, **kw).requires_grad
+    assert not any(t.requires_grad for t in ops.top_logprobs(x, 4))
+    assert not any(t.requires_grad for t in ops.distill_loss_grad(x, torch.ones(3, 1, dtype=torch.long, device=device),
+                                                                  torch.zeros(3, 1, device=device)))
