@@ -22,6 +22,12 @@ DIVERGENCES = {"forward": 0, "reverse": 1, "js": 2}
 TAILS = ("bucket", "drop")
 
 
+def _written(out: torch.Tensor) -> None:
+    """A kernel wrote to a caller's tensor: autograd then refuses a backward pass that saved its old values."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 def _rows(logits: torch.Tensor, op: str) -> torch.Tensor:
     if logits.dim() != 2:
         raise ValueError(f"{op}: logits must be [rows, vocabulary], got {tuple(logits.shape)}")
@@ -80,6 +86,8 @@ def control_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
 
     if out is None:
         out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+    else:
+        _written(out)
     ext().control_logits(logits, history, history_rows, history_lens, prompt_lens, repetition, presence, frequency,
                          bias_offsets, bias_ids, bias_values, mask, mask_rows, out, error_flag(logits.device))
     return out
@@ -181,6 +189,8 @@ def distill_loss_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
 
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    else:
+        _written(out)
     loss = ext().distill_onepass(logits, teacher_ids.contiguous(), teacher_logprobs.contiguous(),
                                  DIVERGENCES[divergence], float(beta), tail == "drop", float(temperature), out,
                                  error_flag(logits.device))

@@ -51,3 +51,22 @@ def test_controls_and_top_logprobs_are_not_differentiated_through(device):
     assert not any(t.requires_grad for t in ops.top_logprobs(x, 4))
     assert not any(t.requires_grad for t in ops.distill_loss_grad(x, torch.ones(3, 1, dtype=torch.long, device=device),
                                                                   torch.zeros(3, 1, device=device)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", ["control_logits", "distill_loss_grad"])
+def test_logits_overwritten_before_their_backward_pass_are_noticed(device, which):
+    x = torch.randn(2, 64, generator=torch.Generator().manual_seed(1)).to(device).requires_grad_(True)
+    ids = torch.tensor([[1, 2], [3, 4]], device=device)
+    lps = torch.log(torch.tensor([[0.5, 0.2], [0.3, 0.3]], device=device))
+    y = x * 1.0
+    loss = y.exp().sum()  # (keeps exp(y); y * y keeps y itself)
+    loss = loss + (y * y).sum()
+    before = y._version
+    if which == "control_logits":
+        assert ops.control_logits(y, mask=torch.zeros(2, 2, dtype=torch.int32, device=device), out=y) is y
+    else:
+        assert ops.distill_loss_grad(y, ids, lps, out=y)[1] is y
+    assert y._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
