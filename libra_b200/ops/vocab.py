@@ -116,7 +116,8 @@ def top_logprobs(logits: torch.Tensor, k: int, temperature: Union[float, torch.T
                                     1.0 if per_row else float(temperature)))
 
 
-def _check_distill(op: str, logits, ids, lps, divergence, beta, tail, temperature) -> None:
+def _check_distill(op: str, logits, ids, lps, divergence, beta, tail, temperature) -> float:
+    """Checks the arguments; returns the beta to use (a fixed one where the divergence has none)."""
     if divergence not in DIVERGENCES:
         raise ValueError(f"{op}: divergence must be one of {sorted(DIVERGENCES)}, got {divergence!r}")
     if tail not in TAILS:
@@ -132,6 +133,7 @@ def _check_distill(op: str, logits, ids, lps, divergence, beta, tail, temperatur
                          f"{tuple(lps.shape)} for {logits.shape[0]} rows")
     if not 1 <= ids.shape[1] <= MAX_TOP:
         raise ValueError(f"{op}: 1 to {MAX_TOP} teacher tokens a row, got {ids.shape[1]}")
+    return float(beta) if divergence == "js" else 0.5
 
 
 def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, *,
@@ -156,7 +158,7 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logpro
     vocabulary have logprob -inf and no gradient, and set the error word that
     ``check_kernel_errors`` raises (ValueError on the CPU)."""
     logits = _rows(logits, "distill_loss")
-    _check_distill("distill_loss", logits, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature)
+    beta = _check_distill("distill_loss", logits, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature)
     if logits.device.type != "cuda":
         loss, logp = ref.distill_loss(logits, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature,
                                       targets)
@@ -164,7 +166,7 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logpro
         from . import error_flag, ext
 
         loss, logp = ext().distill_loss(logits, teacher_ids.contiguous(), teacher_logprobs.contiguous(),
-                                        DIVERGENCES[divergence], float(beta), tail == "drop", float(temperature),
+                                        DIVERGENCES[divergence], beta, tail == "drop", float(temperature),
                                         None if targets is None else targets.contiguous(),
                                         error_flag(logits.device))
     return loss if targets is None else (loss, logp)
@@ -178,7 +180,8 @@ def distill_loss_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     an upstream gradient of one: (loss fp32 [N], gradient [N, V] of the
     logits' type).  ``out``: where the gradient goes; it may be ``logits``."""
     logits = _rows(logits, "distill_loss_grad")
-    _check_distill("distill_loss_grad", logits, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature)
+    beta = _check_distill("distill_loss_grad", logits, teacher_ids, teacher_logprobs, divergence, beta, tail,
+                          temperature)
     if logits.device.type != "cuda":
         with torch.enable_grad():
             z = logits.detach().clone().requires_grad_(True)
@@ -192,7 +195,7 @@ def distill_loss_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     else:
         _written(out)
     loss = ext().distill_onepass(logits, teacher_ids.contiguous(), teacher_logprobs.contiguous(),
-                                 DIVERGENCES[divergence], float(beta), tail == "drop", float(temperature), out,
+                                 DIVERGENCES[divergence], beta, tail == "drop", float(temperature), out,
                                  error_flag(logits.device))
     return loss, out
 
@@ -282,7 +285,7 @@ def lm_head_distill(h: torch.Tensor, w: torch.Tensor, teacher_ids: torch.Tensor,
     ``main_grad`` when it has one.  With ``targets`` int64 [R] the result is
     (loss, logprob of the targets), GRPO's logprobs and the distillation loss
     from one LM head product.  The backward pass runs once."""
-    _check_distill("lm_head_distill", h, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature)
+    beta = _check_distill("lm_head_distill", h, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature)
     if h.dim() != 2 or w.dim() != 2 or h.shape[1] != w.shape[1]:
         raise ValueError(f"lm_head_distill: h [R, H] and w [V, H], got {tuple(h.shape)} and {tuple(w.shape)}")
     if h.device.type != "cuda":
@@ -290,7 +293,7 @@ def lm_head_distill(h: torch.Tensor, w: torch.Tensor, teacher_ids: torch.Tensor,
         loss, logp = ref.distill_loss(logits, teacher_ids, teacher_logprobs, divergence, beta, tail, temperature,
                                       targets)
     else:
-        kind = (DIVERGENCES[divergence], float(beta), tail == "drop", float(temperature))
+        kind = (DIVERGENCES[divergence], beta, tail == "drop", float(temperature))
         loss, logp = _LMHeadDistill.apply(h.contiguous(), w, teacher_ids.contiguous(), teacher_logprobs.contiguous(),
                                           kind, None if targets is None else targets.contiguous())
     return loss if targets is None else (loss, logp)

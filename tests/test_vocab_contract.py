@@ -70,3 +70,20 @@ def test_logits_overwritten_before_their_backward_pass_are_noticed(device, which
     assert y._version > before
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("beta", [0.0, 1.0, 7.0])
+def test_beta_belongs_to_js_alone(device, beta):
+    z = torch.randn(2, 64, generator=torch.Generator().manual_seed(1)).to(device)
+    ids = torch.tensor([[1, 2], [3, 4]], device=device)
+    lps = torch.log(torch.tensor([[0.5, 0.2], [0.3, 0.3]], device=device))
+    for div in ("forward", "reverse"):
+        want = ops.distill_loss_grad(z, ids, lps, divergence=div)
+        assert all(torch.equal(a, b) for a, b in zip(want, ops.distill_loss_grad(z, ids, lps, divergence=div, beta=beta)))
+        assert torch.equal(want[0], ops.distill_loss(z, ids, lps, divergence=div, beta=beta))
+    w, h = torch.randn(64, 64).bfloat16().to(device), torch.randn(2, 64).bfloat16().to(device)
+    assert torch.equal(ops.lm_head_distill(h, w, ids, lps, beta=beta), ops.lm_head_distill(h, w, ids, lps))
+    for f in (ops.distill_loss, ops.distill_loss_grad):
+        with pytest.raises(ValueError, match="beta"):
+            f(z, ids, lps, divergence="js", beta=beta)
