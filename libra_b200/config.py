@@ -545,7 +545,8 @@ class AsyncRLConfig:
     micro_batch_size: int = 4
     kl_coef: float = 0.001
     clip_epsilon: float = 0.2
-    # weight and divergence (forward, reverse, js) of the distillation loss for trajectories with a teacher's top logprobs
+    # weight and divergence (forward, reverse, js) of the distillation loss for trajectories that carry a teacher's top
+    # logprobs; the caller puts them there (a teacher engine's score_teacher), the trainer makes none itself
     distill_coef: float = 0.0
     distill_divergence: str = "forward"
     gamma: float = 1.0

@@ -25,6 +25,7 @@ reference's three backends (FSDP, Megatron3D, Megatron-Core) with one engine:
 
 from __future__ import annotations
 
+import logging
 import math
 import os
 import time
@@ -38,6 +39,8 @@ from libra_b200 import ops
 from libra_b200.models.qwen3 import (PackedBatch, ParamLayout, Qwen3Config, Qwen3Model, get_config, init_params,
                                      is_expert_param, pack_sequences, param_shapes)
 from libra_b200.utils import nvtx
+
+log = logging.getLogger(__name__)
 
 
 class TrainEngine(Protocol):
@@ -102,6 +105,7 @@ class B200TrainEngine:
         # weight of the distillation loss in grpo_update, for trajectories that carry a teacher's top logprobs
         # ("teacher_ids" / "teacher_logprobs", see score_teacher)
         self.distill_coef, self.distill_divergence = float(distill_coef), str(distill_divergence)
+        self._warned_no_teacher = False
         if self.distill_divergence not in ("forward", "reverse", "js"):
             raise ValueError(f"distill_divergence must be forward, reverse or js, got {distill_divergence!r}")
         if self.distill_coef < 0.0:
@@ -645,6 +649,10 @@ class B200TrainEngine:
 
     def prepare_update(self, trajectories: List[Dict[str, Any]]) -> List[Dict[str, Any]]:
         """Host-side packed execution chunks (with loss weights) for one update."""
+        if self.distill_coef > 0.0 and not self._warned_no_teacher and not any("teacher_ids" in t for t in trajectories):
+            self._warned_no_teacher = True
+            log.warning("distill_coef is %g, but none of these trajectories has a teacher's tables (teacher_ids, "
+                        "teacher_logprobs; see score_teacher): the update has no distillation term", self.distill_coef)
         w = self.loss_weights(trajectories)
         return [self.pack([trajectories[i] for i in idx], True, [w[i] for i in idx])
                 for idx in self._align_chunks(self.chunk_by_tokens(trajectories, self.max_tokens_per_micro_batch))]
