@@ -619,19 +619,20 @@ static void check_distill(const torch::Tensor& logits, const torch::Tensor& ids,
               "%s: divergence, beta or temperature", op);
 }
 
-// The tables' memory in one allocation: sums, slices' parts, tokens, exp(x), p, x - log p.
+// The tables' memory in one allocation: sums, slices' parts, exp(x), p, x - log p, and the tokens unless a.clean has a
+// place for them.
 static torch::Tensor alloc_tables(DistArgs& a, const torch::Tensor& logits, int64_t splits) {
   const int64_t NK = (int64_t)a.N * a.K, per = sizeof(TableSums) / 4;
-  auto buf = torch::empty({a.N * (per + 2 * splits) + 4 * NK}, logits.options().dtype(at::kFloat));
+  auto buf = torch::empty({a.N * (per + 2 * splits) + (a.clean ? 3 : 4) * NK}, logits.options().dtype(at::kFloat));
   float* p = buf.data_ptr<float>();
   a.sums = reinterpret_cast<TableSums*>(p);
   p += a.N * per;
   a.parts = reinterpret_cast<MaxSum*>(p);
   p += a.N * 2 * splits;
-  a.clean = reinterpret_cast<int*>(p);
-  a.ex = p + NK;
-  a.p = p + 2 * NK;
-  a.xl = p + 3 * NK;
+  a.ex = p;
+  a.p = p + NK;
+  a.xl = p + 2 * NK;
+  if (!a.clean) a.clean = reinterpret_cast<int*>(p + 3 * NK);
   return buf;
 }
 
@@ -670,11 +671,11 @@ std::vector<torch::Tensor> distill_fwd(torch::Tensor logits, torch::Tensor ids, 
   const int64_t NK = (int64_t)N * K;
   auto saved = torch::empty({4 * (int64_t)N + 3 * NK}, f32);
   if (N == 0) return {loss, logp, saved};
-  auto work = alloc_tables(a, logits, n);
   a.stats = saved.data_ptr<float>();
   a.dk = a.stats + 4 * (int64_t)N;
   a.qk = a.dk + NK;
   a.clean = reinterpret_cast<int*>(a.qk + NK);
+  auto work = alloc_tables(a, logits, n);
   a.targets = targets.has_value() ? targets->data_ptr<int64_t>() : nullptr;
   a.logp = logp.data_ptr<float>();
   cudaStream_t st = at::cuda::getCurrentCUDAStream();

@@ -247,11 +247,6 @@ __device__ __forceinline__ unsigned long long ld_cluster(const unsigned long lon
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ double ld_cluster(const double* p, uint32_t rank) {
-  double v;
-  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
-  return v;
-}
 __device__ __forceinline__ void cluster_arrive() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
