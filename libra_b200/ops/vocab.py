@@ -36,7 +36,6 @@ def _rows(logits: torch.Tensor, op: str) -> torch.Tensor:
     return logits
 
 
-@torch.no_grad()
 def control_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None,
                    history_lens: Optional[torch.Tensor] = None, prompt_lens: Optional[torch.Tensor] = None,
                    history_rows: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
@@ -79,9 +78,10 @@ def control_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     if history is not None and history_lens is None:
         raise ValueError("control_logits: history needs history_lens")
     if logits.device.type != "cuda":
-        res = ref.control_logits(logits, history, history_lens, prompt_lens, history_rows, repetition, presence,
-                                 frequency, bias_offsets, bias_ids, bias_values, mask, mask_rows)
-        return res if out is None else out.copy_(res)
+        with torch.no_grad():
+            res = ref.control_logits(logits, history, history_lens, prompt_lens, history_rows, repetition, presence,
+                                     frequency, bias_offsets, bias_ids, bias_values, mask, mask_rows)
+            return res if out is None else out.copy_(res)
     from . import error_flag, ext
 
     if out is None:
@@ -93,7 +93,6 @@ def control_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     return out
 
 
-@torch.no_grad()
 def top_logprobs(logits: torch.Tensor, k: int, temperature: Union[float, torch.Tensor] = 1.0
                  ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The ``k`` (1 to 256) largest logits of every row [N, V], in descending
@@ -109,7 +108,8 @@ def top_logprobs(logits: torch.Tensor, k: int, temperature: Union[float, torch.T
         raise ValueError(f"top_logprobs: k must lie in [1, {min(MAX_TOP, logits.shape[1])}], got {k}")
     per_row = isinstance(temperature, torch.Tensor)
     if logits.device.type != "cuda":
-        return ref.top_logprobs(logits, k, temperature)
+        with torch.no_grad():
+            return ref.top_logprobs(logits, k, temperature)
     from . import ext
 
     return tuple(ext().top_logprobs(logits.detach(), k, temperature if per_row else None,
