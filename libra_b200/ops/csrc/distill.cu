@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kTableWarps * 32) distill_table_kernel(const T
   for (int i = lane; i < kHash; i += 32) hash[i] = -1;
   __syncwarp();
   bool twice = false, any = false;
-  float mk = -FLT_MAX;
+  float mk = -FLT_MAX, most = -INFINITY;  // of the listed logits and of their logprobs
   for (int k = lane; k < K; k += 32) {
     float lp;
     const int id = slot_token(a, base + k, V, lp);
@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(kTableWarps * 32) distill_table_kernel(const T
     if (id < 0) continue;
     any = true;
     mk = fmaxf(mk, v);
+    most = fmaxf(most, lp);
     unsigned h = ((unsigned)id * 2654435761u) >> 23;
     while (true) {  // at most 256 of the 512 places are taken
       const int old = atomicCAS(&hash[h], -1, id);
@@ -182,18 +183,15 @@ __global__ void __launch_bounds__(kTableWarps * 32) distill_table_kernel(const T
       if (k < K) ids[k] = id;
       __syncwarp();
     }
+    most = -INFINITY;
+    for (int k = lane; k < K; k += 32)
+      if (ids[k] >= 0) most = fmaxf(most, a.lps[base + k]);
   }
   mk = warp_max(mk);
   any = __any_sync(0xffffffffu, any);
   // tail = drop: relative to the row's largest, since only the ratios of the p count and none of them may underflow
-  double lp_max = 0.0;
-  if (a.drop) {
-    float most = -INFINITY;
-    for (int k = lane; k < K; k += 32)
-      if (ids[k] >= 0) most = fmaxf(most, a.lps[base + k]);
-    most = warp_max(most);
-    if (most > -INFINITY) lp_max = (double)most;
-  }
+  most = warp_max(most);
+  const double lp_max = a.drop && any ? (double)most : 0.0;
   double s = 0.0, mass = 0.0, dot = 0.0;
   for (int k = lane; k < K; k += 32) {
     const bool on = ids[k] >= 0;
