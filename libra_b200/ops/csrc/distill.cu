@@ -230,7 +230,8 @@ __device__ __forceinline__ float slot_grad(const DistArgs& a, const RowFin& f, f
   return q == 0.f ? 0.f : q * (bucket_h(a, xl + f.off) - f.mean);
 }
 
-// What the gradients of a row need, in fp32 by one warp.
+// What the gradients of a row need, by one warp in fp32: a listed gradient is a difference of two probabilities, each
+// right to a few 2^-24, and the row waits for this chain (in fp64 it takes some 5 us, see distill_table_kernel).
 __device__ __forceinline__ RowFin finish_grads(const DistArgs& a, int row, const TableSums& u, MaxSum rest, float c) {
   const float mk = u.mk, s_list = u.sf, mass = u.massf, lp_rest = u.lp_rest, log_by = u.log_by;
   const int64_t base = (int64_t)row * a.K;

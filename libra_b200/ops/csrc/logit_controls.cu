@@ -326,12 +326,15 @@ void control_logits(torch::Tensor logits, c10::optional<torch::Tensor> history,
   a.err = err.data_ptr<int>();
   const c10::cuda::CUDAGuard guard(logits.device());
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  // tiles of 32768 tokens, since every tile scans the history once (256 x 151936 fp32 with 16384 tokens of history: 81 us,
-  // 84 us with tiles of 16384, both before the history was read four tokens a load: 75 us, 0.65 of the floor), smaller ones while that leaves SMs without three CTAs
+  // Tiles of 32768 tokens, since every tile scans the history once (256 x 151936 fp32 with 16384 tokens of history:
+  // 75 us, 0.65 of the floor; with the history read one token a load 81 us, and 84 us with tiles of 16384), smaller
+  // ones while that leaves SMs without three CTAs.
   int tile = 32768;
   while (tile > 2048 && (int64_t)B * ((V + tile - 1) / tile) < 3 * 148) tile /= 2;
   const int tiles = std::max(1, (V / 8 + tile / 8 - 1) / (tile / 8));
-  const bool wide = a.has_hist && a.hist_w >= (1 << 15);  // 16-bit counters hold 2^15 - 1 occurrences
+  // 16-bit counters hold 2^15 - 1 occurrences (256 rows bf16, histories up to 4096 in a 65520-wide table: 96 us with
+  // 32-bit ones, one CTA an SM; 65.5 us with 16-bit ones for the same rows as a 4096-wide table)
+  const bool wide = a.has_hist && a.hist_w >= (1 << 15);
   const size_t smem = (size_t)(tile + 32) * (wide ? 4 : 2) + (tile + 32) / 8;
   auto go = [&](auto* in, auto* o) {
     using I = std::remove_const_t<std::remove_pointer_t<decltype(in)>>;

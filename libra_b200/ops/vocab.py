@@ -66,7 +66,8 @@ def control_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     unless given; it may be ``logits`` itself), and are not differentiated
     through.  Row numbers, lengths and
     offsets that point outside their tables are not followed: they set the
-    error word that ``check_kernel_errors`` raises.
+    error word that ``check_kernel_errors`` raises (ValueError on the CPU).  A
+    row whose penalties change nothing need not have a valid history row.
     """
     logits = _rows(logits, "control_logits")
     if history is None and (history_lens is not None or history_rows is not None or prompt_lens is not None):
