@@ -19,6 +19,7 @@ import torch
 _MOST_LOWER = 3.4e38
 _MOST_RAISE = 1e20
 _REPETITION_RANGE = (1e-20, 1e20)
+_TEMPERATURE_RANGE = (1e-8, 1e8)
 
 
 @dataclass
@@ -39,6 +40,11 @@ class SamplingParams:
     top_logprobs: int = 0               # most likely tokens to report beside each sampled one
 
     def __post_init__(self):
+        if math.isnan(self.temperature) or math.isnan(self.top_p):
+            raise ValueError(f"temperature and top_p must be numbers, got {self.temperature} and {self.top_p}")
+        if self.temperature > 0:  # the limits themselves, one-hot and uniform, would be inf or NaN in fp32
+            self.temperature = min(max(self.temperature, _TEMPERATURE_RANGE[0]), _TEMPERATURE_RANGE[1])
+        self.top_p = max(self.top_p, 0.0)
         self.top_k = max(-1, min(int(self.top_k), 2 ** 31 - 1))  # (no vocabulary is larger: no filter)
         lo, hi = _REPETITION_RANGE
         if not lo <= self.repetition_penalty <= hi:

@@ -92,3 +92,23 @@ def test_server_answers_400_for_controls_beyond_fp32():
     finally:
         srv.stop()
         llm.shutdown()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_extreme_temperatures_beside_a_masked_request(device):
+    """A temperature that fp32 holds as 0, as a subnormal or not at all leaves no NaN, masked tokens included."""
+    for bad in (dict(temperature=math.nan), dict(top_p=math.nan)):
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            SamplingParams(**bad)
+    llm = _llm(device)
+    kws = [dict(temperature=t, **kw) for t in (1e-320, 1e-45, 1e-40, 1e-30, 1e30, 1e300, math.inf)
+           for kw in ({}, dict(allowed_token_ids=[3, 4, 5], top_logprobs=2))]
+    kws += [dict(top_p=-1.0), dict(top_p=0.0), dict(top_p=0.0, allowed_token_ids=[3, 4, 5])]
+    for kw in kws:
+        p = SamplingParams(max_tokens=3, **kw)
+        a, b = llm.generate_sync([[1, 2], [3, 4]], [p, SamplingParams(max_tokens=3, temperature=0.0)])
+        assert len(a.output_tokens) == len(b.output_tokens) == 3, kw
+        assert all(v == v and -math.inf < v < 1e-3 for v in a.output_logprobs), (kw, a.output_logprobs)
+        assert all(v == v for row in a.output_top_logprobs for _, v in row), kw
+        if "allowed_token_ids" in kw:
+            assert set(a.output_tokens) <= {3, 4, 5}
