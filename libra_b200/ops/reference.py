@@ -113,7 +113,8 @@ def control_logits(logits, history=None, history_lens=None, prompt_lens=None, hi
     B, V = z.shape
     for b in range(B):
         row = z[b]
-        if history is not None:
+        idle = all(t is None or float(t[b]) == v for t, v in ((repetition, 1.0), (presence, 0.0), (frequency, 0.0)))
+        if history is not None and not idle:
             hr = b if history_rows is None else int(history_rows[b])
             n = int(history_lens[b])
             if not 0 <= hr < history.shape[0] or not 0 <= n <= history.shape[1]:

@@ -64,10 +64,10 @@ def control_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
 
     They apply in this order, in fp32, with one rounding to ``out`` (fp32
     unless given; it may be ``logits`` itself), and are not differentiated
-    through.  Row numbers, lengths and
-    offsets that point outside their tables are not followed: they set the
-    error word that ``check_kernel_errors`` raises (ValueError on the CPU).  A
-    row whose penalties change nothing need not have a valid history row.
+    through.  Row numbers, lengths and offsets that point outside their tables
+    are not followed: they set the error word that ``check_kernel_errors``
+    raises (ValueError on the CPU).  A row whose penalties change nothing
+    (1, 0 and 0) needs no history: its row number and length are not looked at.
     """
     logits = _rows(logits, "control_logits")
     if history is None and (history_lens is not None or history_rows is not None or prompt_lens is not None):

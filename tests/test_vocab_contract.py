@@ -87,3 +87,20 @@ def test_beta_belongs_to_js_alone(device, beta):
     for f in (ops.distill_loss, ops.distill_loss_grad):
         with pytest.raises(ValueError, match="beta"):
             f(z, ids, lps, divergence="js", beta=beta)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_without_a_penalty_need_no_history(device):
+    z = torch.randn(2, 100, generator=torch.Generator().manual_seed(1)).to(device)
+    hist = torch.tensor([[5, 5, 6]], dtype=torch.int32, device=device)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=device)  # noqa: E731
+    f32 = lambda *v: torch.tensor(v, device=device)  # noqa: E731
+    ops.check_kernel_errors()
+    out = ops.control_logits(z, history=hist, history_rows=i32(0, 99), history_lens=i32(3, -5), repetition=f32(1.0, 1.0),
+                             presence=f32(0.5, 0.0), frequency=f32(0.25, 0.0))
+    ops.check_kernel_errors()
+    want = z.clone()
+    want[0, 5] -= 1.0
+    want[0, 6] -= 0.75
+    # two roundings of values near 2
+    assert float((out - want).abs().max()) <= 4 * 2.0 ** -24 * float(z.abs().max() + 1.0)
