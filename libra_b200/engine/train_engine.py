@@ -649,7 +649,8 @@ class B200TrainEngine:
 
     def prepare_update(self, trajectories: List[Dict[str, Any]]) -> List[Dict[str, Any]]:
         """Host-side packed execution chunks (with loss weights) for one update."""
-        if self.distill_coef > 0.0 and not self._warned_no_teacher and not any("teacher_ids" in t for t in trajectories):
+        if (self.distill_coef > 0.0 and trajectories and not self._warned_no_teacher
+                and not any("teacher_ids" in t for t in trajectories)):
             self._warned_no_teacher = True
             log.warning("distill_coef is %g, but none of these trajectories has a teacher's tables (teacher_ids, "
                         "teacher_logprobs; see score_teacher): the update has no distillation term", self.distill_coef)

@@ -40,3 +40,10 @@ def test_no_warning_with_tables_or_without_the_weight(caplog):
         plain.score_teacher(trajs[:1], 4)
         assert eng.grpo_update(trajs)["distill_loss"] > 0
         assert not _warnings(caplog)
+
+
+def test_no_warning_for_a_rank_without_trajectories(caplog):
+    eng = _engine("cpu", seed=7, distill_coef=0.5)
+    with caplog.at_level(logging.WARNING):
+        assert eng.prepare_update([]) == []
+    assert not _warnings(caplog)
