@@ -720,6 +720,8 @@ def grad_sq_norm(grad, out):
     return out
 
 
+from .rows import (ExpertPlan, embedding, expert_plan, moe_combine, moe_dispatch,  # noqa: E402
+                   route_topk)
 from .vocab import (control_logits, distill_loss, distill_loss_grad, lm_head_distill,  # noqa: E402
                     lm_head_top_logprobs, top_logprobs)
 
@@ -727,5 +729,6 @@ __all__ = [
     "ext", "extension_available", "check_kernel_errors", "gemm", "linear", "rmsnorm", "qk_norm_rope", "swiglu",
     "varlen_causal_attention", "lm_head_logprob", "adamw_step", "grad_sq_norm", "ref", "linear_swiglu",
     "paged_decode", "sample_tokens", "grouped_linear", "grouped_swiglu", "control_logits", "top_logprobs",
-    "distill_loss", "distill_loss_grad", "lm_head_distill", "lm_head_top_logprobs",
+    "distill_loss", "distill_loss_grad", "lm_head_distill", "lm_head_top_logprobs", "embedding", "route_topk",
+    "ExpertPlan", "expert_plan", "moe_dispatch", "moe_combine",
 ]

@@ -1,0 +1,589 @@
+// Rows of a mixture-of-experts layer: the router's choice, the plan that sorts (token, slot) pairs by expert, and the
+// moves of rows there (dispatch) and back (combine), with their gradients.
+//
+// Pair j = t * k + i is token t's i-th expert.  The experts' layout gives every expert a group of rows that starts on a
+// multiple of `align`; a group's rows behind its pairs, and the rows behind the last group, are padding.
+#include "row_moves.cuh"
+#include "sorted_keys.cuh"
+
+namespace libra {
+namespace experts {
+
+using namespace rows;
+using vocab::launch_rows;
+using vocab::order_key;
+using vocab::key_value;
+
+// ------------------------------------------------------------------ router
+//
+// A warp takes a row.  The k largest logits are found one after another: every lane knows the order key of its largest
+// value left, the warp's maximum is one redux, and the lowest index that has it another.  -inf ranks lowest, NaN
+// highest; equal logits are taken from the lowest index.  A row of nothing but -inf has weights 0.  Slot j belongs to
+// lane j % 32.
+
+constexpr int kRouteMax = 1024;  // experts
+constexpr int kRouteWarps = 8;
+
+template <typename T, int V, bool kWide>  // kWide: more than 32 slots
+__global__ void __launch_bounds__(kRouteWarps * 32)
+    route_fwd_kernel(const T* __restrict__ z, int64_t ld, int N, int E, int k, bool normalize, float* __restrict__ w,
+                     int64_t* __restrict__ ids, float2* __restrict__ stats) {
+  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+  if (row >= N) return;
+  const T* p = z + row * ld;
+  float v[V];
+  uint32_t key[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = 32 * i + lane;
+    v[i] = e < E ? to_f(p[e]) : -INFINITY;
+    key[i] = e < E ? order_key(v[i]) : 0u;  // no float has key 0
+  }
+  float top = 0.f, picked = 0.f, sum = 0.f;
+  int at = 0;
+  for (int j = 0; j < k; ++j) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) best = max(best, key[i]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    uint32_t first = 0xffffffffu;
+#pragma unroll
+    for (int i = V - 1; i >= 0; --i)
+      if (key[i] == best) first = 32 * i + lane;
+    first = __reduce_min_sync(0xffffffffu, first);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (first == 32u * i + lane) key[i] = 0;
+    const float val = key_value(best);
+    if (j == 0) top = val;
+    const float ex = top == -INFINITY ? 0.f : expf(val - top);
+    if (lane == (j & 31)) {
+      if (kWide) {
+        w[(int64_t)row * k + j] = ex;
+        ids[(int64_t)row * k + j] = first;
+      } else {
+        picked = ex;
+        at = (int)first;
+      }
+    }
+    sum += ex;
+  }
+  if (!normalize) {
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (32 * i + lane < E && top != -INFINITY) sum += expf(v[i] - top);
+    sum = warp_sum(sum);
+  }
+  const int64_t o = (int64_t)row * k;
+  if (kWide) {
+    for (int j = lane; j < k; j += 32) w[o + j] = sum == 0.f ? 0.f : w[o + j] / sum;
+  } else if (lane < k) {
+    w[o + lane] = sum == 0.f ? 0.f : picked / sum;
+    ids[o + lane] = at;
+  }
+  if (stats && lane == 0) stats[row] = make_float2(top, sum);
+}
+
+// Gradient of the weights with respect to the logits.  Renormalised weights are a softmax of the chosen logits alone:
+// dz_i = w_i (g_i - sum_j w_j g_j), nothing elsewhere.  Otherwise w_i = p_i, and dz_e = p_e ([e chosen] g_e - sum_j w_j
+// g_j) with p from the logits and the row's statistics.
+template <typename T, int V>
+__global__ void __launch_bounds__(kRouteWarps * 32)
+    route_bwd_kernel(const T* __restrict__ z, int64_t ld, int N, int E, int k, const float* __restrict__ w,
+                     const int64_t* __restrict__ ids, const float2* __restrict__ stats, const float* __restrict__ g,
+                     T* __restrict__ dz) {
+  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+  if (row >= N) return;
+  const int64_t o = (int64_t)row * k;
+  float inner = 0.f;
+  for (int j = lane; j < k; j += 32) inner = fmaf(w[o + j], g[o + j], inner);
+  inner = warp_sum(inner);
+  float d[V];
+  const float2 s = stats ? stats[row] : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = 32 * i + lane;
+    d[i] = s.y != 0.f && e < E ? -expf(to_f(z[row * ld + e]) - s.x) / s.y * inner : 0.f;
+  }
+  for (int j0 = 0; j0 < k; j0 += 32) {
+    float mine = 0.f;
+    int at = -1;
+    if (j0 + lane < k) {
+      const int64_t j = o + j0 + lane;
+      mine = w[j] * (stats ? g[j] : g[j] - inner);
+      at = (int)ids[j];
+    }
+    for (int j = 0; j < min(32, k - j0); ++j) {
+      const float val = __shfl_sync(0xffffffffu, mine, j);
+      const int e = __shfl_sync(0xffffffffu, at, j);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (e == 32 * i + lane) d[i] += val;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (32 * i + lane < E) from_f(dz + (int64_t)row * E + 32 * i + lane, d[i]);
+}
+
+template <typename F>
+static void by_width(int E, F&& go) {
+  if (E <= 32) go(std::integral_constant<int, 1>());
+  else if (E <= 64) go(std::integral_constant<int, 2>());
+  else if (E <= 128) go(std::integral_constant<int, 4>());
+  else if (E <= 256) go(std::integral_constant<int, 8>());
+  else if (E <= 512) go(std::integral_constant<int, 16>());
+  else go(std::integral_constant<int, 32>());
+}
+
+// -> {weights fp32 [N, k], experts int64 [N, k], stats fp32 [N, 2] or empty}
+static std::vector<torch::Tensor> route_fwd(const torch::Tensor& z, int64_t k, bool normalize, bool want_stats) {
+  LIBRA_CHECK(z.is_cuda() && z.dim() == 2 && row_type(z), "route_topk: logits must be a 2-D bf16 or fp32 CUDA tensor");
+  LIBRA_CHECK(z.size(1) <= 1 || z.stride(1) == 1, "route_topk: logits need a unit inner stride");
+  const int64_t N = z.size(0), E = z.size(1);
+  LIBRA_CHECK(E >= 1 && E <= kRouteMax && k >= 1 && k <= E, "route_topk: 1 to %d experts and k in [1, %lld]", kRouteMax,
+              (long long)E);
+  LIBRA_CHECK(N < (1ll << 31), "route_topk: too many rows");
+  const c10::cuda::CUDAGuard guard(z.device());
+  auto w = torch::empty({N, k}, z.options().dtype(at::kFloat));
+  auto ids = torch::empty({N, k}, z.options().dtype(at::kLong));
+  torch::Tensor stats;
+  if (want_stats) stats = torch::empty({N, 2}, z.options().dtype(at::kFloat));
+  if (N == 0) return {w, ids, stats};
+  cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  by_width((int)E, [&](auto v) {
+    auto go = [&](auto* p) {
+      using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+      constexpr int V = decltype(v)::value;
+      launch_rows(k > 32 ? route_fwd_kernel<T, V, true> : route_fwd_kernel<T, V, false>, (N + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32, 0, 1,
+                  false, st, p, z.stride(0), (int)N, (int)E, (int)k, normalize, w.data_ptr<float>(),
+                  ids.data_ptr<int64_t>(), want_stats ? (float2*)stats.data_ptr<float>() : (float2*)nullptr);
+    };
+    if (z.scalar_type() == at::kFloat)
+      go((const float*)z.data_ptr());
+    else
+      go((const __nv_bfloat16*)z.data_ptr());
+  });
+  return {w, ids, stats};
+}
+
+static torch::Tensor route_bwd(const torch::Tensor& z, const torch::Tensor& w, const torch::Tensor& ids,
+                               const torch::Tensor& stats, const torch::Tensor& g) {
+  const int64_t N = z.size(0), E = z.size(1), k = w.size(1);
+  const c10::cuda::CUDAGuard guard(z.device());
+  auto dz = torch::empty({N, E}, z.options());
+  if (N == 0) return dz;
+  cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  by_width((int)E, [&](auto v) {
+    auto go = [&](auto* p) {
+      using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+      launch_rows(route_bwd_kernel<T, decltype(v)::value>, (N + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32, 0, 1,
+                  false, st, p, z.stride(0), (int)N, (int)E, (int)k, (const float*)w.data_ptr<float>(),
+                  (const int64_t*)ids.data_ptr<int64_t>(),
+                  stats.defined() ? (const float2*)stats.data_ptr<float>() : (const float2*)nullptr,
+                  (const float*)g.data_ptr<float>(), (T*)dz.data_ptr());
+    };
+    if (z.scalar_type() == at::kFloat)
+      go((const float*)z.data_ptr());
+    else
+      go((const __nv_bfloat16*)z.data_ptr());
+  });
+  return dz;
+}
+
+struct RouteTopk : public torch::autograd::Function<RouteTopk> {
+  using List = torch::autograd::variable_list;
+  static List forward(torch::autograd::AutogradContext* ctx, torch::Tensor z, int64_t k, bool normalize) {
+    auto r = route_fwd(z, k, normalize, !normalize);
+    ctx->save_for_backward({z, r[0], r[1], r[2]});
+    ctx->mark_non_differentiable({r[1]});
+    ctx->set_materialize_grads(false);
+    return {r[0], r[1]};
+  }
+  static List backward(torch::autograd::AutogradContext* ctx, List up) {
+    LIBRA_CHECK(!at::GradMode::is_enabled(), "route_topk: its gradient is not differentiable");
+    List out(3);
+    if (!up[0].defined()) return out;
+    const auto s = ctx->get_saved_variables();
+    out[0] = route_bwd(s[0], s[1], s[2], s[3], up[0].contiguous());
+    return out;
+  }
+};
+
+// -> {weights fp32 [N, k], experts int64 [N, k]}, differentiable
+std::vector<torch::Tensor> route_topk(torch::Tensor z, int64_t k, bool normalize) {
+  if (at::GradMode::is_enabled() && z.requires_grad()) return RouteTopk::apply(z, k, normalize);
+  auto r = route_fwd(z, k, normalize, false);
+  r.pop_back();
+  return r;
+}
+
+// ------------------------------------------------------------------ plan
+
+template <typename I>
+struct PlanItems {
+  using Item = int;
+  const I* ids;
+  int* rows;
+  int *offs, *counts;
+  int E;
+  uint32_t align;
+  int* err;
+  __device__ __forceinline__ Item load(int i) const {
+    const I e = ids[i];
+    if (e >= (I)E) {
+      atomicCAS(err, 0, kBadArgument);
+      return -1;
+    }
+    return e < 0 ? -1 : (int)e;
+  }
+  __device__ __forceinline__ int bin(Item e) const { return e; }
+  __device__ __forceinline__ void put(int i, Item, uint32_t place) { rows[i] = (int)place; }
+  __device__ __forceinline__ void group(int e, uint32_t start, uint32_t count) {
+    offs[e] = (int)start;
+    counts[e] = (int)count;
+    if (e == E - 1) offs[E] = (int)(start + (count + align - 1) / align * align);
+  }
+};
+
+template <typename I>
+__global__ void __launch_bounds__(sorted::kThreads) plan_kernel(int n, int ctas, PlanItems<I> items) {
+  extern __shared__ uint32_t sm[];
+  sorted::counting_pass(n, items.E, items.align, sm, ctas, items);
+}
+
+// -> {rows int32 [n], offs int32 [E + 1], counts int32 [E]}
+std::vector<torch::Tensor> expert_plan(torch::Tensor ids, int64_t E, int64_t align, torch::Tensor err) {
+  LIBRA_CHECK(ids.is_cuda() && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) && ids.is_contiguous(),
+              "expert_plan: experts must be a contiguous int64 or int32 CUDA tensor");
+  LIBRA_CHECK(E >= 1 && E <= sorted::kMaxBins, "expert_plan: 1 to %d experts", sorted::kMaxBins);
+  const int64_t n = ids.numel();
+  LIBRA_CHECK(align >= 1 && n + (align - 1) * std::min(E, n) < (1ll << 31), "expert_plan: too many rows");
+  LIBRA_CHECK(err.device() == ids.device() && err.scalar_type() == at::kInt, "expert_plan: error word");
+  const c10::cuda::CUDAGuard guard(ids.device());
+  const auto i32 = ids.options().dtype(at::kInt);
+  auto rows_t = torch::empty({n}, i32), offs = torch::empty({E + 1}, i32), counts = torch::empty({E}, i32);
+  const int ctas = sorted::sort_ctas(n);
+  cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  auto go = [&](auto* p) {
+    using I = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+    PlanItems<I> it{p, rows_t.data_ptr<int>(), offs.data_ptr<int>(), counts.data_ptr<int>(), (int)E, (uint32_t)align,
+                    err.data_ptr<int>()};
+    launch_rows(plan_kernel<I>, ctas, sorted::kThreads, sorted::pass_smem((int)E), ctas, false, st, (int)n, ctas, it);
+  };
+  if (ids.scalar_type() == at::kLong)
+    go((const int64_t*)ids.data_ptr<int64_t>());
+  else
+    go((const int*)ids.data_ptr<int>());
+  return {rows_t, offs, counts};
+}
+
+// ------------------------------------------------------------------ moves
+
+struct Plan {
+  const int *rows, *offs, *counts;
+  int E, k, cap;
+};
+
+// Zeros into the layout's padding rows: part `part` of `parts` of it.
+template <typename T, int V>
+__device__ void zero_padding(const Plan& pl, T* out, int H, int part, int parts) {
+  Bits<T, V> z;
+  z.zero();
+  auto clear = [&](int64_t lo, int64_t hi, int64_t first, int64_t step) {
+    for (int64_t i = lo * (H / V) + first; i < hi * (H / V); i += step) z.store(out + i * V);
+  };
+  auto row = [&](int r) { return r < 0 ? 0 : (r < pl.cap ? r : pl.cap); };
+  for (int e = part; e < pl.E; e += parts)
+    clear(row(pl.offs[e] + pl.counts[e]), row(pl.offs[e + 1]), threadIdx.x, blockDim.x);
+  clear(row(pl.offs[pl.E]), pl.cap, (int64_t)part * blockDim.x + threadIdx.x, (int64_t)parts * blockDim.x);
+}
+
+// CTA t < N copies row t of x to its pairs' rows; the CTAs behind clear the padding.
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+    dispatch_kernel(const T* __restrict__ x, int64_t ld, int N, int H, Plan pl, T* __restrict__ out) {
+  const int t = blockIdx.x;
+  if (t >= N) {
+    zero_padding<T, V>(pl, out, H, t - N, gridDim.x - N);
+    return;
+  }
+  const int* r = pl.rows + (int64_t)t * pl.k;
+  for (int c = threadIdx.x * V; c < H; c += blockDim.x * V) {
+    Bits<T, V> b;
+    b.load(x + t * ld + c);
+    for (int i = 0; i < pl.k; ++i) {
+      const int to = r[i];
+      if ((unsigned)to < (unsigned)pl.cap) b.store(out + (int64_t)to * H + c);
+    }
+  }
+}
+
+// CTA t sums its pairs' rows: out[t] = residual[t] + sum_i w[t, i] y[rows[t, i]], in fp32 with one rounding.
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+    combine_kernel(const T* __restrict__ y, int64_t ldy, const float* __restrict__ w, const T* __restrict__ res,
+                   int64_t ldr, int H, Plan pl, T* __restrict__ out) {
+  constexpr int kBatch = 8;
+  const int64_t t = blockIdx.x;
+  for (int c = threadIdx.x * V; c < H; c += blockDim.x * V) {
+    float acc[V] = {};
+    for (int i0 = 0; i0 < pl.k; i0 += kBatch) {
+      Bits<T, V> b[kBatch];
+      float wi[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int i = i0 + u;
+        const int at = i < pl.k ? pl.rows[t * pl.k + i] : -1;
+        const bool here = (unsigned)at < (unsigned)pl.cap;
+        b[u].zero();
+        wi[u] = 0.f;
+        if (here) {
+          b[u].load(y + at * ldy + c);
+          wi[u] = w ? w[t * pl.k + i] : 1.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        if (i0 + u >= pl.k) break;
+        float v[V];
+        b[u].get(v);
+#pragma unroll
+        for (int q = 0; q < V; ++q) acc[q] = fmaf(wi[u], v[q], acc[q]);
+      }
+    }
+    if (res) {
+      Bits<T, V> b;
+      b.load(res + t * ldr + c);
+      float v[V];
+      b.get(v);
+#pragma unroll
+      for (int q = 0; q < V; ++q) acc[q] += v[q];
+    }
+    Bits<T, V> o;
+    o.set(acc);
+    o.store(out + t * H + c);
+  }
+}
+
+// A warp takes pair j: dy[rows[j]] = w[j] g[j / k], dw[j] = <g[j / k], y[rows[j]]>; the CTAs behind clear dy's padding.
+constexpr int kPairWarps = 8;
+template <typename T, int V>
+__global__ void __launch_bounds__(kPairWarps * 32)
+    combine_bwd_kernel(const T* __restrict__ g, int64_t ldg, const T* __restrict__ y, int64_t ldy,
+                       const float* __restrict__ w, int pairs, int pair_ctas, int H, Plan pl, T* __restrict__ dy,
+                       float* __restrict__ dw) {
+  if ((int)blockIdx.x >= pair_ctas) {
+    if (dy) zero_padding<T, V>(pl, dy, H, blockIdx.x - pair_ctas, gridDim.x - pair_ctas);
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+  const int64_t j = (int64_t)blockIdx.x * kPairWarps + (threadIdx.x >> 5);
+  if (j >= pairs) return;
+  const int at = pl.rows[j];
+  if ((unsigned)at >= (unsigned)pl.cap) {
+    if (dw && lane == 0) dw[j] = 0.f;
+    return;
+  }
+  const T* gr = g + j / pl.k * ldg;
+  const T* yr = y + at * ldy;
+  const float wj = w[j];
+  float dot = 0.f;
+#pragma unroll 4
+  for (int c = lane * V; c < H; c += 32 * V) {
+    Bits<T, V> b;
+    b.load(gr + c);
+    float v[V];
+    b.get(v);
+    if (dw) {
+      Bits<T, V> a;
+      a.load_once(yr + c);
+      float u[V];
+      a.get(u);
+#pragma unroll
+      for (int q = 0; q < V; ++q) dot = fmaf(v[q], u[q], dot);
+    }
+    if (dy) {
+#pragma unroll
+      for (int q = 0; q < V; ++q) v[q] *= wj;
+      b.set(v);
+      b.store(dy + (int64_t)at * H + c);
+    }
+  }
+  dot = warp_sum(dot);
+  if (dw && lane == 0) dw[j] = dot;
+}
+
+static int clear_ctas(const Plan& pl) { return std::max(1, std::min(pl.E, 148)); }
+
+static Plan plan_of(const torch::Tensor& rows_t, const torch::Tensor& offs, const torch::Tensor& counts, int64_t k,
+                    int64_t cap, int64_t N, const torch::Tensor& like, const char* op) {
+  const int64_t E = counts.numel();
+  auto ints = [&](const torch::Tensor& t) {
+    return t.device() == like.device() && t.scalar_type() == at::kInt && t.is_contiguous();
+  };
+  LIBRA_CHECK(ints(rows_t) && ints(offs) && ints(counts) && offs.numel() == E + 1, "%s: not a plan on the rows' device",
+              op);
+  LIBRA_CHECK(k >= 1 && rows_t.numel() == N * k, "%s: %lld rows for a plan of %lld pairs, %lld a token", op,
+              (long long)N, (long long)rows_t.numel(), (long long)k);
+  LIBRA_CHECK(cap >= 0 && cap < (1ll << 31), "%s: capacity", op);
+  return {rows_t.data_ptr<int>(), offs.data_ptr<int>(), counts.data_ptr<int>(), (int)E, (int)k, (int)cap};
+}
+
+static void check_move(const torch::Tensor& x, const char* op, const char* what) {
+  LIBRA_CHECK(x.is_cuda() && x.dim() == 2 && row_type(x), "%s: %s must be a 2-D bf16 or fp32 CUDA tensor", op, what);
+  LIBRA_CHECK(x.size(0) < (1ll << 31) && x.size(1) < (1ll << 30), "%s: %s is too large", op, what);
+}
+
+static int move_threads(int64_t H, int V) { return (int)std::min<int64_t>(256, ((H + V - 1) / V + 31) / 32 * 32); }
+
+// T, and vectors or single elements
+template <typename F>
+static void by_type(const torch::Tensor& t, bool vec, F&& go) {
+  if (t.scalar_type() == at::kFloat) {
+    if (vec) go((float*)nullptr, std::integral_constant<int, 4>());
+    else go((float*)nullptr, std::integral_constant<int, 1>());
+  } else {
+    if (vec) go((__nv_bfloat16*)nullptr, std::integral_constant<int, 8>());
+    else go((__nv_bfloat16*)nullptr, std::integral_constant<int, 1>());
+  }
+}
+
+static torch::Tensor spread(torch::Tensor x, const torch::Tensor& rows_t, const torch::Tensor& offs,
+                            const torch::Tensor& counts, int64_t k, int64_t cap) {
+  check_move(x, "moe_dispatch", "x");
+  const int64_t N = x.size(0), H = x.size(1);
+  const Plan pl = plan_of(rows_t, offs, counts, k, cap, N, x, "moe_dispatch");
+  const c10::cuda::CUDAGuard guard(x.device());
+  x = unit_inner(x);
+  auto out = torch::empty({cap, H}, x.options());
+  if (cap == 0 || H == 0) return out;
+  cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  by_type(x, row_vectors(x) && row_vectors(out), [&](auto* p, auto v) {
+    using T = std::remove_pointer_t<decltype(p)>;
+    constexpr int V = decltype(v)::value;
+    launch_rows(dispatch_kernel<T, V>, N + clear_ctas(pl), move_threads(H, V), 0, 1, false, st,
+                (const T*)x.data_ptr(), x.stride(0), (int)N, (int)H, pl, (T*)out.data_ptr());
+  });
+  return out;
+}
+
+static torch::Tensor sum_back(torch::Tensor y, const c10::optional<torch::Tensor>& w,
+                              const c10::optional<torch::Tensor>& res, const torch::Tensor& rows_t,
+                              const torch::Tensor& offs, const torch::Tensor& counts, int64_t k, int64_t N) {
+  check_move(y, "moe_combine", "y");
+  const int64_t cap = y.size(0), H = y.size(1);
+  const Plan pl = plan_of(rows_t, offs, counts, k, cap, N, y, "moe_combine");
+  if (w.has_value())
+    LIBRA_CHECK(vocab::vec_of(*w, y, at::kFloat, N * k), "moe_combine: weights must be contiguous fp32 [T, k]");
+  const c10::cuda::CUDAGuard guard(y.device());
+  y = unit_inner(y);
+  torch::Tensor r;
+  if (res.has_value()) {
+    LIBRA_CHECK(res->device() == y.device() && res->scalar_type() == y.scalar_type() && res->dim() == 2 &&
+                    res->size(0) == N && res->size(1) == H,
+                "moe_combine: the residual must be [T, H] of y's type");
+    r = unit_inner(*res);
+  }
+  auto out = torch::empty({N, H}, y.options());
+  if (N == 0 || H == 0) return out;
+  cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  by_type(y, row_vectors(y) && row_vectors(out) && (!r.defined() || row_vectors(r)), [&](auto* p, auto v) {
+    using T = std::remove_pointer_t<decltype(p)>;
+    constexpr int V = decltype(v)::value;
+    launch_rows(combine_kernel<T, V>, N, move_threads(H, V), 0, 1, false, st, (const T*)y.data_ptr(), y.stride(0),
+                w.has_value() ? (const float*)w->data_ptr<float>() : (const float*)nullptr,
+                r.defined() ? (const T*)r.data_ptr() : (const T*)nullptr, r.defined() ? r.stride(0) : 0, (int)H, pl,
+                (T*)out.data_ptr());
+  });
+  return out;
+}
+
+// -> {dy or nothing, dw or nothing}
+static std::vector<torch::Tensor> combine_bwd(torch::Tensor g, torch::Tensor y, const torch::Tensor& w,
+                                              const torch::Tensor& rows_t, const torch::Tensor& offs,
+                                              const torch::Tensor& counts, int64_t k, bool want_y, bool want_w) {
+  const int64_t N = g.size(0), cap = y.size(0), H = y.size(1), pairs = N * k;
+  const Plan pl = plan_of(rows_t, offs, counts, k, cap, N, y, "moe_combine");
+  const c10::cuda::CUDAGuard guard(y.device());
+  g = unit_inner(g);
+  y = unit_inner(y);
+  torch::Tensor dy, dw;
+  if (want_y) dy = torch::empty({cap, H}, y.options());
+  if (want_w) dw = H == 0 ? torch::zeros_like(w) : torch::empty_like(w);
+  if (H == 0 || (cap == 0 && pairs == 0)) return {dy, dw};
+  cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  const int64_t ctas = (pairs + kPairWarps - 1) / kPairWarps;
+  by_type(y, row_vectors(y) && row_vectors(g) && (!want_y || row_vectors(dy)), [&](auto* p, auto v) {
+    using T = std::remove_pointer_t<decltype(p)>;
+    constexpr int V = decltype(v)::value;
+    launch_rows(combine_bwd_kernel<T, V>, ctas + (want_y ? clear_ctas(pl) : 0), kPairWarps * 32, 0, 1, false, st,
+                (const T*)g.data_ptr(), g.stride(0), (const T*)y.data_ptr(), y.stride(0),
+                (const float*)w.data_ptr<float>(), (int)pairs, (int)ctas, (int)H, pl,
+                want_y ? (T*)dy.data_ptr() : (T*)nullptr, want_w ? dw.data_ptr<float>() : (float*)nullptr);
+  });
+  return {dy, dw};
+}
+
+struct Dispatch : public torch::autograd::Function<Dispatch> {
+  using List = torch::autograd::variable_list;
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor x, torch::Tensor rows_t,
+                               torch::Tensor offs, torch::Tensor counts, int64_t k, int64_t cap) {
+    ctx->save_for_backward({rows_t, offs, counts});
+    ctx->saved_data["k"] = k;
+    ctx->saved_data["N"] = x.size(0);
+    return spread(x, rows_t, offs, counts, k, cap);
+  }
+  static List backward(torch::autograd::AutogradContext* ctx, List up) {
+    LIBRA_CHECK(!at::GradMode::is_enabled(), "moe_dispatch: its gradient is not differentiable");
+    const auto s = ctx->get_saved_variables();
+    List out(6);
+    out[0] = sum_back(up[0], c10::nullopt, c10::nullopt, s[0], s[1], s[2], ctx->saved_data["k"].toInt(),
+                      ctx->saved_data["N"].toInt());
+    return out;
+  }
+};
+
+torch::Tensor moe_dispatch(torch::Tensor x, torch::Tensor rows_t, torch::Tensor offs, torch::Tensor counts, int64_t k,
+                           int64_t cap) {
+  if (at::GradMode::is_enabled() && x.requires_grad()) return Dispatch::apply(x, rows_t, offs, counts, k, cap);
+  return spread(x, rows_t, offs, counts, k, cap);
+}
+
+struct Combine : public torch::autograd::Function<Combine> {
+  using List = torch::autograd::variable_list;
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor y, torch::Tensor w,
+                               c10::optional<torch::Tensor> res, torch::Tensor rows_t, torch::Tensor offs,
+                               torch::Tensor counts, int64_t k, int64_t N) {
+    ctx->save_for_backward({y, w, rows_t, offs, counts});
+    ctx->saved_data["k"] = k;
+    return sum_back(y, w, res, rows_t, offs, counts, k, N);
+  }
+  static List backward(torch::autograd::AutogradContext* ctx, List up) {
+    LIBRA_CHECK(!at::GradMode::is_enabled(), "moe_combine: its gradient is not differentiable");
+    const auto s = ctx->get_saved_variables();
+    List out(8);
+    const bool want_y = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+    if (want_y || want_w) {
+      auto r = combine_bwd(up[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["k"].toInt(), want_y, want_w);
+      out[0] = r[0];
+      out[1] = r[1];
+    }
+    if (ctx->needs_input_grad(2)) out[2] = up[0];
+    return out;
+  }
+};
+
+torch::Tensor moe_combine(torch::Tensor y, torch::Tensor w, c10::optional<torch::Tensor> res, torch::Tensor rows_t,
+                          torch::Tensor offs, torch::Tensor counts, int64_t k, int64_t N) {
+  if (at::GradMode::is_enabled() &&
+      (y.requires_grad() || w.requires_grad() || (res.has_value() && res->requires_grad())))
+    return Combine::apply(y, w, res, rows_t, offs, counts, k, N);
+  return sum_back(y, w, res, rows_t, offs, counts, k, N);
+}
+
+}  // namespace experts
+}  // namespace libra

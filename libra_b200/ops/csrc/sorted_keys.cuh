@@ -1,0 +1,145 @@
+// Stable counting sort of small integer keys, one pass at a time, by one cluster of CTAs.
+//
+// The items are dealt to the cluster's warps in consecutive runs.  A pass counts each warp's keys, sums the counts
+// (warps before this one in the CTA, CTAs before this one in the cluster, bins before this one), and walks the same
+// items again: an item's place is its bin's start, plus the items of its key in earlier runs, plus those before it in
+// its own.  Places depend on the keys alone, never on the order in which warps run, so whatever sums follow the sorted
+// order are the same every time.  One cluster and its barrier take the place of three launches (count, scan, place).
+#pragma once
+#include "vocab_rows.cuh"
+
+namespace libra {
+namespace sorted {
+
+constexpr int kThreads = 1024, kWarps = 32, kMaxBins = 1024;
+
+inline size_t pass_smem(int bins) { return ((size_t)kWarps * bins + bins + 64) * 4; }
+
+__device__ __forceinline__ uint32_t ld_cluster_u32(const uint32_t* p, uint32_t rank) {
+  return (uint32_t)vocab::ld_cluster(reinterpret_cast<const int*>(p), rank);
+}
+
+// Exclusive sum over the block's 1024 threads.
+__device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t* tmp) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t s = v;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint32_t o = __shfl_up_sync(0xffffffffu, s, off);
+    if (lane >= off) s += o;
+  }
+  if (lane == 31) tmp[warp] = s;
+  __syncthreads();
+  if (warp == 0) {
+    uint32_t t = tmp[lane];
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, t, off);
+      if (lane >= off) t += o;
+    }
+    tmp[lane] = t;
+  }
+  __syncthreads();
+  return s - v + (warp ? tmp[warp - 1] : 0);
+}
+
+// One pass.  Items has
+//   Item load(int i)            item i; called twice for each
+//   int bin(const Item&)        its bin, or -1 for an item that gets no place
+//   void put(int i, Item, uint32_t place)   (place 0xffffffff for none)
+//   void group(int bin, uint32_t start, uint32_t count)   once for each bin; starts are multiples of `align`
+// Every CTA of the cluster calls it with all its threads; sm: pass_smem(bins) bytes.  What put writes to global memory
+// is visible to the whole cluster afterwards.
+template <class Items>
+__device__ __forceinline__ void counting_pass(int n, int bins, uint32_t align, uint32_t* sm, int ctas, Items& items) {
+  constexpr int kBatch = 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = threadIdx.x;
+  const int rank = ctas > 1 ? (int)cluster_ctarank() : 0;
+  uint32_t* total = sm + kWarps * bins;
+  uint32_t* tmp = total + bins;
+  uint32_t* mine = sm + warp * bins;
+  const int64_t per = (((int64_t)n + ctas * kWarps - 1) / (ctas * kWarps) + 31) / 32 * 32;
+  const int64_t lo = (rank * kWarps + warp) * per;
+  const int64_t hi = lo + per < n ? lo + per : n;
+
+  for (int i = lane; i < bins; i += 32) mine[i] = 0;
+  __syncwarp();
+  for (int64_t i0 = lo; i0 < hi; i0 += 32 * kBatch) {
+    int key[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int64_t i = i0 + 32 * u + lane;
+      key[u] = i < hi ? items.bin(items.load((int)i)) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (key[u] >= 0) atomicAdd(mine + key[u], 1u);
+  }
+  __syncthreads();
+
+  uint32_t sum = 0;
+  if (b < bins) {
+#pragma unroll 8
+    for (int w = 0; w < kWarps; ++w) sum += sm[w * bins + b];
+    total[b] = sum;
+  }
+  uint32_t all = sum, below = 0;
+  if (ctas > 1) {
+    vocab::cluster_meet();
+    if (b < bins) {
+      all = 0;
+      for (int c = 0; c < ctas; ++c) {
+        const uint32_t v = ld_cluster_u32(total + b, c);
+        all += v;
+        if (c < rank) below += v;
+      }
+    }
+  } else {
+    __syncthreads();
+  }
+  const uint32_t start = block_before(b < bins ? (all + align - 1) / align * align : 0, tmp);
+  if (b < bins) {
+    if (rank == 0) items.group(b, start, all);
+    uint32_t at = start + below;
+#pragma unroll 8
+    for (int w = 0; w < kWarps; ++w) {
+      const uint32_t c = sm[w * bins + b];
+      sm[w * bins + b] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+
+  for (int64_t i0 = lo; i0 < hi; i0 += 32 * kBatch) {
+    typename Items::Item it[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int64_t i = i0 + 32 * u + lane;
+      if (i < hi) it[u] = items.load((int)i);
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int64_t i = i0 + 32 * u + lane;
+      const int key = i < hi ? items.bin(it[u]) : -1;
+      const uint32_t peers = __match_any_sync(0xffffffffu, key);
+      const int before = __popc(peers & ((1u << lane) - 1));
+      uint32_t at = 0xffffffffu;
+      if (key >= 0) at = mine[key] + before;
+      __syncwarp();
+      if (key >= 0 && before == 0) mine[key] += __popc(peers);
+      __syncwarp();
+      if (i < hi) items.put((int)i, it[u], at);
+    }
+  }
+  // the totals outlive their readers, and the next pass reads what this one wrote
+  if (ctas > 1)
+    vocab::cluster_meet();
+  else
+    __syncthreads();
+}
+
+// CTAs of the cluster for n items.
+inline int sort_ctas(int64_t n) { return n <= 2048 ? 1 : 8; }
+
+}  // namespace sorted
+}  // namespace libra

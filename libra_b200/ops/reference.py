@@ -215,3 +215,77 @@ def distill_loss(logits, ids, lps, divergence: str, beta: float, tail: str, temp
         raise ValueError("distill_loss: target outside the vocabulary")
     logp = logq.gather(1, t.unsqueeze(1)).squeeze(1)
     return loss, torch.where(dead, torch.full_like(logp, float("-inf")), logp).float()
+
+
+def embedding(tokens, w, scale, first, whole):
+    """Rows ``tokens - first`` of ``w`` times ``scale``, zeros for tokens outside the table."""
+    r = tokens.reshape(-1).long() - first
+    here = (r >= 0) & (r < w.shape[0])
+    if whole and not bool(here.all()):
+        raise ValueError("embedding: a token lies outside the table")
+    out = w.index_select(0, r.clamp(0, max(w.shape[0] - 1, 0))) if w.shape[0] else w.new_zeros(r.numel(), w.shape[1])
+    if scale != 1.0:
+        out = (out.float() * scale).to(w.dtype)
+    if not whole:
+        out = out.masked_fill(~here.unsqueeze(1), 0)
+    return out.view(*tokens.shape, w.shape[1])
+
+
+def embedding_grad(tokens, g, rows, scale, first, main):
+    """Adds scale * sum of g over each token's positions to ``main``, or returns it as [rows, H] of g's type."""
+    r = tokens.reshape(-1).long() - first
+    here = (r >= 0) & (r < rows)
+    g = g.float()
+    if not bool(here.all()):
+        g, r = g[here], r[here]
+    if scale != 1.0:
+        g = g * scale
+    if main is not None:
+        main.view(rows, -1).index_add_(0, r, g)
+        return None
+    return torch.zeros(rows, g.shape[1]).index_add_(0, r, g)
+
+
+def route_topk(logits, k, normalize):
+    """Softmax weights and indices of the k largest logits of each row, ties at the lowest index."""
+    z = logits.float()
+    empty = (z == float("-inf")).all(-1, keepdim=True)
+    p = z.masked_fill(empty, 0.0).softmax(dim=-1).masked_fill(empty, 0.0)
+    ids = torch.sort(z.detach(), dim=-1, descending=True, stable=True).indices[:, :k]
+    w = p.gather(1, ids)
+    if normalize:
+        w = w / w.sum(-1, keepdim=True).masked_fill(empty, 1.0)
+    return w, ids
+
+
+def expert_plan(experts, num_experts, align):
+    """(rows int32 [T*k], offs int32 [E+1], counts int32 [E]) of (token, slot) pairs sorted by expert."""
+    flat = experts.reshape(-1).long()
+    if bool((flat >= num_experts).any()):
+        raise ValueError("expert_plan: an expert id is not below num_experts")
+    here = flat >= 0
+    key = torch.where(here, flat, torch.full_like(flat, num_experts))
+    counts = torch.bincount(key, minlength=num_experts + 1)
+    padded = (counts + align - 1) // align * align
+    start = padded.cumsum(0) - padded
+    first = counts.cumsum(0) - counts
+    order = torch.argsort(key, stable=True)
+    rank = torch.empty_like(key)
+    rank[order] = torch.arange(key.numel()) - first[key[order]]
+    rows = torch.where(here, start[key] + rank, torch.full_like(key, -1))
+    return rows.int(), start.int(), counts[:num_experts].int()
+
+
+def moe_dispatch(x, rows, k, capacity):
+    to = torch.where(rows >= 0, rows, capacity).long()
+    out = x.new_zeros(capacity + 1, x.shape[1], dtype=torch.float32)
+    return out.index_copy(0, to, x.float().repeat_interleave(k, dim=0))[:capacity].to(x.dtype)
+
+
+def moe_combine(y, weights, rows, k, residual):
+    here = (rows >= 0).unsqueeze(1)
+    picked = y.index_select(0, rows.clamp(min=0).long()).float().masked_fill(~here, 0.0)
+    out = (picked.view(rows.numel() // k, k, y.shape[1]) * weights.unsqueeze(-1)).sum(1)
+    if residual is not None:
+        out = out + residual.float()
+    return out.to(y.dtype)
