@@ -238,7 +238,7 @@ class InferenceRunner:
 
             x = vocab_parallel_embedding(tok_t, self.p["embed_tokens"], self.tp_group, dist.get_rank(self.tp_group))
         else:
-            x = self.p["embed_tokens"].index_select(0, tok_t)
+            x = ops.embedding(tok_t, self.p["embed_tokens"])
         peer = self.peer_ar if self.peer_ar is not None and x.shape[0] <= self.peer_ar.max_rows else None
         L = cfg.num_hidden_layers
         if peer is not None:

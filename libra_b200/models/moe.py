@@ -69,14 +69,16 @@ class GroupedLinear(torch.autograd.Function):
         return dx, (None if main is not None else dw.to(w.dtype)), None, None
 
 
+def router_logits(h, router_w):
+    """h W_r^T in fp32."""
+    return torch.nn.functional.linear(h.float(), router_w.float())
+
+
 def route(h, router_w, top_k: int, normalize: bool = True):
     """Returns (weights [T, k] fp32, experts [T, k] int64, router probs [T, E])."""
-    logits = torch.nn.functional.linear(h.float(), router_w.float())
-    probs = logits.softmax(dim=-1)
-    weights, experts = probs.topk(top_k, dim=-1)
-    if normalize:
-        weights = weights / weights.sum(-1, keepdim=True)
-    return weights, experts, probs
+    logits = router_logits(h, router_w)
+    weights, experts = ops.route_topk(logits, top_k, normalize=normalize)
+    return weights, experts, logits.softmax(dim=-1)
 
 
 GROUP_ALIGN = 128  # rows: every expert's group starts on a tensor-core tile boundary
@@ -87,43 +89,21 @@ def expert_layout(experts: torch.Tensor, num_experts: int, align: int = GROUP_AL
 
     Returns ``offs`` (int32 [E+1]: group e owns rows [offs[e], offs[e+1]), each
     start a multiple of ``align``) and ``rows`` (int64 [T*k]: the row of
-    assignment j = t*k + kk).  Nothing is read back to the host: the counts come
-    from a scatter-add, not a bincount whose size depends on the data."""
-    flat = experts.reshape(-1)
-    counts = torch.zeros(num_experts, dtype=torch.int64, device=flat.device)
-    counts.scatter_add_(0, flat, torch.ones_like(flat))
-    padded = (counts + align - 1) // align * align
-    offs = torch.zeros(num_experts + 1, dtype=torch.int64, device=flat.device)
-    offs[1:] = padded.cumsum(0)
-    order = torch.argsort(flat, stable=True)
-    g = flat[order]
-    first = counts.cumsum(0) - counts
-    rank = torch.arange(flat.numel(), device=flat.device) - first[g]
-    rows = torch.empty_like(flat)
-    rows[order] = offs[g] + rank
-    return offs.to(torch.int32), rows
-
-
-def grouped_capacity(tokens: int, k: int, num_groups: int, align: int = GROUP_ALIGN) -> int:
-    """Rows that always hold the padded layout of ``tokens * k`` assignments over ``num_groups`` groups."""
-    return tokens * k + (align - 1) * num_groups + align
+    assignment j = t*k + kk), as ``ops.expert_plan`` sorts them."""
+    plan = ops.expert_plan(experts.reshape(-1, 1), num_experts, align=align)
+    return plan.offs, plan.rows.long()
 
 
 def moe_mlp(h, residual, router_w, w1, w2, cfg):
     """residual + sum_k w_k * Expert_{e_k}(h), with every expert's rows in one
     padded buffer and both expert GEMMs as single grouped launches (no host
     synchronisation, no per-expert loop)."""
-    T, H = h.shape
-    E, k = cfg.num_experts, cfg.num_experts_per_tok
-    weights, experts, _ = route(h, router_w, k, cfg.norm_topk_prob)
-    offs, rows = expert_layout(experts, E)
-    cap = grouped_capacity(T, k, E)
-    xs = h.new_zeros(cap, H).index_copy(0, rows, h.repeat_interleave(k, dim=0))
-    a = ops.grouped_swiglu(xs, w1, offs)
-    ys = ops.grouped_linear(a, w2, offs)
-    picked = ys.index_select(0, rows).view(T, k, H)
-    out = (picked.float() * weights.unsqueeze(-1)).sum(1) + residual.float()
-    return out.to(h.dtype)
+    weights, experts = ops.route_topk(router_logits(h, router_w), cfg.num_experts_per_tok,
+                                      normalize=cfg.norm_topk_prob)
+    plan = ops.expert_plan(experts, cfg.num_experts, align=GROUP_ALIGN)
+    a = ops.grouped_swiglu(ops.moe_dispatch(h, plan), w1, plan.offs)
+    ys = ops.grouped_linear(a, w2, plan.offs)
+    return ops.moe_combine(ys, weights, plan, residual=residual)
 
 
 def moe_mlp_looped(h, residual, router_w, w1, w2, cfg):

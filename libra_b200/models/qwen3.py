@@ -415,7 +415,7 @@ class Qwen3Model(nn.Module):
     def embed(self, tokens):
         w = self.p["embed_tokens"]
         if self.tp_size == 1:
-            return _Embedding.apply(tokens, w)
+            return ops.embedding(tokens, w)
         from libra_b200.parallel.tensor_parallel import vocab_parallel_embedding
 
         return vocab_parallel_embedding(tokens, w, self.tp_group, self.tp_rank)
@@ -486,26 +486,6 @@ class Qwen3Model(nn.Module):
         """Full logits [T, V] (inference/sampling helper)."""
         h = self.hidden_states(batch)
         return ops.linear(h, self.lm_head_weight)
-
-
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, tokens, w):
-        ctx.save_for_backward(tokens)
-        ctx.wref = w
-        return w.index_select(0, tokens)
-
-    @staticmethod
-    def backward(ctx, g):
-        (tokens,) = ctx.saved_tensors
-        w = ctx.wref
-        main = getattr(w, "main_grad", None)
-        if main is not None:
-            main.index_add_(0, tokens, g.float())
-            return None, None
-        out = torch.zeros(w.shape, dtype=torch.float32, device=w.device)
-        out.index_add_(0, tokens, g.float())
-        return None, out.to(w.dtype)
 
 
 def config_from_arch(arch) -> Qwen3Config:

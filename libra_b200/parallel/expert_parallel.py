@@ -53,15 +53,12 @@ def ep_moe_mlp(h, residual, router, w1_local, w2_local, cfg, group, exchange: Op
         return _ep_moe_mlp_peer(h, residual, router, w1_local, w2_local, cfg, exchange)
     ep = dist.get_world_size(group) if dist.is_initialized() else 1
     E_l = w1_local.shape[0]
-    T, H = h.shape
-    k = cfg.num_experts_per_tok
-    from libra_b200.models.moe import route
+    from libra_b200.models.moe import router_logits
 
-    weights, experts, _ = route(h, router, k, cfg.norm_topk_prob)
-    flat_e = experts.reshape(-1)
-    order = torch.argsort(flat_e, stable=True)
-    dest = flat_e[order] // E_l
-    send_counts = torch.bincount(dest, minlength=ep)
+    weights, experts = ops.route_topk(router_logits(h, router), cfg.num_experts_per_tok,
+                                      normalize=cfg.norm_topk_prob)
+    plan = ops.expert_plan(experts, cfg.num_experts, align=1)  # pairs in expert order, hence in rank order
+    send_counts = plan.counts.long().view(ep, E_l).sum(1)
     counts = send_counts.clone()
     recv = torch.empty_like(counts)
     if ep > 1:
@@ -69,9 +66,9 @@ def ep_moe_mlp(h, residual, router, w1_local, w2_local, cfg, group, exchange: Op
     else:
         recv = counts
     sc, rc = send_counts.tolist(), recv.tolist()
-    tok = order // k
-    x_send = h.index_select(0, tok)
-    e_send = (flat_e[order] % E_l).to(torch.int32)
+    x_send = ops.moe_dispatch(h, plan)
+    e_send = torch.empty_like(plan.rows)
+    e_send[plan.rows.long()] = (experts.reshape(-1) % E_l).to(torch.int32)
     x_recv = _AllToAll.apply(x_send, sc, rc, group) if ep > 1 else x_send
     e_recv = _all_to_all(e_send, sc, rc, group) if ep > 1 else e_send
     # local experts on the received rows
@@ -85,10 +82,7 @@ def ep_moe_mlp(h, residual, router, w1_local, w2_local, cfg, group, exchange: Op
         a = ops.swiglu(gu)
         y_recv = y_recv.index_add(0, sel, ops.linear(a, w2_local[e]))
     y_send = _AllToAll.apply(y_recv, rc, sc, group) if ep > 1 else y_recv
-    wsel = weights.reshape(-1)[order].unsqueeze(1)
-    out = torch.zeros((T, H), dtype=torch.float32, device=h.device)
-    out = out.index_add(0, tok, y_send.float() * wsel)
-    return (out + residual.float()).to(h.dtype)
+    return ops.moe_combine(y_send, weights, plan, residual=residual)
 
 
 # ----------------------------------------------------------------------------- peer-memory dispatch / combine
@@ -285,9 +279,10 @@ class _PeerCombine(torch.autograd.Function):
 
 
 def _ep_moe_mlp_peer(h, residual, router, w1_local, w2_local, cfg, xchg: PeerExpertExchange):
-    from libra_b200.models.moe import route
+    from libra_b200.models.moe import router_logits
 
-    weights, experts, _ = route(h, router, cfg.num_experts_per_tok, cfg.norm_topk_prob)
+    weights, experts = ops.route_topk(router_logits(h, router), cfg.num_experts_per_tok,
+                                      normalize=cfg.norm_topk_prob)
     plan = xchg.plan(experts, cfg.num_experts)
     x_recv = _PeerDispatch.apply(h, plan, xchg)
     # both expert projections are single grouped launches over the padded per-expert groups; the second

@@ -20,6 +20,7 @@ import torch
 import torch.distributed as dist
 
 from libra_b200 import ops
+from libra_b200.ops.rows import embedding_grad, embedding_rows
 
 
 def _ws(group) -> int:
@@ -93,30 +94,18 @@ def row_parallel_linear_allreduce(a, w_local, residual, group):
 class _VocabParallelEmbedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, w_local, group, rank, reduce=True):
-        V_l = w_local.shape[0]
-        lo = rank * V_l
-        local = (tokens >= lo) & (tokens < lo + V_l)
-        idx = torch.where(local, tokens - lo, torch.zeros_like(tokens))
-        out = w_local.index_select(0, idx) * local.unsqueeze(-1).to(w_local.dtype)
-        out = out.contiguous()
+        tokens, lo = tokens.contiguous(), rank * w_local.shape[0]
+        out = embedding_rows(tokens, w_local, 1.0, lo, False)
         if reduce and _ws(group) > 1:
             dist.all_reduce(out, group=group)
-        ctx.save_for_backward(idx, local)
-        ctx.wref = w_local
+        ctx.save_for_backward(tokens)
+        ctx.w, ctx.lo = w_local, lo
         return out
 
     @staticmethod
     def backward(ctx, g):
-        idx, local = ctx.saved_tensors
-        w = ctx.wref
-        gl = g.float() * local.unsqueeze(-1).float()
-        main = getattr(w, "main_grad", None)
-        if main is not None:
-            main.index_add_(0, idx, gl)
-            return None, None, None, None, None
-        out = torch.zeros(w.shape, dtype=torch.float32, device=w.device)
-        out.index_add_(0, idx, gl)
-        return None, out.to(w.dtype), None, None, None
+        (tokens,) = ctx.saved_tensors
+        return None, embedding_grad(tokens, g, ctx.w, 1.0, ctx.lo), None, None, None
 
 
 def vocab_parallel_embedding(tokens, w_local, group, rank, reduce: bool = True):
