@@ -126,18 +126,20 @@ void distill_bwd(torch::Tensor logits, torch::Tensor out, double T, int64_t K, c
                  torch::Tensor saved, c10::optional<torch::Tensor> g, c10::optional<torch::Tensor> g_lp);
 }  // namespace vocab
 namespace embed {
-torch::Tensor embedding_fwd(torch::Tensor tokens, torch::Tensor w, double scale, int64_t first, bool whole,
-                            torch::Tensor err);
-torch::Tensor embedding_bwd(torch::Tensor tokens, torch::Tensor g, torch::Tensor w, double scale, int64_t first,
+torch::Tensor embedding(torch::Tensor tokens, torch::Tensor w, double scale, int64_t first, bool whole,
+                        torch::Tensor err);
+std::vector<torch::Tensor> embedding_fwd(torch::Tensor tokens, torch::Tensor w, double scale, int64_t first, bool whole,
+                                         bool want_order, torch::Tensor err);
+torch::Tensor embedding_bwd(torch::Tensor order, torch::Tensor g, torch::Tensor w, double scale,
                             c10::optional<torch::Tensor> main);
 }  // namespace embed
 namespace experts {
 std::vector<torch::Tensor> route_topk(torch::Tensor z, int64_t k, bool normalize);
 std::vector<torch::Tensor> expert_plan(torch::Tensor ids, int64_t E, int64_t align, torch::Tensor err);
 torch::Tensor moe_dispatch(torch::Tensor x, torch::Tensor rows_t, torch::Tensor offs, torch::Tensor counts, int64_t k,
-                           int64_t cap);
+                           int64_t align, int64_t cap);
 torch::Tensor moe_combine(torch::Tensor y, torch::Tensor w, c10::optional<torch::Tensor> res, torch::Tensor rows_t,
-                          torch::Tensor offs, torch::Tensor counts, int64_t k, int64_t N);
+                          torch::Tensor offs, torch::Tensor counts, int64_t k, int64_t align, int64_t N);
 }  // namespace experts
 }  // namespace libra
 
@@ -204,8 +206,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("distill_loss", &libra::vocab::distill_loss, "distill_fwd with autograd through distill_bwd");
   m.def("distill_onepass", &libra::vocab::distill_onepass, "distillation loss and unit gradient in one pass");
   m.def("distill_bwd", &libra::vocab::distill_bwd, "gradient of distill_fwd with respect to the logits");
-  m.def("embedding_fwd", &libra::embed::embedding_fwd, "embedding rows of a table or a shard of it, scaled");
-  m.def("embedding_bwd", &libra::embed::embedding_bwd, "gradient of embedding_fwd by sorted tokens");
+  m.def("embedding", &libra::embed::embedding, "embedding rows, differentiable with respect to the table");
+  m.def("embedding_fwd", &libra::embed::embedding_fwd, "embedding rows of a table or a shard of it, scaled, and the tokens' order");
+  m.def("embedding_bwd", &libra::embed::embedding_bwd, "gradient of embedding_fwd from the tokens' order");
   m.def("route_topk", &libra::experts::route_topk, "k largest logits of every row and their softmax weights");
   m.def("expert_plan", &libra::experts::expert_plan, "rows of (token, slot) pairs sorted by expert");
   m.def("moe_dispatch", &libra::experts::moe_dispatch, "rows copied to their experts' groups");

@@ -1,10 +1,15 @@
 // Embedding lookup with scaling, and its gradient by sorted tokens.
 //
 // dW[v] = scale * sum over the positions i with token v of g[i].  The (token, position) pairs are sorted by token
-// (stable, so a token's positions stay in order), cut into chunks of equally many pairs whatever the tokens are, and
-// every chunk sums its runs of equal tokens in fp32.  A run inside one chunk goes straight to its row; a run that
-// crosses a border leaves one partial sum a chunk, which a second kernel joins from left to right.  No atomics: the
-// same inputs give the same bits, and a token that fills half the batch is spread over as many CTAs as any other half.
+// (stable, so a token's positions stay in order) and cut into chunks of equally many pairs, whatever the tokens are.  A
+// CTA sums the runs of equal tokens that start in its chunk, in fp32, and writes each to its row once.  A run that goes
+// on through the whole next chunk is shared: every chunk leaves its part of it, and a second kernel joins the parts
+// from left to right.  Each row is written by one thread a column, so the same inputs give the same bits, and a token
+// that fills half the batch is spread over as many CTAs as any other half.
+//
+// A forward pass whose table wants a gradient sorts its tokens in the first CTAs of the lookup's own launch: the sort
+// is a chain of barriers on a few SMs that moves next to nothing, and the lookup has the others meanwhile (8192 tokens:
+// 16 us as a launch of its own).
 #include "row_moves.cuh"
 #include "sorted_keys.cuh"
 
@@ -14,53 +19,39 @@ namespace embed {
 using namespace rows;
 using vocab::launch_rows;
 
-// ------------------------------------------------------------------ lookup
-
-template <typename T, int V, typename I>
-__global__ void __launch_bounds__(256)
-    lookup_kernel(const I* __restrict__ tokens, const T* __restrict__ w, int64_t ld, int64_t rows_w, int64_t first,
-                  bool whole, float scale, int H, T* __restrict__ out, int* err) {
-  const int64_t i = blockIdx.x;
-  const int64_t r = (int64_t)tokens[i] - first;
-  const bool here = r >= 0 && r < rows_w;
-  if (!here && whole && threadIdx.x == 0) atomicCAS(err, 0, kBadArgument);
-  for (int c = threadIdx.x * V; c < H; c += blockDim.x * V) {
-    Bits<T, V> b;
-    b.zero();
-    if (here) {
-      b.load(w + r * ld + c);
-      if (scale != 1.f) {
-        float v[V];
-        b.get(v);
-#pragma unroll
-        for (int q = 0; q < V; ++q) v[q] *= scale;
-        b.set(v);
-      }
-    }
-    b.store(out + i * H + c);
+struct Tokens {
+  const void* p;
+  bool wide;  // int64
+  int64_t first;
+  int rows;   // of the table
+  // Row of the table, or `rows` for a token outside it.
+  __device__ __forceinline__ uint32_t row(int i) const {
+    const int64_t r = (wide ? static_cast<const int64_t*>(p)[i] : (int64_t)static_cast<const int*>(p)[i]) - first;
+    return r >= 0 && r < rows ? (uint32_t)r : (uint32_t)rows;
   }
-}
+};
 
 // ------------------------------------------------------------------ sort
 
-template <typename I>
-struct FirstPass {  // from the tokens themselves; what is not in the table sorts behind it
+struct Digit {
+  int shift;
+  uint32_t mask;
+  __device__ __forceinline__ int of(uint32_t key) const { return (int)((key >> shift) & mask); }
+};
+
+struct FirstPass {  // from the tokens themselves; notes which rows occur
   struct Item {
     uint32_t key;
   };
-  const I* tokens;
-  int64_t first, rows_w;
-  int shift;
-  uint32_t mask;
-  uint32_t *key_out, *pos_out;
-  __device__ __forceinline__ Item load(int i) const {
-    const int64_t r = (int64_t)tokens[i] - first;
-    return {r >= 0 && r < rows_w ? (uint32_t)r : (uint32_t)rows_w};
-  }
-  __device__ __forceinline__ int bin(const Item& a) const { return (int)(a.key & mask); }
+  Tokens tk;
+  Digit d;
+  uint32_t *key_out, *pos_out, *seen;
+  __device__ __forceinline__ Item load(int i) const { return {tk.row(i)}; }
+  __device__ __forceinline__ int bin(const Item& a) const { return d.of(a.key); }
   __device__ __forceinline__ void put(int i, const Item& a, uint32_t at) {
     key_out[at] = a.key;
     pos_out[at] = (uint32_t)i;
+    if (a.key < (uint32_t)tk.rows) atomicOr(seen + (a.key >> 5), 1u << (a.key & 31));
   }
   __device__ __forceinline__ void group(int, uint32_t, uint32_t) {}
 };
@@ -69,11 +60,10 @@ struct NextPass {
     uint32_t key, pos;
   };
   const uint32_t *key_in, *pos_in;
-  int shift;
-  uint32_t mask;
+  Digit d;
   uint32_t *key_out, *pos_out;
   __device__ __forceinline__ Item load(int i) const { return {__ldcg(key_in + i), __ldcg(pos_in + i)}; }
-  __device__ __forceinline__ int bin(const Item& a) const { return (int)((a.key >> shift) & mask); }
+  __device__ __forceinline__ int bin(const Item& a) const { return d.of(a.key); }
   __device__ __forceinline__ void put(int, const Item& a, uint32_t at) {
     key_out[at] = a.key;
     pos_out[at] = a.pos;
@@ -81,23 +71,90 @@ struct NextPass {
   __device__ __forceinline__ void group(int, uint32_t, uint32_t) {}
 };
 
-// Radix sort of the tokens by `passes` digits of `bits` bits; the sorted pairs end in buffer (passes - 1) % 2.
-template <typename I>
-__global__ void __launch_bounds__(sorted::kThreads)
-    sort_kernel(const I* __restrict__ tokens, int n, int64_t first, int64_t rows_w, int passes, int bits, int ctas,
-                uint32_t* buf) {
-  extern __shared__ uint32_t sm[];
-  const uint32_t mask = (1u << bits) - 1;
-  uint32_t* at[2] = {buf, buf + 2 * (int64_t)n};
-  FirstPass<I> p0{tokens, first, rows_w, 0, mask, at[0], at[0] + n};
-  sorted::counting_pass(n, 1 << bits, 1u, sm, ctas, p0);
-  for (int p = 1; p < passes; ++p) {
-    NextPass q{at[(p - 1) & 1], at[(p - 1) & 1] + n, p * bits, mask, at[p & 1], at[p & 1] + n};
-    sorted::counting_pass(n, 1 << bits, 1u, sm, ctas, q);
+// What a sort leaves: keys [n], positions [n], and a bit for every row of the table that occurs.
+struct Order {
+  uint32_t *key, *pos, *seen, *scratch;  // scratch: 2 n
+  int n, passes, bits, ctas;
+};
+constexpr int kDigit = 9;  // at most sorted::kWordBins bins a pass
+
+__device__ __forceinline__ void sort_tokens(const Tokens& tk, const Order& o, uint32_t* sm) {
+  const uint32_t mask = (1u << o.bits) - 1;
+  const int words = (tk.rows + 31) / 32;
+  // cleared before the first put: a pass's barriers lie between
+  for (int i = blockIdx.x * sorted::kThreads + threadIdx.x; i < words; i += o.ctas * sorted::kThreads) o.seen[i] = 0;
+  auto key = [&](int p) { return ((o.passes - 1 - p) & 1) ? o.scratch : o.key; };
+  auto pos = [&](int p) { return ((o.passes - 1 - p) & 1) ? o.scratch + o.n : o.pos; };
+  FirstPass p0{tk, {0, mask}, key(0), pos(0), o.seen};
+  sorted::counting_pass(o.n, 1 << o.bits, 1u, sm, o.ctas, p0);
+  for (int p = 1; p < o.passes; ++p) {
+    NextPass q{key(p - 1), pos(p - 1), {p * o.bits, mask}, key(p), pos(p)};
+    sorted::counting_pass(o.n, 1 << o.bits, 1u, sm, o.ctas, q);
   }
 }
 
+// ------------------------------------------------------------------ lookup
+
+// A warp takes a row, eight loads a lane at a time.
+template <class B>
+__device__ __forceinline__ void look_up(const Tokens& tk, int i, const typename B::T* w, int64_t ld, bool whole,
+                                        float scale, int H, typename B::T* out, int* err) {
+  constexpr int U = 8;
+  const int lane = threadIdx.x & 31, lanes = B::lanes(H);
+  const uint32_t r = tk.row(i);
+  const bool here = r < (uint32_t)tk.rows;
+  if (!here && whole && lane == 0) atomicCAS(err, 0, kBadArgument);
+  const typename B::T* src = w + (int64_t)r * ld;
+  typename B::T* dst = out + (int64_t)i * H;
+  for (int c = lane; c < lanes; c += 32 * U) {
+    B b[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (here && c + 32 * u < lanes) b[u].load(src, c + 32 * u, H);
+      else b[u].zero();
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (c + 32 * u >= lanes) break;
+      if (scale != 1.f) {
+        float v[B::V];
+        b[u].get(v);
+#pragma unroll
+        for (int q = 0; q < B::V; ++q) v[q] *= scale;
+        b[u].set(v);
+      }
+      b[u].store(dst, c + 32 * u, H);
+    }
+  }
+}
+
+constexpr int kLookWarps = 4;
+template <class B>
+__global__ void __launch_bounds__(kLookWarps * 32)
+    lookup_kernel(Tokens tk, int n, const typename B::T* __restrict__ w, int64_t ld, bool whole, float scale, int H,
+                  typename B::T* __restrict__ out, int* err) {
+  const int i = blockIdx.x * kLookWarps + (threadIdx.x >> 5);
+  if (i < n) look_up<B>(tk, i, w, ld, whole, scale, H, out, err);
+}
+
+// The first cluster sorts, the CTAs behind it look up.
+template <class B>
+__global__ void __launch_bounds__(sorted::kThreads)
+    lookup_sort_kernel(Tokens tk, Order o, const typename B::T* __restrict__ w, int64_t ld, bool whole, float scale,
+                       int H, typename B::T* __restrict__ out, int* err) {
+  extern __shared__ uint32_t sm[];
+  if ((int)blockIdx.x < o.ctas) {
+    sort_tokens(tk, o, sm);
+    return;
+  }
+  const int warps = (gridDim.x - o.ctas) * sorted::kWarps;
+  for (int i = (blockIdx.x - o.ctas) * sorted::kWarps + (threadIdx.x >> 5); i < o.n; i += warps)
+    look_up<B>(tk, i, w, ld, whole, scale, H, out, err);
+}
+
 // ------------------------------------------------------------------ sums of runs
+
+constexpr uint32_t kNoKey = 0xffffffffu;
 
 struct Target {  // where a row's gradient goes
   void* out;     // dense: the gradient, of the table's type
@@ -105,171 +162,229 @@ struct Target {  // where a row's gradient goes
   float scale;
 };
 
-template <typename T, int V>
-__device__ __forceinline__ void write_row(const Target& to, uint32_t row, int H, int c, const float (&acc)[V]) {
-  const int64_t o = (int64_t)row * H + c;
-  if (to.main) {
-    if constexpr (V == 1) {
-      to.main[o] = fmaf(to.scale, acc[0], to.main[o]);
-    } else {
+template <class B>
+__device__ __forceinline__ void write_row(const Target& to, uint32_t row, int i, int H, float (&acc)[B::V]) {
 #pragma unroll
-      for (int q = 0; q < V; q += 4) {
-        float4* p = reinterpret_cast<float4*>(to.main + o + q);
-        float4 m = *p;
-        m.x = fmaf(to.scale, acc[q], m.x);
-        m.y = fmaf(to.scale, acc[q + 1], m.y);
-        m.z = fmaf(to.scale, acc[q + 2], m.z);
-        m.w = fmaf(to.scale, acc[q + 3], m.w);
-        *p = m;
+  for (int q = 0; q < B::V; ++q) acc[q] *= to.scale;
+  if (to.main) {
+    float* m = to.main + (int64_t)row * H;
+    B::sum_f(m, i, H, acc);
+    B::put_f(m, i, H, acc);
+  } else {
+    B b;
+    b.set(acc);
+    b.store((typename B::T*)to.out + (int64_t)row * H, i, H);
+  }
+}
+
+// A chunk has L pairs, the last one fewer; chunk c of the grid's first `chunks * slices` CTAs, slice by slice of 128
+// lanes of the rows.  parts holds two fp32 rows a chunk: its part of a shared run that came in from the left, and of
+// one that starts here.  The CTAs behind clear the rows of a dense gradient that no token names.
+//
+// Loads run ahead of the sums by U pairs, those of main's rows too (kMain): a run is one or two pairs long as a rule,
+// and what a row's sum is added to would else be waited for at every run.  (Reductions at L2 in its place, 8192 x 2560:
+// 43 us, bound by their rate, against 34 us of waiting.)
+constexpr int kRunThreads = 128;
+template <class B, int L, bool kMain>
+__global__ void __launch_bounds__(kRunThreads)
+    run_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos, const uint32_t* __restrict__ seen,
+               int n, uint32_t R, const typename B::T* __restrict__ g, int64_t ldg, int H, int chunks, int slices,
+               Target to, float* __restrict__ parts) {
+  static_assert(L <= 32, "a warp looks at a chunk");
+  const int lane = threadIdx.x & 31, lanes = B::lanes(H);
+  if ((int)blockIdx.x >= chunks * slices) {
+    const int warp = (blockIdx.x - chunks * slices) * (kRunThreads / 32) + (threadIdx.x >> 5);
+    const int warps = (gridDim.x - chunks * slices) * (kRunThreads / 32);
+    B z;
+    z.zero();
+    for (uint32_t r = warp; r < R; r += warps) {
+      if (seen[r >> 5] >> (r & 31) & 1) continue;
+      for (int c = lane; c < lanes; c += 32) z.store((typename B::T*)to.out + (int64_t)r * H, c, H);
+    }
+    return;
+  }
+  __shared__ uint32_t sk[3 * L + 2], sp[2 * L];
+  const int chunk = blockIdx.x / slices, i = (blockIdx.x - chunk * slices) * kRunThreads + threadIdx.x;
+  const int lo = chunk * L, hi = min(n, lo + L);
+  for (int t = threadIdx.x; t < 3 * L + 2; t += kRunThreads) {
+    const int at = lo - L - 1 + t;
+    sk[t] = at >= 0 && at < n ? key[at] : kNoKey;
+  }
+  for (int t = threadIdx.x; t < 2 * L; t += kRunThreads) sp[t] = lo + t < n ? pos[lo + t] : 0;
+  __syncthreads();
+  auto K = [&](int at) { return sk[at - (lo - L - 1)]; };
+
+  // pairs [beg, end) are this CTA's
+  int beg = lo, end = hi;
+  const uint32_t k0 = K(lo), k1 = K(hi - 1);
+  const bool from_left = K(lo - 1) == k0;
+  if (from_left && K(lo - L - 1) != k0) {  // it starts in the chunk before ...
+    const int same = __ffs(~__ballot_sync(0xffffffffu, lane < hi - lo && K(lo + lane) == k0)) - 1;
+    const int stop = lo + (same < 0 ? 32 : same);
+    if (stop < hi || K(hi) != k0) beg = stop;  // ... and ends in this one: that chunk sums it
+  }
+  const bool from_far = from_left && beg == lo;
+  if (K(hi) == k1) {
+    const int same = __ffs(~__ballot_sync(0xffffffffu, lane < L && K(hi + lane) == k1)) - 1;
+    const int stop = hi + (same < 0 ? 32 : same);
+    const bool here = !(from_far && k1 == k0) && beg < hi;  // the run starts in this chunk
+    if (here && K(stop) != k1) end = stop;                  // (stop <= hi + L) and ends in the next
+  }
+  if (i >= lanes) return;
+  float* part = parts + 2 * (int64_t)chunk * H;
+  // what becomes of the sum behind pair `at`: it goes on, is a part from the left or to the right, or a row
+  enum { kOn, kLeft, kRight, kRow };
+  auto then = [&](int at) {
+    const uint32_t k = K(at);
+    const bool more = K(at + 1) == k;
+    if (more && at + 1 < end) return kOn;
+    return from_far && k == k0 ? kLeft : more ? kRight : kRow;
+  };
+  float acc[B::V] = {};
+  constexpr int U = kMain ? 4 : 8;
+  for (int s = beg; s < end; s += U) {
+    B b[U];
+    float m[kMain ? U : 1][B::V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s + u >= end || K(s + u) >= R) break;
+      b[u].load_once(g + (int64_t)sp[s + u - lo] * ldg, i, H);
+      if constexpr (kMain) {
+        if (then(s + u) == kRow) B::get_f(to.main + (int64_t)K(s + u) * H, i, H, m[u]);
       }
     }
-  } else {
-    float v[V];
 #pragma unroll
-    for (int q = 0; q < V; ++q) v[q] = acc[q] * to.scale;
-    Bits<T, V> b;
-    b.set(v);
-    b.store((T*)to.out + o);
-  }
-}
-
-template <int V>
-__device__ __forceinline__ void write_part(float* p, const float (&acc)[V]) {
+    for (int u = 0; u < U; ++u) {
+      if (s + u >= end) break;
+      const uint32_t k = K(s + u);
+      if (k >= R) return;  // tokens outside the table, behind all others
+      float v[B::V];
+      b[u].get(v);
 #pragma unroll
-  for (int q = 0; q < V; ++q) p[q] = acc[q];
-}
-
-// CTA (chunk, column slice): sorted pairs [chunk * L, chunk * L + L).  parts holds two fp32 rows a chunk: the sum of a
-// run that came in from the chunk before, and that of one that starts here and goes on into the next.
-template <typename T, int V>
-__global__ void __launch_bounds__(256)
-    run_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos, int n, int L, uint32_t rows_w,
-               const T* __restrict__ g, int64_t ldg, int H, Target to, float* __restrict__ parts) {
-  const int lo = blockIdx.x * L, hi = min(n, lo + L);
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
-  if (c >= H) return;
-  const uint32_t before = lo > 0 ? key[lo - 1] : 0xffffffffu, after = hi < n ? key[hi] : 0xffffffffu;
-  float* part = parts + 2 * (int64_t)blockIdx.x * H + c;
-  float acc[V] = {};
-  uint32_t now = key[lo];
-  bool from_left = now == before;
-  for (int i = lo; i < hi; ++i) {
-    if (now >= rows_w) return;  // tokens outside the table, behind all others
-    Bits<T, V> b;
-    b.load_once(g + (int64_t)pos[i] * ldg + c);
-    float v[V];
-    b.get(v);
+      for (int q = 0; q < B::V; ++q) acc[q] += v[q];
+      const int what = then(s + u);
+      if (what == kOn) continue;
+      if (what == kRow) {
+        if constexpr (kMain) {
 #pragma unroll
-    for (int q = 0; q < V; ++q) acc[q] += v[q];
-    const uint32_t next = i + 1 < hi ? key[i + 1] : after;
-    if (next != now || i + 1 == hi) {
-      if (from_left)
-        write_part<V>(part, acc);
-      else if (next == now)
-        write_part<V>(part + H, acc);
-      else
-        write_row<T, V>(to, now, H, c, acc);
+          for (int q = 0; q < B::V; ++q) acc[q] = fmaf(acc[q], to.scale, m[u][q]);
+          B::put_f(to.main + (int64_t)k * H, i, H, acc);
+        } else {
+          write_row<B>(to, k, i, H, acc);
+        }
+      } else {
+        B::put_f(what == kLeft ? part : part + H, i, H, acc);
+      }
 #pragma unroll
-      for (int q = 0; q < V; ++q) acc[q] = 0.f;
-      now = next;
-      from_left = false;
+      for (int q = 0; q < B::V; ++q) acc[q] = 0.f;
     }
   }
 }
 
-// CTA (chunk, column slice): joins the run that starts in this chunk and goes on into the next ones, if there is one.
-template <typename T, int V>
-__global__ void __launch_bounds__(256)
-    join_kernel(const uint32_t* __restrict__ key, int n, int L, uint32_t rows_w, int H, Target to,
+// Joins the shared runs.  A CTA looks at 32 chunks (a lane each) for runs that start there and go on through the whole
+// next chunk, and sums their parts for 128 lanes of the row.
+template <class B, int L>
+__global__ void __launch_bounds__(kRunThreads)
+    join_kernel(const uint32_t* __restrict__ key, int n, uint32_t R, int H, int slices, Target to,
                 const float* __restrict__ parts) {
-  const int64_t hi = (int64_t)(blockIdx.x + 1) * L;
-  if (hi >= n) return;
-  const uint32_t k = key[hi - 1];
-  if (k >= rows_w || key[hi] != k) return;
-  const int lo = blockIdx.x * L;
-  if (lo > 0 && key[lo - 1] == k) return;  // it came in from the left: that chunk joins it
-  int a = (int)hi, b = n;                  // the run's end: the first pair behind hi with another token
-  while (a < b) {
-    const int mid = a + (b - a) / 2;
-    if (key[mid] > k) b = mid; else a = mid + 1;
+  pdl_wait();
+  const int block = blockIdx.x / slices, i = (blockIdx.x - block * slices) * kRunThreads + threadIdx.x;
+  const int lane = threadIdx.x & 31;
+  const int64_t lo = (int64_t)(block * 32 + lane) * L, hi = lo + L;
+  uint32_t k = kNoKey;
+  bool starts = false;
+  if (hi + L < n) {
+    k = key[hi - 1];
+    starts = k < R && key[hi + L] == k && (lo == 0 || key[lo - 1] != k);
   }
-  const int last = (a - 1) / L;
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
-  if (c >= H) return;
-  float acc[V];
-  const float* p = parts + (2 * (int64_t)blockIdx.x + 1) * H + c;
-#pragma unroll
-  for (int q = 0; q < V; ++q) acc[q] = p[q];
-#pragma unroll 4
-  for (int j = blockIdx.x + 1; j <= last; ++j) {
-    p = parts + 2 * (int64_t)j * H + c;
-#pragma unroll
-    for (int q = 0; q < V; ++q) acc[q] += p[q];
+  uint32_t todo = __ballot_sync(0xffffffffu, starts);
+  if (i >= B::lanes(H)) return;
+  while (todo) {
+    const int at = __ffs(todo) - 1, chunk = block * 32 + at;
+    todo &= todo - 1;
+    const uint32_t kr = key[(int64_t)(chunk + 1) * L - 1];
+    int a = (chunk + 2) * L, b = n;  // the first pair behind the run
+    while (a < b) {
+      const int mid = a + (b - a) / 2;
+      if (key[mid] > kr) b = mid; else a = mid + 1;
+    }
+    const int last = (a - 1) / L;
+    float acc[B::V] = {};
+    B::sum_f(parts + (2 * (int64_t)chunk + 1) * H, i, H, acc);
+#pragma unroll 8
+    for (int j = chunk + 1; j <= last; ++j) B::sum_f(parts + 2 * (int64_t)j * H, i, H, acc);
+    write_row<B>(to, kr, i, H, acc);
   }
-  write_row<T, V>(to, k, H, c, acc);
 }
 
-static void check_tokens(const torch::Tensor& tokens, const torch::Tensor& w, const char* op) {
+static void check_tokens(const torch::Tensor& tokens, const torch::Tensor& w) {
   LIBRA_CHECK(w.is_cuda() && w.dim() == 2 && row_type(w) && (w.size(1) <= 1 || w.stride(1) == 1),
-              "%s: the table must be a 2-D bf16 or fp32 CUDA tensor with a unit inner stride", op);
+              "embedding: the table must be a 2-D bf16 or fp32 CUDA tensor with a unit inner stride");
   LIBRA_CHECK(tokens.device() == w.device() && tokens.is_contiguous() &&
                   (tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt),
-              "%s: tokens must be int64 or int32 on the table's device", op);
+              "embedding: tokens must be contiguous int64 or int32 on the table's device");
   LIBRA_CHECK(tokens.numel() < (1ll << 30) && w.size(0) < (1ll << 30) && w.size(1) < (1ll << 30),
-              "%s: too many tokens, or too large a table", op);
+              "embedding: too many tokens, or too large a table");
 }
 
-template <typename F>
-static void by_token(const torch::Tensor& t, F&& go) {
-  if (t.scalar_type() == at::kLong)
-    go((const int64_t*)t.data_ptr<int64_t>());
-  else
-    go((const int*)t.data_ptr<int>());
-}
-template <typename F>
-static void by_row(const torch::Tensor& t, bool vec, F&& go) {
-  if (t.scalar_type() == at::kFloat) {
-    if (vec) go((float*)nullptr, std::integral_constant<int, 4>());
-    else go((float*)nullptr, std::integral_constant<int, 1>());
-  } else {
-    if (vec) go((__nv_bfloat16*)nullptr, std::integral_constant<int, 8>());
-    else go((__nv_bfloat16*)nullptr, std::integral_constant<int, 1>());
-  }
-}
-
-// out [n, H]; whole: a token outside the table is an error, else it is another shard's.
-torch::Tensor embedding_fwd(torch::Tensor tokens, torch::Tensor w, double scale, int64_t first, bool whole,
-                            torch::Tensor err) {
-  check_tokens(tokens, w, "embedding");
+// -> {rows [*tokens, H], order or nothing}; whole: a token outside the table is an error, else it is another shard's;
+// want_order: the tokens' order too, which embedding_bwd takes.
+std::vector<torch::Tensor> embedding_fwd(torch::Tensor tokens, torch::Tensor w, double scale, int64_t first, bool whole,
+                                         bool want_order, torch::Tensor err) {
+  check_tokens(tokens, w);
   LIBRA_CHECK(err.device() == w.device() && err.scalar_type() == at::kInt, "embedding: error word");
-  const int64_t n = tokens.numel(), H = w.size(1);
+  const int64_t n = tokens.numel(), H = w.size(1), R = w.size(0);
   const c10::cuda::CUDAGuard guard(w.device());
   auto sizes = tokens.sizes().vec();
   sizes.push_back(H);
   auto out = torch::empty(sizes, w.options());
-  if (n == 0 || H == 0) return out;
+  torch::Tensor order, scratch;
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  by_row(w, row_vectors(w), [&](auto* p, auto v) {
-    using T = std::remove_pointer_t<decltype(p)>;
-    constexpr int V = decltype(v)::value;
-    const int threads = (int)std::min<int64_t>(256, ((H + V - 1) / V + 31) / 32 * 32);
-    by_token(tokens, [&](auto* tk) {
-      using I = std::remove_const_t<std::remove_pointer_t<decltype(tk)>>;
-      launch_rows(lookup_kernel<T, V, I>, n, threads, 0, 1, false, st, tk, (const T*)w.data_ptr(), w.stride(0),
-                  w.size(0), first, whole, (float)scale, (int)H, (T*)out.data_ptr(), err.data_ptr<int>());
-    });
+  const Tokens tk{tokens.data_ptr(), tokens.scalar_type() == at::kLong, first, (int)R};
+  if (want_order) order = torch::empty({2 * n + (R + 31) / 32}, w.options().dtype(at::kInt));
+  if (n == 0 || H == 0) return {out, order};
+  by_lanes(w, row_vectors(w), [&](auto lanes) {
+    using B = decltype(lanes);
+    using T = typename B::T;
+    const T* table = (const T*)w.data_ptr();
+    T* to = (T*)out.data_ptr();
+    if (!want_order) {
+      launch_rows(lookup_kernel<B>, (n + kLookWarps - 1) / kLookWarps, kLookWarps * 32, 0, 1, false, st, tk, (int)n, table,
+                  w.stride(0), whole, (float)scale, (int)H, to, err.data_ptr<int>());
+      return;
+    }
+    int total = 1;
+    while ((R >> total) != 0) ++total;  // bits of the largest key, R itself
+    Order o;
+    o.n = (int)n;
+    o.passes = (total + kDigit - 1) / kDigit;
+    o.bits = (total + o.passes - 1) / o.passes;
+    o.ctas = n <= 1024 ? 1 : 8;
+    if (o.passes > 1) scratch = torch::empty({2 * n}, w.options().dtype(at::kInt));
+    o.key = (uint32_t*)order.data_ptr<int>();
+    o.pos = o.key + n;
+    o.seen = o.key + 2 * n;
+    o.scratch = o.passes > 1 ? (uint32_t*)scratch.data_ptr<int>() : nullptr;
+    const int64_t look = std::min<int64_t>((n + sorted::kWarps - 1) / sorted::kWarps, 148 - o.ctas);
+    launch_rows(lookup_sort_kernel<B>, o.ctas * (1 + (look + o.ctas - 1) / o.ctas), sorted::kThreads,
+                sorted::pass_smem(1 << o.bits), o.ctas, false, st, tk, o, table, w.stride(0), whole, (float)scale, (int)H,
+                to, err.data_ptr<int>());
   });
-  return out;
+  return {out, order};
 }
 
-// Gradient of the table w [rows, H] from g [n, H]: added to main (fp32, contiguous) or returned, of w's type.
-torch::Tensor embedding_bwd(torch::Tensor tokens, torch::Tensor g, torch::Tensor w, double scale, int64_t first,
+// Gradient of the table w [rows, H] from g [n, H] and the tokens' order: added to main (fp32, contiguous) or returned,
+// of w's type.
+torch::Tensor embedding_bwd(torch::Tensor order, torch::Tensor g, torch::Tensor w, double scale,
                             c10::optional<torch::Tensor> main) {
-  check_tokens(tokens, w, "embedding");
-  const int64_t n = tokens.numel(), H = w.size(1), R = w.size(0);
-  LIBRA_CHECK(g.device() == w.device() && g.dim() == 2 && g.size(0) == n && g.size(1) == H &&
-                  g.scalar_type() == w.scalar_type(),
-              "embedding: the gradient must be [tokens, H] of the table's type");
+  const int64_t H = w.size(1), R = w.size(0);
+  LIBRA_CHECK(g.device() == w.device() && g.dim() >= 1 && g.size(-1) == H && g.scalar_type() == w.scalar_type(),
+              "embedding: the gradient must be [*, H] of the table's type");
+  if (g.dim() != 2) g = g.reshape({H ? g.numel() / H : 0, H});
+  const int64_t n = g.size(0);
+  LIBRA_CHECK(order.device() == w.device() && order.scalar_type() == at::kInt && order.is_contiguous() &&
+                  (H == 0 || order.numel() == 2 * n + (R + 31) / 32),
+              "embedding: the order is not that of these tokens");
   if (main.has_value())
     LIBRA_CHECK(main->device() == w.device() && main->scalar_type() == at::kFloat && main->is_contiguous() &&
                     main->numel() == R * H,
@@ -277,41 +392,77 @@ torch::Tensor embedding_bwd(torch::Tensor tokens, torch::Tensor g, torch::Tensor
   const c10::cuda::CUDAGuard guard(w.device());
   g = unit_inner(g);
   torch::Tensor out;
-  if (!main.has_value()) out = torch::zeros({R, H}, w.options());
-  if (n == 0 || H == 0 || R == 0) return out;
-  cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  int total = 1;
-  while ((R >> total) != 0) ++total;  // bits of the largest key, R itself
-  const int passes = (total + 9) / 10, bits = (total + passes - 1) / passes;
-  const int ctas = sorted::sort_ctas(n);
-  const int L = n <= 16384 ? 16 : 64;
-  const int64_t chunks = (n + L - 1) / L;
-  auto buf = torch::empty({4 * n}, w.options().dtype(at::kInt));
-  auto parts = torch::empty({chunks, 2, H}, w.options().dtype(at::kFloat));
-  uint32_t* b = (uint32_t*)buf.data_ptr<int>();
-  by_token(tokens, [&](auto* tk) {
-    using I = std::remove_const_t<std::remove_pointer_t<decltype(tk)>>;
-    launch_rows(sort_kernel<I>, ctas, sorted::kThreads, sorted::pass_smem(1 << bits), ctas, false, st, tk, (int)n,
-                first, R, passes, bits, ctas, b);
-  });
-  const uint32_t *key = b + ((passes - 1) & 1) * 2 * n, *pos = key + n;
+  if (n == 0 || H == 0 || R == 0) {
+    if (!main.has_value()) out = torch::zeros({R, H}, w.options());
+    return out;
+  }
+  if (!main.has_value()) out = torch::empty({R, H}, w.options());
+  const uint32_t *key = (const uint32_t*)order.data_ptr<int>(), *pos = key + n, *seen = key + 2 * n;
   const Target to{main.has_value() ? nullptr : out.data_ptr(), main.has_value() ? main->data_ptr<float>() : nullptr,
                   (float)scale};
-  const bool vec = row_vectors(g) && H % 8 == 0 && (main.has_value() ? reinterpret_cast<uintptr_t>(to.main) % 16 == 0
-                                                                      : row_vectors(out));
-  by_row(g, vec, [&](auto* p, auto v) {
-    using T = std::remove_pointer_t<decltype(p)>;
-    constexpr int V = decltype(v)::value;
-    const int64_t lanes = (H + V - 1) / V;
-    const int threads = (int)std::min<int64_t>(128, (lanes + 31) / 32 * 32);
-    const dim3 grid((unsigned)chunks, (unsigned)((lanes + threads - 1) / threads));
-    run_kernel<T, V><<<grid, threads, 0, st>>>(key, pos, (int)n, L, (uint32_t)R, (const T*)g.data_ptr(), g.stride(0),
-                                               (int)H, to, parts.data_ptr<float>());
-    LIBRA_LAUNCH_CHECK();
-    join_kernel<T, V><<<grid, threads, 0, st>>>(key, (int)n, L, (uint32_t)R, (int)H, to, parts.data_ptr<float>());
-    LIBRA_LAUNCH_CHECK();
+  const bool wide = row_vectors(g) && (main.has_value() ? reinterpret_cast<uintptr_t>(to.main) % 16 == 0
+                                                         : row_vectors(out));
+  cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  by_lanes(w, wide, [&](auto lanes_type) {
+    using B = decltype(lanes_type);
+    using T = typename B::T;
+    auto go = [&](auto len) {
+      constexpr int L = decltype(len)::value;
+      const int64_t chunks = (n + L - 1) / L;
+      const int slices = (B::lanes((int)H) + kRunThreads - 1) / kRunThreads;
+      auto parts = torch::empty({chunks, 2, H}, w.options().dtype(at::kFloat));
+      const int64_t clear = main.has_value() ? 0 : std::min<int64_t>((R + 3) / 4, 148 * 8);
+      LIBRA_CHECK(chunks * slices + clear < (1ll << 31), "embedding: too many tokens");
+      launch_rows(main.has_value() ? run_kernel<B, L, true> : run_kernel<B, L, false>, chunks * slices + clear, kRunThreads, 0, 1, false, st, key, pos, seen, (int)n,
+                  (uint32_t)R, (const T*)g.data_ptr(), g.stride(0), (int)H, (int)chunks, slices, to,
+                  parts.data_ptr<float>());
+      launch_rows(join_kernel<B, L>, (chunks + 31) / 32 * slices, kRunThreads, 0, 1, true, st, key, (int)n, (uint32_t)R,
+                  (int)H, slices, to, (const float*)parts.data_ptr<float>());
+    };
+    if (n <= 16384)
+      go(std::integral_constant<int, 16>());
+    else
+      go(std::integral_constant<int, 32>());
   });
   return out;
+}
+
+// The fp32 buffer that a parameter's gradients accumulate into, where it has one.
+static c10::optional<torch::Tensor> main_grad_of(const torch::Tensor& w) {
+  py::gil_scoped_acquire gil;
+  const py::object p = py::cast(w);
+  const py::object m = py::getattr(p, "main_grad", py::none());
+  if (m.is_none()) return c10::nullopt;
+  return m.cast<torch::Tensor>();
+}
+
+// embedding_fwd and embedding_bwd as one differentiable function of the table.  In C++, since a Python function's trips
+// through the interpreter cost a small batch more than its kernels.
+struct Embedding : public torch::autograd::Function<Embedding> {
+  using List = torch::autograd::variable_list;
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor tokens, torch::Tensor w,
+                               double scale, int64_t first, bool whole, torch::Tensor err) {
+    auto r = embedding_fwd(tokens, w, scale, first, whole, true, err);
+    ctx->saved_data["w"] = w;  // its shape and main_grad; the values may change before the backward pass
+    ctx->saved_data["order"] = r[1];
+    ctx->saved_data["scale"] = scale;
+    return r[0];
+  }
+  static List backward(torch::autograd::AutogradContext* ctx, List up) {
+    LIBRA_CHECK(!at::GradMode::is_enabled(), "embedding: its gradient is not differentiable");
+    const auto w = ctx->saved_data["w"].toTensor();
+    auto main = main_grad_of(w);
+    List out(6);
+    out[1] = embedding_bwd(ctx->saved_data["order"].toTensor(), up[0], w, ctx->saved_data["scale"].toDouble(), main);
+    if (main.has_value() && !main->is_inference()) main->unsafeGetTensorImpl()->bump_version();
+    return out;
+  }
+};
+
+torch::Tensor embedding(torch::Tensor tokens, torch::Tensor w, double scale, int64_t first, bool whole,
+                        torch::Tensor err) {
+  if (at::GradMode::is_enabled() && w.requires_grad()) return Embedding::apply(tokens, w, scale, first, whole, err);
+  return embedding_fwd(tokens, w, scale, first, whole, false, err)[0];
 }
 
 }  // namespace embed

@@ -223,18 +223,18 @@ std::vector<torch::Tensor> route_topk(torch::Tensor z, int64_t k, bool normalize
 
 // ------------------------------------------------------------------ plan
 
-template <typename I>
 struct PlanItems {
   using Item = int;
-  const I* ids;
+  const void* ids;
+  bool wide;  // int64
   int* rows;
   int *offs, *counts;
   int E;
   uint32_t align;
   int* err;
   __device__ __forceinline__ Item load(int i) const {
-    const I e = ids[i];
-    if (e >= (I)E) {
+    const int64_t e = wide ? static_cast<const int64_t*>(ids)[i] : (int64_t)static_cast<const int*>(ids)[i];
+    if (e >= E) {
       atomicCAS(err, 0, kBadArgument);
       return -1;
     }
@@ -249,8 +249,15 @@ struct PlanItems {
   }
 };
 
-template <typename I>
-__global__ void __launch_bounds__(sorted::kThreads) plan_kernel(int n, int ctas, PlanItems<I> items) {
+// CTAs of the cluster: as many as leave a warp the eight items a lane that it keeps in registers (131072 pairs of 128
+// experts: 26 us with 8 CTAs that load them twice).
+static int plan_ctas(int64_t n) {
+  int ctas = 1;
+  while (ctas < sorted::kMaxCtas && ctas * 32 * 32 * sorted::kBatch < n) ctas *= 2;
+  return ctas;
+}
+
+__global__ void __launch_bounds__(sorted::kThreads) plan_kernel(int n, int ctas, PlanItems items) {
   extern __shared__ uint32_t sm[];
   sorted::counting_pass(n, items.E, items.align, sm, ctas, items);
 }
@@ -266,18 +273,11 @@ std::vector<torch::Tensor> expert_plan(torch::Tensor ids, int64_t E, int64_t ali
   const c10::cuda::CUDAGuard guard(ids.device());
   const auto i32 = ids.options().dtype(at::kInt);
   auto rows_t = torch::empty({n}, i32), offs = torch::empty({E + 1}, i32), counts = torch::empty({E}, i32);
-  const int ctas = sorted::sort_ctas(n);
-  cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  auto go = [&](auto* p) {
-    using I = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
-    PlanItems<I> it{p, rows_t.data_ptr<int>(), offs.data_ptr<int>(), counts.data_ptr<int>(), (int)E, (uint32_t)align,
-                    err.data_ptr<int>()};
-    launch_rows(plan_kernel<I>, ctas, sorted::kThreads, sorted::pass_smem((int)E), ctas, false, st, (int)n, ctas, it);
-  };
-  if (ids.scalar_type() == at::kLong)
-    go((const int64_t*)ids.data_ptr<int64_t>());
-  else
-    go((const int*)ids.data_ptr<int>());
+  const int ctas = plan_ctas(n);
+  PlanItems it{ids.data_ptr(), ids.scalar_type() == at::kLong, rows_t.data_ptr<int>(), offs.data_ptr<int>(),
+               counts.data_ptr<int>(), (int)E, (uint32_t)align, err.data_ptr<int>()};
+  launch_rows(plan_kernel, ctas, sorted::kThreads, sorted::pass_smem((int)E), ctas, false,
+              at::cuda::getCurrentCUDAStream(), (int)n, ctas, it);
   return {rows_t, offs, counts};
 }
 
@@ -286,141 +286,167 @@ std::vector<torch::Tensor> expert_plan(torch::Tensor ids, int64_t E, int64_t ali
 struct Plan {
   const int *rows, *offs, *counts;
   int E, k, cap;
+  int64_t align;
 };
 
-// Zeros into the layout's padding rows: part `part` of `parts` of it.
-template <typename T, int V>
-__device__ void zero_padding(const Plan& pl, T* out, int H, int part, int parts) {
-  Bits<T, V> z;
+// Zeros into the layout's padding rows by warps [warp, warps): a slot for every row that a group may have as padding,
+// then one for every row behind the last group.
+template <class B>
+__device__ __forceinline__ void clear_padding(const Plan& pl, typename B::T* out, int H, int64_t warp, int64_t warps) {
+  const int lane = threadIdx.x & 31, lanes = B::lanes(H);
+  const int64_t slots = pl.E * (pl.align - 1), behind = pl.offs[pl.E];
+  B z;
   z.zero();
-  auto clear = [&](int64_t lo, int64_t hi, int64_t first, int64_t step) {
-    for (int64_t i = lo * (H / V) + first; i < hi * (H / V); i += step) z.store(out + i * V);
-  };
-  auto row = [&](int r) { return r < 0 ? 0 : (r < pl.cap ? r : pl.cap); };
-  for (int e = part; e < pl.E; e += parts)
-    clear(row(pl.offs[e] + pl.counts[e]), row(pl.offs[e + 1]), threadIdx.x, blockDim.x);
-  clear(row(pl.offs[pl.E]), pl.cap, (int64_t)part * blockDim.x + threadIdx.x, (int64_t)parts * blockDim.x);
+  for (int64_t s = warp; s < slots + (pl.cap - behind); s += warps) {
+    int64_t r;
+    if (s < slots) {
+      const int e = (int)(s / (pl.align - 1));
+      r = (int64_t)pl.offs[e] + pl.counts[e] + (s - e * (pl.align - 1));
+      if (r >= pl.offs[e + 1]) continue;
+    } else {
+      r = behind + (s - slots);
+    }
+    if (r < 0 || r >= pl.cap) continue;
+    for (int c = lane; c < lanes; c += 32) z.store(out + r * H, c, H);
+  }
 }
 
-// CTA t < N copies row t of x to its pairs' rows; the CTAs behind clear the padding.
-template <typename T, int V>
-__global__ void __launch_bounds__(256)
-    dispatch_kernel(const T* __restrict__ x, int64_t ld, int N, int H, Plan pl, T* __restrict__ out) {
-  const int t = blockIdx.x;
-  if (t >= N) {
-    zero_padding<T, V>(pl, out, H, t - N, gridDim.x - N);
+// A warp copies row t of x to its pairs' rows; the grid's first `clear` CTAs zero the padding.
+constexpr int kMoveWarps = 8;
+template <class B>
+__global__ void __launch_bounds__(kMoveWarps * 32)
+    dispatch_kernel(const typename B::T* __restrict__ x, int64_t ld, int N, int H, Plan pl, int clear,
+                    typename B::T* __restrict__ out) {
+  constexpr int U = 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lanes = B::lanes(H);
+  if ((int)blockIdx.x < clear) {
+    clear_padding<B>(pl, out, H, blockIdx.x * kMoveWarps + warp, (int64_t)clear * kMoveWarps);
     return;
   }
+  const int t = (blockIdx.x - clear) * kMoveWarps + warp;
+  if (t >= N) return;
+  const typename B::T* src = x + t * ld;
   const int* r = pl.rows + (int64_t)t * pl.k;
-  for (int c = threadIdx.x * V; c < H; c += blockDim.x * V) {
-    Bits<T, V> b;
-    b.load(x + t * ld + c);
+  for (int c = lane; c < lanes; c += 32 * U) {
+    B b[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c + 32 * u < lanes) b[u].load(src, c + 32 * u, H);
     for (int i = 0; i < pl.k; ++i) {
       const int to = r[i];
-      if ((unsigned)to < (unsigned)pl.cap) b.store(out + (int64_t)to * H + c);
+      if ((unsigned)to >= (unsigned)pl.cap) continue;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c + 32 * u < lanes) b[u].store(out + (int64_t)to * H, c + 32 * u, H);
     }
   }
 }
 
 // CTA t sums its pairs' rows: out[t] = residual[t] + sum_i w[t, i] y[rows[t, i]], in fp32 with one rounding.
-template <typename T, int V>
-__global__ void __launch_bounds__(256)
-    combine_kernel(const T* __restrict__ y, int64_t ldy, const float* __restrict__ w, const T* __restrict__ res,
-                   int64_t ldr, int H, Plan pl, T* __restrict__ out) {
-  constexpr int kBatch = 8;
+template <class B>
+__global__ void __launch_bounds__(256, 4)
+    combine_kernel(const typename B::T* __restrict__ y, int64_t ldy, const float* __restrict__ w,
+                   const typename B::T* __restrict__ res, int64_t ldr, int H, Plan pl, typename B::T* __restrict__ out) {
+  constexpr int U = 8;
   const int64_t t = blockIdx.x;
-  for (int c = threadIdx.x * V; c < H; c += blockDim.x * V) {
-    float acc[V] = {};
-    for (int i0 = 0; i0 < pl.k; i0 += kBatch) {
-      Bits<T, V> b[kBatch];
-      float wi[kBatch];
+  const int lanes = B::lanes(H);
+  for (int c = threadIdx.x; c < lanes; c += blockDim.x) {
+    float acc[B::V] = {};
+    B r;
+    if (res) r.load_once(res + t * ldr, c, H);
+    for (int i0 = 0; i0 < pl.k; i0 += U) {
+      B b[U];
+      float wi[U];
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int i = i0 + u;
-        const int at = i < pl.k ? pl.rows[t * pl.k + i] : -1;
-        const bool here = (unsigned)at < (unsigned)pl.cap;
+      for (int u = 0; u < U; ++u) {
+        const int at = i0 + u < pl.k ? pl.rows[t * pl.k + i0 + u] : -1;
         b[u].zero();
         wi[u] = 0.f;
-        if (here) {
-          b[u].load(y + at * ldy + c);
-          wi[u] = w ? w[t * pl.k + i] : 1.f;
+        if ((unsigned)at < (unsigned)pl.cap) {
+          b[u].load_once(y + at * ldy, c, H);
+          wi[u] = w ? w[t * pl.k + i0 + u] : 1.f;
         }
       }
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
+      for (int u = 0; u < U; ++u) {
         if (i0 + u >= pl.k) break;
-        float v[V];
+        float v[B::V];
         b[u].get(v);
 #pragma unroll
-        for (int q = 0; q < V; ++q) acc[q] = fmaf(wi[u], v[q], acc[q]);
+        for (int q = 0; q < B::V; ++q) acc[q] = fmaf(wi[u], v[q], acc[q]);
       }
     }
     if (res) {
-      Bits<T, V> b;
-      b.load(res + t * ldr + c);
-      float v[V];
-      b.get(v);
+      float v[B::V];
+      r.get(v);
 #pragma unroll
-      for (int q = 0; q < V; ++q) acc[q] += v[q];
+      for (int q = 0; q < B::V; ++q) acc[q] += v[q];
     }
-    Bits<T, V> o;
+    B o;
     o.set(acc);
-    o.store(out + t * H + c);
+    o.store(out + t * H, c, H);
   }
 }
 
-// A warp takes pair j: dy[rows[j]] = w[j] g[j / k], dw[j] = <g[j / k], y[rows[j]]>; the CTAs behind clear dy's padding.
-constexpr int kPairWarps = 8;
-template <typename T, int V>
-__global__ void __launch_bounds__(kPairWarps * 32)
-    combine_bwd_kernel(const T* __restrict__ g, int64_t ldg, const T* __restrict__ y, int64_t ldy,
-                       const float* __restrict__ w, int pairs, int pair_ctas, int H, Plan pl, T* __restrict__ dy,
+// A warp takes pair j: dy[rows[j]] = w[j] g[j / k], dw[j] = <g[j / k], y[rows[j]]>; the grid's first `clear` CTAs zero
+// dy's padding.
+template <class B>
+__global__ void __launch_bounds__(kMoveWarps * 32)
+    combine_bwd_kernel(const typename B::T* __restrict__ g, int64_t ldg, const typename B::T* __restrict__ y, int64_t ldy,
+                       const float* __restrict__ w, int pairs, int clear, int H, Plan pl, typename B::T* __restrict__ dy,
                        float* __restrict__ dw) {
-  if ((int)blockIdx.x >= pair_ctas) {
-    if (dy) zero_padding<T, V>(pl, dy, H, blockIdx.x - pair_ctas, gridDim.x - pair_ctas);
+  constexpr int U = 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lanes = B::lanes(H);
+  if ((int)blockIdx.x < clear) {
+    clear_padding<B>(pl, dy, H, blockIdx.x * kMoveWarps + warp, (int64_t)clear * kMoveWarps);
     return;
   }
-  const int lane = threadIdx.x & 31;
-  const int64_t j = (int64_t)blockIdx.x * kPairWarps + (threadIdx.x >> 5);
+  const int64_t j = (int64_t)(blockIdx.x - clear) * kMoveWarps + warp;
   if (j >= pairs) return;
   const int at = pl.rows[j];
   if ((unsigned)at >= (unsigned)pl.cap) {
     if (dw && lane == 0) dw[j] = 0.f;
     return;
   }
-  const T* gr = g + j / pl.k * ldg;
-  const T* yr = y + at * ldy;
+  const typename B::T *gr = g + j / pl.k * ldg, *yr = y + at * ldy;
   const float wj = w[j];
   float dot = 0.f;
-#pragma unroll 4
-  for (int c = lane * V; c < H; c += 32 * V) {
-    Bits<T, V> b;
-    b.load(gr + c);
-    float v[V];
-    b.get(v);
-    if (dw) {
-      Bits<T, V> a;
-      a.load_once(yr + c);
-      float u[V];
-      a.get(u);
+  for (int c = lane; c < lanes; c += 32 * U) {
+    B b[U], a[U];
 #pragma unroll
-      for (int q = 0; q < V; ++q) dot = fmaf(v[q], u[q], dot);
+    for (int u = 0; u < U; ++u) {
+      a[u].zero();
+      b[u].zero();
+      if (c + 32 * u < lanes) {
+        if (dw) a[u].load_once(yr, c + 32 * u, H);
+        b[u].load(gr, c + 32 * u, H);
+      }
     }
-    if (dy) {
 #pragma unroll
-      for (int q = 0; q < V; ++q) v[q] *= wj;
-      b.set(v);
-      b.store(dy + (int64_t)at * H + c);
+    for (int u = 0; u < U; ++u) {
+      if (c + 32 * u >= lanes) break;
+      float v[B::V], x[B::V];
+      b[u].get(v);
+      a[u].get(x);
+#pragma unroll
+      for (int q = 0; q < B::V; ++q) dot = fmaf(v[q], x[q], dot);
+      if (dy) {
+#pragma unroll
+        for (int q = 0; q < B::V; ++q) v[q] *= wj;
+        b[u].set(v);
+        b[u].store(dy + (int64_t)at * H, c + 32 * u, H);
+      }
     }
   }
   dot = warp_sum(dot);
   if (dw && lane == 0) dw[j] = dot;
 }
 
-static int clear_ctas(const Plan& pl) { return std::max(1, std::min(pl.E, 148)); }
+// CTAs that clear: as many as the padding rows could keep busy, at most two on every SM.
+static int clear_ctas(const Plan& pl) { return (int)std::max<int64_t>(1, std::min<int64_t>(pl.cap / kMoveWarps, 296)); }
 
 static Plan plan_of(const torch::Tensor& rows_t, const torch::Tensor& offs, const torch::Tensor& counts, int64_t k,
-                    int64_t cap, int64_t N, const torch::Tensor& like, const char* op) {
+                    int64_t align, int64_t cap, int64_t N, const torch::Tensor& like, const char* op) {
   const int64_t E = counts.numel();
   auto ints = [&](const torch::Tensor& t) {
     return t.device() == like.device() && t.scalar_type() == at::kInt && t.is_contiguous();
@@ -429,8 +455,8 @@ static Plan plan_of(const torch::Tensor& rows_t, const torch::Tensor& offs, cons
               op);
   LIBRA_CHECK(k >= 1 && rows_t.numel() == N * k, "%s: %lld rows for a plan of %lld pairs, %lld a token", op,
               (long long)N, (long long)rows_t.numel(), (long long)k);
-  LIBRA_CHECK(cap >= 0 && cap < (1ll << 31), "%s: capacity", op);
-  return {rows_t.data_ptr<int>(), offs.data_ptr<int>(), counts.data_ptr<int>(), (int)E, (int)k, (int)cap};
+  LIBRA_CHECK(cap >= 0 && cap < (1ll << 31) && align >= 1 && align < (1ll << 31), "%s: capacity or alignment", op);
+  return {rows_t.data_ptr<int>(), offs.data_ptr<int>(), counts.data_ptr<int>(), (int)E, (int)k, (int)cap, align};
 }
 
 static void check_move(const torch::Tensor& x, const char* op, const char* what) {
@@ -438,47 +464,41 @@ static void check_move(const torch::Tensor& x, const char* op, const char* what)
   LIBRA_CHECK(x.size(0) < (1ll << 31) && x.size(1) < (1ll << 30), "%s: %s is too large", op, what);
 }
 
-static int move_threads(int64_t H, int V) { return (int)std::min<int64_t>(256, ((H + V - 1) / V + 31) / 32 * 32); }
-
-// T, and vectors or single elements
-template <typename F>
-static void by_type(const torch::Tensor& t, bool vec, F&& go) {
-  if (t.scalar_type() == at::kFloat) {
-    if (vec) go((float*)nullptr, std::integral_constant<int, 4>());
-    else go((float*)nullptr, std::integral_constant<int, 1>());
-  } else {
-    if (vec) go((__nv_bfloat16*)nullptr, std::integral_constant<int, 8>());
-    else go((__nv_bfloat16*)nullptr, std::integral_constant<int, 1>());
+// The plan's tensors and numbers, as the three entries hand them on.
+struct PlanArgs {
+  torch::Tensor rows, offs, counts;
+  int64_t k, align;
+  Plan of(int64_t cap, int64_t N, const torch::Tensor& like, const char* op) const {
+    return plan_of(rows, offs, counts, k, align, cap, N, like, op);
   }
-}
+};
 
-static torch::Tensor spread(torch::Tensor x, const torch::Tensor& rows_t, const torch::Tensor& offs,
-                            const torch::Tensor& counts, int64_t k, int64_t cap) {
+static torch::Tensor spread(torch::Tensor x, const PlanArgs& pa, int64_t cap) {
   check_move(x, "moe_dispatch", "x");
   const int64_t N = x.size(0), H = x.size(1);
-  const Plan pl = plan_of(rows_t, offs, counts, k, cap, N, x, "moe_dispatch");
+  const Plan pl = pa.of(cap, N, x, "moe_dispatch");
   const c10::cuda::CUDAGuard guard(x.device());
   x = unit_inner(x);
   auto out = torch::empty({cap, H}, x.options());
   if (cap == 0 || H == 0) return out;
-  cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  by_type(x, row_vectors(x) && row_vectors(out), [&](auto* p, auto v) {
-    using T = std::remove_pointer_t<decltype(p)>;
-    constexpr int V = decltype(v)::value;
-    launch_rows(dispatch_kernel<T, V>, N + clear_ctas(pl), move_threads(H, V), 0, 1, false, st,
-                (const T*)x.data_ptr(), x.stride(0), (int)N, (int)H, pl, (T*)out.data_ptr());
+  const int clear = clear_ctas(pl);
+  by_lanes(x, row_vectors(x) && row_vectors(out), [&](auto lanes) {
+    using B = decltype(lanes);
+    using T = typename B::T;
+    launch_rows(dispatch_kernel<B>, clear + (N + kMoveWarps - 1) / kMoveWarps, kMoveWarps * 32, 0, 1, false,
+                at::cuda::getCurrentCUDAStream(), (const T*)x.data_ptr(), x.stride(0), (int)N, (int)H, pl, clear,
+                (T*)out.data_ptr());
   });
   return out;
 }
 
 static torch::Tensor sum_back(torch::Tensor y, const c10::optional<torch::Tensor>& w,
-                              const c10::optional<torch::Tensor>& res, const torch::Tensor& rows_t,
-                              const torch::Tensor& offs, const torch::Tensor& counts, int64_t k, int64_t N) {
+                              const c10::optional<torch::Tensor>& res, const PlanArgs& pa, int64_t N) {
   check_move(y, "moe_combine", "y");
   const int64_t cap = y.size(0), H = y.size(1);
-  const Plan pl = plan_of(rows_t, offs, counts, k, cap, N, y, "moe_combine");
+  const Plan pl = pa.of(cap, N, y, "moe_combine");
   if (w.has_value())
-    LIBRA_CHECK(vocab::vec_of(*w, y, at::kFloat, N * k), "moe_combine: weights must be contiguous fp32 [T, k]");
+    LIBRA_CHECK(vocab::vec_of(*w, y, at::kFloat, N * pa.k), "moe_combine: weights must be contiguous fp32 [T, k]");
   const c10::cuda::CUDAGuard guard(y.device());
   y = unit_inner(y);
   torch::Tensor r;
@@ -490,12 +510,12 @@ static torch::Tensor sum_back(torch::Tensor y, const c10::optional<torch::Tensor
   }
   auto out = torch::empty({N, H}, y.options());
   if (N == 0 || H == 0) return out;
-  cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  by_type(y, row_vectors(y) && row_vectors(out) && (!r.defined() || row_vectors(r)), [&](auto* p, auto v) {
-    using T = std::remove_pointer_t<decltype(p)>;
-    constexpr int V = decltype(v)::value;
-    launch_rows(combine_kernel<T, V>, N, move_threads(H, V), 0, 1, false, st, (const T*)y.data_ptr(), y.stride(0),
-                w.has_value() ? (const float*)w->data_ptr<float>() : (const float*)nullptr,
+  by_lanes(y, row_vectors(y) && row_vectors(out) && (!r.defined() || row_vectors(r)), [&](auto lanes) {
+    using B = decltype(lanes);
+    using T = typename B::T;
+    const int threads = std::min(256, (B::lanes((int)H) + 31) / 32 * 32);
+    launch_rows(combine_kernel<B>, N, threads, 0, 1, false, at::cuda::getCurrentCUDAStream(), (const T*)y.data_ptr(),
+                y.stride(0), w.has_value() ? (const float*)w->data_ptr<float>() : (const float*)nullptr,
                 r.defined() ? (const T*)r.data_ptr() : (const T*)nullptr, r.defined() ? r.stride(0) : 0, (int)H, pl,
                 (T*)out.data_ptr());
   });
@@ -504,25 +524,23 @@ static torch::Tensor sum_back(torch::Tensor y, const c10::optional<torch::Tensor
 
 // -> {dy or nothing, dw or nothing}
 static std::vector<torch::Tensor> combine_bwd(torch::Tensor g, torch::Tensor y, const torch::Tensor& w,
-                                              const torch::Tensor& rows_t, const torch::Tensor& offs,
-                                              const torch::Tensor& counts, int64_t k, bool want_y, bool want_w) {
-  const int64_t N = g.size(0), cap = y.size(0), H = y.size(1), pairs = N * k;
-  const Plan pl = plan_of(rows_t, offs, counts, k, cap, N, y, "moe_combine");
+                                              const PlanArgs& pa, bool want_y, bool want_w) {
+  const int64_t N = g.size(0), cap = y.size(0), H = y.size(1), pairs = N * pa.k;
+  const Plan pl = pa.of(cap, N, y, "moe_combine");
   const c10::cuda::CUDAGuard guard(y.device());
   g = unit_inner(g);
   y = unit_inner(y);
   torch::Tensor dy, dw;
   if (want_y) dy = torch::empty({cap, H}, y.options());
   if (want_w) dw = H == 0 ? torch::zeros_like(w) : torch::empty_like(w);
-  if (H == 0 || (cap == 0 && pairs == 0)) return {dy, dw};
-  cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  const int64_t ctas = (pairs + kPairWarps - 1) / kPairWarps;
-  by_type(y, row_vectors(y) && row_vectors(g) && (!want_y || row_vectors(dy)), [&](auto* p, auto v) {
-    using T = std::remove_pointer_t<decltype(p)>;
-    constexpr int V = decltype(v)::value;
-    launch_rows(combine_bwd_kernel<T, V>, ctas + (want_y ? clear_ctas(pl) : 0), kPairWarps * 32, 0, 1, false, st,
-                (const T*)g.data_ptr(), g.stride(0), (const T*)y.data_ptr(), y.stride(0),
-                (const float*)w.data_ptr<float>(), (int)pairs, (int)ctas, (int)H, pl,
+  if (H == 0 || pairs == 0) return {dy, dw};
+  const int clear = want_y ? clear_ctas(pl) : 0;
+  by_lanes(y, row_vectors(y) && row_vectors(g) && (!want_y || row_vectors(dy)), [&](auto lanes) {
+    using B = decltype(lanes);
+    using T = typename B::T;
+    launch_rows(combine_bwd_kernel<B>, clear + (pairs + kMoveWarps - 1) / kMoveWarps, kMoveWarps * 32, 0, 1, false,
+                at::cuda::getCurrentCUDAStream(), (const T*)g.data_ptr(), g.stride(0), (const T*)y.data_ptr(),
+                y.stride(0), (const float*)w.data_ptr<float>(), (int)pairs, clear, (int)H, pl,
                 want_y ? (T*)dy.data_ptr() : (T*)nullptr, want_w ? dw.data_ptr<float>() : (float*)nullptr);
   });
   return {dy, dw};
@@ -531,44 +549,47 @@ static std::vector<torch::Tensor> combine_bwd(torch::Tensor g, torch::Tensor y, 
 struct Dispatch : public torch::autograd::Function<Dispatch> {
   using List = torch::autograd::variable_list;
   static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor x, torch::Tensor rows_t,
-                               torch::Tensor offs, torch::Tensor counts, int64_t k, int64_t cap) {
+                               torch::Tensor offs, torch::Tensor counts, int64_t k, int64_t align, int64_t cap) {
     ctx->save_for_backward({rows_t, offs, counts});
     ctx->saved_data["k"] = k;
     ctx->saved_data["N"] = x.size(0);
-    return spread(x, rows_t, offs, counts, k, cap);
+    return spread(x, {rows_t, offs, counts, k, align}, cap);
   }
   static List backward(torch::autograd::AutogradContext* ctx, List up) {
     LIBRA_CHECK(!at::GradMode::is_enabled(), "moe_dispatch: its gradient is not differentiable");
     const auto s = ctx->get_saved_variables();
-    List out(6);
-    out[0] = sum_back(up[0], c10::nullopt, c10::nullopt, s[0], s[1], s[2], ctx->saved_data["k"].toInt(),
+    List out(7);
+    out[0] = sum_back(up[0], c10::nullopt, c10::nullopt, {s[0], s[1], s[2], ctx->saved_data["k"].toInt(), 1},
                       ctx->saved_data["N"].toInt());
     return out;
   }
 };
 
 torch::Tensor moe_dispatch(torch::Tensor x, torch::Tensor rows_t, torch::Tensor offs, torch::Tensor counts, int64_t k,
-                           int64_t cap) {
-  if (at::GradMode::is_enabled() && x.requires_grad()) return Dispatch::apply(x, rows_t, offs, counts, k, cap);
-  return spread(x, rows_t, offs, counts, k, cap);
+                           int64_t align, int64_t cap) {
+  if (at::GradMode::is_enabled() && x.requires_grad()) return Dispatch::apply(x, rows_t, offs, counts, k, align, cap);
+  return spread(x, {rows_t, offs, counts, k, align}, cap);
 }
 
 struct Combine : public torch::autograd::Function<Combine> {
   using List = torch::autograd::variable_list;
   static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor y, torch::Tensor w,
                                c10::optional<torch::Tensor> res, torch::Tensor rows_t, torch::Tensor offs,
-                               torch::Tensor counts, int64_t k, int64_t N) {
+                               torch::Tensor counts, int64_t k, int64_t align, int64_t N) {
     ctx->save_for_backward({y, w, rows_t, offs, counts});
     ctx->saved_data["k"] = k;
-    return sum_back(y, w, res, rows_t, offs, counts, k, N);
+    ctx->saved_data["align"] = align;
+    return sum_back(y, w, res, {rows_t, offs, counts, k, align}, N);
   }
   static List backward(torch::autograd::AutogradContext* ctx, List up) {
     LIBRA_CHECK(!at::GradMode::is_enabled(), "moe_combine: its gradient is not differentiable");
     const auto s = ctx->get_saved_variables();
-    List out(8);
+    List out(9);
     const bool want_y = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
     if (want_y || want_w) {
-      auto r = combine_bwd(up[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["k"].toInt(), want_y, want_w);
+      auto r = combine_bwd(up[0], s[0], s[1],
+                           {s[2], s[3], s[4], ctx->saved_data["k"].toInt(), ctx->saved_data["align"].toInt()}, want_y,
+                           want_w);
       out[0] = r[0];
       out[1] = r[1];
     }
@@ -578,11 +599,11 @@ struct Combine : public torch::autograd::Function<Combine> {
 };
 
 torch::Tensor moe_combine(torch::Tensor y, torch::Tensor w, c10::optional<torch::Tensor> res, torch::Tensor rows_t,
-                          torch::Tensor offs, torch::Tensor counts, int64_t k, int64_t N) {
+                          torch::Tensor offs, torch::Tensor counts, int64_t k, int64_t align, int64_t N) {
   if (at::GradMode::is_enabled() &&
       (y.requires_grad() || w.requires_grad() || (res.has_value() && res->requires_grad())))
-    return Combine::apply(y, w, res, rows_t, offs, counts, k, N);
-  return sum_back(y, w, res, rows_t, offs, counts, k, N);
+    return Combine::apply(y, w, res, rows_t, offs, counts, k, align, N);
+  return sum_back(y, w, res, {rows_t, offs, counts, k, align}, N);
 }
 
 }  // namespace experts

@@ -11,9 +11,15 @@
 namespace libra {
 namespace sorted {
 
-constexpr int kThreads = 1024, kWarps = 32, kMaxBins = 1024;
+constexpr int kThreads = 1024, kWarps = 32, kMaxBins = 1024, kMaxCtas = 16;
 
-inline size_t pass_smem(int bins) { return ((size_t)kWarps * bins + bins + 64) * 4; }
+// Bins up to which a warp's lanes find their equals through words in shared memory: each sets its bit in its bin's word.
+// (8192 items, 512 bins: about 1 us for a CTA, with __match_any_sync 8.6 us, which takes a step for every distinct key.)
+constexpr int kWordBins = 512;
+
+inline size_t pass_smem(int bins) {
+  return ((size_t)kWarps * bins * (bins <= kWordBins ? 2 : 1) + bins + 64) * 4;
+}
 
 __device__ __forceinline__ uint32_t ld_cluster_u32(const uint32_t* p, uint32_t rank) {
   return (uint32_t)vocab::ld_cluster(reinterpret_cast<const int*>(p), rank);
@@ -43,43 +49,56 @@ __device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t* tmp) {
   return s - v + (warp ? tmp[warp - 1] : 0);
 }
 
+// Up to this many items a warp stay in registers between the two walks.
+constexpr int kBatch = 8;
+
 // One pass.  Items has
-//   Item load(int i)            item i; called twice for each
+//   Item load(int i)            item i
 //   int bin(const Item&)        its bin, or -1 for an item that gets no place
 //   void put(int i, Item, uint32_t place)   (place 0xffffffff for none)
 //   void group(int bin, uint32_t start, uint32_t count)   once for each bin; starts are multiples of `align`
-// Every CTA of the cluster calls it with all its threads; sm: pass_smem(bins) bytes.  What put writes to global memory
-// is visible to the whole cluster afterwards.
+// Every CTA of the cluster (of `ctas`, at most 16) calls it with all its threads; sm: pass_smem(bins) bytes.  What put
+// writes to global memory is visible to the whole cluster afterwards.
 template <class Items>
 __device__ __forceinline__ void counting_pass(int n, int bins, uint32_t align, uint32_t* sm, int ctas, Items& items) {
-  constexpr int kBatch = 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = threadIdx.x;
   const int rank = ctas > 1 ? (int)cluster_ctarank() : 0;
   uint32_t* total = sm + kWarps * bins;
   uint32_t* tmp = total + bins;
   uint32_t* mine = sm + warp * bins;
+  const bool by_word = bins <= kWordBins;
+  uint32_t* word = tmp + 64 + warp * bins;
   const int64_t per = (((int64_t)n + ctas * kWarps - 1) / (ctas * kWarps) + 31) / 32 * 32;
   const int64_t lo = (rank * kWarps + warp) * per;
   const int64_t hi = lo + per < n ? lo + per : n;
-
-  for (int i = lane; i < bins; i += 32) mine[i] = 0;
-  __syncwarp();
-  for (int64_t i0 = lo; i0 < hi; i0 += 32 * kBatch) {
-    int key[kBatch];
+  typename Items::Item it[kBatch];
+  auto fetch = [&](int64_t i0) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const int64_t i = i0 + 32 * u + lane;
-      key[u] = i < hi ? items.bin(items.load((int)i)) : -1;
+      if (i < hi) it[u] = items.load((int)i);
     }
+  };
+
+  fetch(lo);
+  for (int i = lane; i < bins; i += 32) {
+    mine[i] = 0;
+    if (by_word) word[i] = 0;
+  }
+  __syncwarp();
+  for (int64_t i0 = lo; i0 < hi; i0 += 32 * kBatch) {
+    if (i0 > lo) fetch(i0);
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (key[u] >= 0) atomicAdd(mine + key[u], 1u);
+    for (int u = 0; u < kBatch; ++u) {
+      const int key = i0 + 32 * u + lane < hi ? items.bin(it[u]) : -1;
+      if (key >= 0) atomicAdd(mine + key, 1u);
+    }
   }
   __syncthreads();
 
   uint32_t sum = 0;
   if (b < bins) {
-#pragma unroll 8
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) sum += sm[w * bins + b];
     total[b] = sum;
   }
@@ -87,11 +106,14 @@ __device__ __forceinline__ void counting_pass(int n, int bins, uint32_t align, u
   if (ctas > 1) {
     vocab::cluster_meet();
     if (b < bins) {
+      uint32_t v[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) v[c] = c < ctas ? ld_cluster_u32(total + b, c) : 0u;
       all = 0;
-      for (int c = 0; c < ctas; ++c) {
-        const uint32_t v = ld_cluster_u32(total + b, c);
-        all += v;
-        if (c < rank) below += v;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        all += v[c];
+        below += c < rank ? v[c] : 0u;
       }
     }
   } else {
@@ -110,23 +132,29 @@ __device__ __forceinline__ void counting_pass(int n, int bins, uint32_t align, u
   }
   __syncthreads();
 
+  const bool kept = per <= 32 * kBatch;
   for (int64_t i0 = lo; i0 < hi; i0 += 32 * kBatch) {
-    typename Items::Item it[kBatch];
+    if (!kept) fetch(i0);
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int64_t i = i0 + 32 * u + lane;
-      if (i < hi) it[u] = items.load((int)i);
-    }
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
+      if (i0 + 32 * u >= hi) break;
       const int64_t i = i0 + 32 * u + lane;
       const int key = i < hi ? items.bin(it[u]) : -1;
-      const uint32_t peers = __match_any_sync(0xffffffffu, key);
+      uint32_t peers = 0, at = 0xffffffffu;
+      if (by_word) {
+        if (key >= 0) atomicOr(word + key, 1u << lane);
+        __syncwarp();
+        if (key >= 0) peers = word[key];
+      } else {
+        peers = __match_any_sync(0xffffffffu, key);
+      }
       const int before = __popc(peers & ((1u << lane) - 1));
-      uint32_t at = 0xffffffffu;
       if (key >= 0) at = mine[key] + before;
       __syncwarp();
-      if (key >= 0 && before == 0) mine[key] += __popc(peers);
+      if (key >= 0 && before == 0) {
+        mine[key] += __popc(peers);
+        if (by_word) word[key] = 0;
+      }
       __syncwarp();
       if (i < hi) items.put((int)i, it[u], at);
     }
@@ -137,9 +165,6 @@ __device__ __forceinline__ void counting_pass(int n, int bins, uint32_t align, u
   else
     __syncthreads();
 }
-
-// CTAs of the cluster for n items.
-inline int sort_ctas(int64_t n) { return n <= 2048 ? 1 : 8; }
 
 }  // namespace sorted
 }  // namespace libra

@@ -4,8 +4,7 @@ and combine.
 
 They dispatch like the other operators of :mod:`libra_b200.ops`: CUDA tensors
 run the kernels of ``embedding.cu`` and ``expert_rows.cu``; CPU tensors run
-:mod:`libra_b200.ops.reference`.  None of them uses atomics on values: the same
-inputs give the same bits.
+:mod:`libra_b200.ops.reference`.  The same inputs give the same bits.
 """
 
 from __future__ import annotations
@@ -27,40 +26,41 @@ _ROW_TYPES = (torch.bfloat16, torch.float32)
 # embedding
 # ---------------------------------------------------------------------------
 
-def embedding_rows(tokens: torch.Tensor, weight: torch.Tensor, scale: float, first: int, whole: bool) -> torch.Tensor:
-    """``embedding`` without a gradient."""
+def embedding_rows(tokens: torch.Tensor, weight: torch.Tensor, scale: float, first: int, whole: bool,
+                   want_order: bool = False):
+    """``embedding`` without a gradient: the rows, and with ``want_order`` what ``embedding_grad`` takes of the tokens."""
     if weight.device.type != "cuda":
         with torch.no_grad():
-            return ref.embedding(tokens, weight, scale, first, whole)
+            return ref.embedding(tokens, weight, scale, first, whole), tokens
     from . import error_flag, ext
 
-    return ext().embedding_fwd(tokens, weight, scale, first, whole, error_flag(weight.device))
+    out, order = ext().embedding_fwd(tokens, weight, scale, first, whole, want_order, error_flag(weight.device))
+    return out, order
 
 
-def embedding_grad(tokens: torch.Tensor, g: torch.Tensor, weight: torch.Tensor, scale: float,
+def embedding_grad(order: torch.Tensor, g: torch.Tensor, weight: torch.Tensor, scale: float,
                    first: int) -> Optional[torch.Tensor]:
     """Gradient of ``embedding`` with respect to ``weight`` from that of its
     result: added to ``weight.main_grad`` when there is one, else returned."""
     main = getattr(weight, "main_grad", None)
-    g = g.reshape(-1, weight.shape[1])
     if weight.device.type != "cuda":
-        dw = ref.embedding_grad(tokens, g, weight.shape[0], scale, first, main)
+        dw = ref.embedding_grad(order, g.reshape(-1, weight.shape[1]), weight.shape[0], scale, first, main)
         return None if dw is None else dw.to(weight.dtype)
     from . import ext
 
-    dw = ext().embedding_bwd(tokens, g, weight, scale, first, main)
+    dw = ext().embedding_bwd(order, g, weight, scale, main)
     if main is not None:
         torch.autograd.graph.increment_version(main)
         return None
     return dw
 
 
-class _Embedding(torch.autograd.Function):
+class _EmbeddingCPU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, w, scale, first, whole):
         ctx.save_for_backward(tokens)
         ctx.w, ctx.scale, ctx.first = w, scale, first  # the gradient needs the table's shape, not its values
-        return embedding_rows(tokens, w, scale, first, whole)
+        return embedding_rows(tokens, w, scale, first, whole)[0]
 
     @staticmethod
     @once_differentiable
@@ -81,8 +81,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     raises (ValueError on the CPU).
 
     Differentiable with respect to the weight.  The gradient sums each token's
-    rows in fp32, in the order of their positions' chunks and without atomics, so that
-    it does not change from run to run.  It is added to ``weight.main_grad``
+    rows in fp32 in a fixed order, so that it does not change from run to run.  It is added to ``weight.main_grad``
     (fp32) when there is one, else it is a dense tensor like the weight."""
     if weight.dim() != 2 or weight.dtype not in _ROW_TYPES:
         raise ValueError(f"embedding: weight must be [V, H], bf16 or fp32, got {tuple(weight.shape)} {weight.dtype}")
@@ -93,9 +92,11 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
         raise ValueError("embedding: the weight's rows must be contiguous")
     tokens = tokens.contiguous()
     first, whole = (0, True) if vocab_start is None else (int(vocab_start), False)
-    if weight.requires_grad and torch.is_grad_enabled():
-        return _Embedding.apply(tokens, weight, float(scale), first, whole)
-    return embedding_rows(tokens, weight, float(scale), first, whole)
+    if weight.device.type != "cuda":
+        return _EmbeddingCPU.apply(tokens, weight, float(scale), first, whole)
+    from . import error_flag, ext
+
+    return ext().embedding(tokens, weight, scale, first, whole, error_flag(weight.device))
 
 
 # ---------------------------------------------------------------------------
@@ -139,6 +140,7 @@ class ExpertPlan:
     counts: torch.Tensor  # int32 [E]: of which the first counts[e] are its pairs', in the pairs' order
     num_tokens: int
     k: int
+    align: int
     capacity: int
 
 
@@ -167,7 +169,7 @@ def expert_plan(experts: torch.Tensor, num_experts: int, *, align: int = 128) ->
         from . import error_flag, ext
 
         rows, offs, counts = ext().expert_plan(experts.contiguous(), num_experts, align, error_flag(experts.device))
-    return ExpertPlan(rows, offs, counts, T, k, capacity)
+    return ExpertPlan(rows, offs, counts, T, k, align, capacity)
 
 
 def _check_rows(op: str, what: str, x: torch.Tensor, plan: ExpertPlan, count: int) -> None:
@@ -186,7 +188,7 @@ def moe_dispatch(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
         return ref.moe_dispatch(x, plan.rows, plan.k, plan.capacity)
     from . import ext
 
-    return ext().moe_dispatch(x, plan.rows, plan.offs, plan.counts, plan.k, plan.capacity)
+    return ext().moe_dispatch(x, plan.rows, plan.offs, plan.counts, plan.k, plan.align, plan.capacity)
 
 
 def moe_combine(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan,
@@ -211,4 +213,4 @@ def moe_combine(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan,
     from . import ext
 
     return ext().moe_combine(y, weights.contiguous(), residual, plan.rows, plan.offs, plan.counts, plan.k,
-                             plan.num_tokens)
+                             plan.align, plan.num_tokens)

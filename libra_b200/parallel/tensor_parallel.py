@@ -95,17 +95,17 @@ class _VocabParallelEmbedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, w_local, group, rank, reduce=True):
         tokens, lo = tokens.contiguous(), rank * w_local.shape[0]
-        out = embedding_rows(tokens, w_local, 1.0, lo, False)
+        out, order = embedding_rows(tokens, w_local, 1.0, lo, False, want_order=ctx.needs_input_grad[1])
         if reduce and _ws(group) > 1:
             dist.all_reduce(out, group=group)
-        ctx.save_for_backward(tokens)
+        ctx.save_for_backward(order)
         ctx.w, ctx.lo = w_local, lo
         return out
 
     @staticmethod
     def backward(ctx, g):
-        (tokens,) = ctx.saved_tensors
-        return None, embedding_grad(tokens, g, ctx.w, 1.0, ctx.lo), None, None, None
+        (order,) = ctx.saved_tensors
+        return None, embedding_grad(order, g, ctx.w, 1.0, ctx.lo), None, None, None
 
 
 def vocab_parallel_embedding(tokens, w_local, group, rank, reduce: bool = True):
