@@ -134,12 +134,13 @@ torch::Tensor embedding_bwd(torch::Tensor order, torch::Tensor g, torch::Tensor 
                             c10::optional<torch::Tensor> main);
 }  // namespace embed
 namespace experts {
-std::vector<torch::Tensor> route_topk(torch::Tensor z, int64_t k, bool normalize);
-std::vector<torch::Tensor> expert_plan(torch::Tensor ids, int64_t E, int64_t align, torch::Tensor err);
+std::tuple<torch::Tensor, torch::Tensor> route_topk(torch::Tensor z, int64_t k, bool normalize);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, int64_t> expert_plan(torch::Tensor ids, int64_t E,
+                                                                             int64_t align, torch::Tensor err);
 torch::Tensor moe_dispatch(torch::Tensor x, torch::Tensor rows_t, torch::Tensor offs, torch::Tensor counts, int64_t k,
                            int64_t align, int64_t cap);
 torch::Tensor moe_combine(torch::Tensor y, torch::Tensor w, c10::optional<torch::Tensor> res, torch::Tensor rows_t,
-                          torch::Tensor offs, torch::Tensor counts, int64_t k, int64_t align, int64_t N);
+                          torch::Tensor offs, torch::Tensor counts, int64_t k, int64_t align, int64_t cap, int64_t N);
 }  // namespace experts
 }  // namespace libra
 

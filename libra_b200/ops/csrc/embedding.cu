@@ -177,14 +177,14 @@ __device__ __forceinline__ void write_row(const Target& to, uint32_t row, int i,
   }
 }
 
-// A chunk has L pairs, the last one fewer; chunk c of the grid's first `chunks * slices` CTAs, slice by slice of 128
-// lanes of the rows.  parts holds two fp32 rows a chunk: its part of a shared run that came in from the left, and of
+// A chunk has L pairs, the last one fewer; chunk c of the grid's first `chunks * slices` CTAs, slice by slice of the
+// rows.  parts holds two fp32 rows a chunk: its part of a shared run that came in from the left, and of
 // one that starts here.  The CTAs behind clear the rows of a dense gradient that no token names.
 //
 // Loads run ahead of the sums by U pairs, those of main's rows too (kMain): a run is one or two pairs long as a rule,
 // and what a row's sum is added to would else be waited for at every run.  (Reductions at L2 in its place, 8192 x 2560:
 // 43 us, bound by their rate, against 34 us of waiting.)
-constexpr int kRunThreads = 128;
+constexpr int kRunThreads = 192;  // at most
 template <class B, int L, bool kMain>
 __global__ void __launch_bounds__(kRunThreads)
     run_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos, const uint32_t* __restrict__ seen,
@@ -193,8 +193,8 @@ __global__ void __launch_bounds__(kRunThreads)
   static_assert(L <= 32, "a warp looks at a chunk");
   const int lane = threadIdx.x & 31, lanes = B::lanes(H);
   if ((int)blockIdx.x >= chunks * slices) {
-    const int warp = (blockIdx.x - chunks * slices) * (kRunThreads / 32) + (threadIdx.x >> 5);
-    const int warps = (gridDim.x - chunks * slices) * (kRunThreads / 32);
+    const int warp = (blockIdx.x - chunks * slices) * (blockDim.x / 32) + (threadIdx.x >> 5);
+    const int warps = (gridDim.x - chunks * slices) * (blockDim.x / 32);
     B z;
     z.zero();
     for (uint32_t r = warp; r < R; r += warps) {
@@ -204,13 +204,13 @@ __global__ void __launch_bounds__(kRunThreads)
     return;
   }
   __shared__ uint32_t sk[3 * L + 2], sp[2 * L];
-  const int chunk = blockIdx.x / slices, i = (blockIdx.x - chunk * slices) * kRunThreads + threadIdx.x;
+  const int chunk = blockIdx.x / slices, i = (blockIdx.x - chunk * slices) * blockDim.x + threadIdx.x;
   const int lo = chunk * L, hi = min(n, lo + L);
-  for (int t = threadIdx.x; t < 3 * L + 2; t += kRunThreads) {
+  for (int t = threadIdx.x; t < 3 * L + 2; t += blockDim.x) {
     const int at = lo - L - 1 + t;
     sk[t] = at >= 0 && at < n ? key[at] : kNoKey;
   }
-  for (int t = threadIdx.x; t < 2 * L; t += kRunThreads) sp[t] = lo + t < n ? pos[lo + t] : 0;
+  for (int t = threadIdx.x; t < 2 * L; t += blockDim.x) sp[t] = lo + t < n ? pos[lo + t] : 0;
   __syncthreads();
   auto K = [&](int at) { return sk[at - (lo - L - 1)]; };
 
@@ -282,13 +282,13 @@ __global__ void __launch_bounds__(kRunThreads)
 }
 
 // Joins the shared runs.  A CTA looks at 32 chunks (a lane each) for runs that start there and go on through the whole
-// next chunk, and sums their parts for 128 lanes of the row.
+// next chunk, and sums their parts for a slice of the row.
 template <class B, int L>
 __global__ void __launch_bounds__(kRunThreads)
     join_kernel(const uint32_t* __restrict__ key, int n, uint32_t R, int H, int slices, Target to,
                 const float* __restrict__ parts) {
   pdl_wait();
-  const int block = blockIdx.x / slices, i = (blockIdx.x - block * slices) * kRunThreads + threadIdx.x;
+  const int block = blockIdx.x / slices, i = (blockIdx.x - block * slices) * blockDim.x + threadIdx.x;
   const int lane = threadIdx.x & 31;
   const int64_t lo = (int64_t)(block * 32 + lane) * L, hi = lo + L;
   uint32_t k = kNoKey;
@@ -318,13 +318,12 @@ __global__ void __launch_bounds__(kRunThreads)
 }
 
 static void check_tokens(const torch::Tensor& tokens, const torch::Tensor& w) {
-  LIBRA_CHECK(w.is_cuda() && w.dim() == 2 && row_type(w) && (w.size(1) <= 1 || w.stride(1) == 1),
-              "embedding: the table must be a 2-D bf16 or fp32 CUDA tensor with a unit inner stride");
-  LIBRA_CHECK(tokens.device() == w.device() && tokens.is_contiguous() &&
-                  (tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt),
-              "embedding: tokens must be contiguous int64 or int32 on the table's device");
-  LIBRA_CHECK(tokens.numel() < (1ll << 30) && w.size(0) < (1ll << 30) && w.size(1) < (1ll << 30),
-              "embedding: too many tokens, or too large a table");
+  ROWS_CHECK(w.is_cuda() && w.dim() == 2 && row_type(w), "embedding: weight must be [V, H], bf16 or fp32");
+  ROWS_CHECK(w.size(1) <= 1 || w.stride(1) == 1, "embedding: the weight's rows must be contiguous");
+  ROWS_CHECK(tokens.device() == w.device() && (tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt),
+             "embedding: tokens must be int64 or int32 on the weight's device");
+  ROWS_CHECK(tokens.numel() < (1ll << 30) && w.size(0) < (1ll << 30) && w.size(1) < (1ll << 30),
+             "embedding: too many tokens, or too large a table");
 }
 
 // -> {rows [*tokens, H], order or nothing}; whole: a token outside the table is an error, else it is another shard's;
@@ -332,16 +331,17 @@ static void check_tokens(const torch::Tensor& tokens, const torch::Tensor& w) {
 std::vector<torch::Tensor> embedding_fwd(torch::Tensor tokens, torch::Tensor w, double scale, int64_t first, bool whole,
                                          bool want_order, torch::Tensor err) {
   check_tokens(tokens, w);
+  tokens = tokens.contiguous();
   LIBRA_CHECK(err.device() == w.device() && err.scalar_type() == at::kInt, "embedding: error word");
   const int64_t n = tokens.numel(), H = w.size(1), R = w.size(0);
   const c10::cuda::CUDAGuard guard(w.device());
   auto sizes = tokens.sizes().vec();
   sizes.push_back(H);
   auto out = torch::empty(sizes, w.options());
-  torch::Tensor order, scratch;
+  torch::Tensor order;
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   const Tokens tk{tokens.data_ptr(), tokens.scalar_type() == at::kLong, first, (int)R};
-  if (want_order) order = torch::empty({2 * n + (R + 31) / 32}, w.options().dtype(at::kInt));
+  if (want_order) order = torch::empty({4 * n + (R + 31) / 32}, w.options().dtype(at::kInt));  // 2 n of it scratch
   if (n == 0 || H == 0) return {out, order};
   by_lanes(w, row_vectors(w), [&](auto lanes) {
     using B = decltype(lanes);
@@ -360,11 +360,10 @@ std::vector<torch::Tensor> embedding_fwd(torch::Tensor tokens, torch::Tensor w, 
     o.passes = (total + kDigit - 1) / kDigit;
     o.bits = (total + o.passes - 1) / o.passes;
     o.ctas = n <= 1024 ? 1 : 8;
-    if (o.passes > 1) scratch = torch::empty({2 * n}, w.options().dtype(at::kInt));
     o.key = (uint32_t*)order.data_ptr<int>();
     o.pos = o.key + n;
-    o.seen = o.key + 2 * n;
-    o.scratch = o.passes > 1 ? (uint32_t*)scratch.data_ptr<int>() : nullptr;
+    o.scratch = o.key + 2 * n;
+    o.seen = o.key + 4 * n;
     const int64_t look = std::min<int64_t>((n + sorted::kWarps - 1) / sorted::kWarps, 148 - o.ctas);
     launch_rows(lookup_sort_kernel<B>, o.ctas * (1 + (look + o.ctas - 1) / o.ctas), sorted::kThreads,
                 sorted::pass_smem(1 << o.bits), o.ctas, false, st, tk, o, table, w.stride(0), whole, (float)scale, (int)H,
@@ -383,10 +382,10 @@ torch::Tensor embedding_bwd(torch::Tensor order, torch::Tensor g, torch::Tensor 
   if (g.dim() != 2) g = g.reshape({H ? g.numel() / H : 0, H});
   const int64_t n = g.size(0);
   LIBRA_CHECK(order.device() == w.device() && order.scalar_type() == at::kInt && order.is_contiguous() &&
-                  (H == 0 || order.numel() == 2 * n + (R + 31) / 32),
+                  (H == 0 || order.numel() == 4 * n + (R + 31) / 32),
               "embedding: the order is not that of these tokens");
   if (main.has_value())
-    LIBRA_CHECK(main->device() == w.device() && main->scalar_type() == at::kFloat && main->is_contiguous() &&
+    ROWS_CHECK(main->device() == w.device() && main->scalar_type() == at::kFloat && main->is_contiguous() &&
                     main->numel() == R * H,
                 "embedding: main_grad must be contiguous fp32 of the table's shape");
   const c10::cuda::CUDAGuard guard(w.device());
@@ -397,7 +396,7 @@ torch::Tensor embedding_bwd(torch::Tensor order, torch::Tensor g, torch::Tensor 
     return out;
   }
   if (!main.has_value()) out = torch::empty({R, H}, w.options());
-  const uint32_t *key = (const uint32_t*)order.data_ptr<int>(), *pos = key + n, *seen = key + 2 * n;
+  const uint32_t *key = (const uint32_t*)order.data_ptr<int>(), *pos = key + n, *seen = key + 4 * n;
   const Target to{main.has_value() ? nullptr : out.data_ptr(), main.has_value() ? main->data_ptr<float>() : nullptr,
                   (float)scale};
   const bool wide = row_vectors(g) && (main.has_value() ? reinterpret_cast<uintptr_t>(to.main) % 16 == 0
@@ -409,14 +408,15 @@ torch::Tensor embedding_bwd(torch::Tensor order, torch::Tensor g, torch::Tensor 
     auto go = [&](auto len) {
       constexpr int L = decltype(len)::value;
       const int64_t chunks = (n + L - 1) / L;
-      const int slices = (B::lanes((int)H) + kRunThreads - 1) / kRunThreads;
+      const int lanes = B::lanes((int)H), slices = (lanes + kRunThreads - 1) / kRunThreads;
+      const int threads = ((lanes + slices - 1) / slices + 31) / 32 * 32;
       auto parts = torch::empty({chunks, 2, H}, w.options().dtype(at::kFloat));
       const int64_t clear = main.has_value() ? 0 : std::min<int64_t>((R + 3) / 4, 148 * 8);
       LIBRA_CHECK(chunks * slices + clear < (1ll << 31), "embedding: too many tokens");
-      launch_rows(main.has_value() ? run_kernel<B, L, true> : run_kernel<B, L, false>, chunks * slices + clear, kRunThreads, 0, 1, false, st, key, pos, seen, (int)n,
+      launch_rows(main.has_value() ? run_kernel<B, L, true> : run_kernel<B, L, false>, chunks * slices + clear, threads, 0, 1, false, st, key, pos, seen, (int)n,
                   (uint32_t)R, (const T*)g.data_ptr(), g.stride(0), (int)H, (int)chunks, slices, to,
                   parts.data_ptr<float>());
-      launch_rows(join_kernel<B, L>, (chunks + 31) / 32 * slices, kRunThreads, 0, 1, true, st, key, (int)n, (uint32_t)R,
+      launch_rows(join_kernel<B, L>, (chunks + 31) / 32 * slices, threads, 0, 1, true, st, key, (int)n, (uint32_t)R,
                   (int)H, slices, to, (const float*)parts.data_ptr<float>());
     };
     if (n <= 16384)

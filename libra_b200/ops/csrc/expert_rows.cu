@@ -141,12 +141,11 @@ static void by_width(int E, F&& go) {
 
 // -> {weights fp32 [N, k], experts int64 [N, k], stats fp32 [N, 2] or empty}
 static std::vector<torch::Tensor> route_fwd(const torch::Tensor& z, int64_t k, bool normalize, bool want_stats) {
-  LIBRA_CHECK(z.is_cuda() && z.dim() == 2 && row_type(z), "route_topk: logits must be a 2-D bf16 or fp32 CUDA tensor");
-  LIBRA_CHECK(z.size(1) <= 1 || z.stride(1) == 1, "route_topk: logits need a unit inner stride");
+  ROWS_CHECK(z.is_cuda() && z.dim() == 2 && row_type(z), "route_topk: logits must be [T, E], bf16 or fp32");
   const int64_t N = z.size(0), E = z.size(1);
-  LIBRA_CHECK(E >= 1 && E <= kRouteMax && k >= 1 && k <= E, "route_topk: 1 to %d experts and k in [1, %lld]", kRouteMax,
-              (long long)E);
-  LIBRA_CHECK(N < (1ll << 31), "route_topk: too many rows");
+  ROWS_CHECK(E >= 1 && E <= kRouteMax && k >= 1 && k <= E, "route_topk: 1 to %d experts and k in [1, %lld], got %lld and "
+             "%lld", kRouteMax, (long long)E, (long long)E, (long long)k);
+  ROWS_CHECK(N < (1ll << 31), "route_topk: too many rows");
   const c10::cuda::CUDAGuard guard(z.device());
   auto w = torch::empty({N, k}, z.options().dtype(at::kFloat));
   auto ids = torch::empty({N, k}, z.options().dtype(at::kLong));
@@ -213,12 +212,12 @@ struct RouteTopk : public torch::autograd::Function<RouteTopk> {
   }
 };
 
-// -> {weights fp32 [N, k], experts int64 [N, k]}, differentiable
-std::vector<torch::Tensor> route_topk(torch::Tensor z, int64_t k, bool normalize) {
-  if (at::GradMode::is_enabled() && z.requires_grad()) return RouteTopk::apply(z, k, normalize);
-  auto r = route_fwd(z, k, normalize, false);
-  r.pop_back();
-  return r;
+// -> weights fp32 [N, k], experts int64 [N, k], differentiable
+std::tuple<torch::Tensor, torch::Tensor> route_topk(torch::Tensor z, int64_t k, bool normalize) {
+  if (z.dim() == 2) z = unit_inner(z);
+  const auto r = at::GradMode::is_enabled() && z.requires_grad() ? RouteTopk::apply(z, k, normalize)
+                                                                  : route_fwd(z, k, normalize, false);
+  return {r[0], r[1]};
 }
 
 // ------------------------------------------------------------------ plan
@@ -262,13 +261,19 @@ __global__ void __launch_bounds__(sorted::kThreads) plan_kernel(int n, int ctas,
   sorted::counting_pass(n, items.E, items.align, sm, ctas, items);
 }
 
-// -> {rows int32 [n], offs int32 [E + 1], counts int32 [E]}
-std::vector<torch::Tensor> expert_plan(torch::Tensor ids, int64_t E, int64_t align, torch::Tensor err) {
-  LIBRA_CHECK(ids.is_cuda() && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) && ids.is_contiguous(),
-              "expert_plan: experts must be a contiguous int64 or int32 CUDA tensor");
-  LIBRA_CHECK(E >= 1 && E <= sorted::kMaxBins, "expert_plan: 1 to %d experts", sorted::kMaxBins);
+// experts [T, k] -> rows int32 [T * k], offs int32 [E + 1], counts int32 [E], and the layout's capacity
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, int64_t> expert_plan(torch::Tensor ids, int64_t E, int64_t align,
+                                                                             torch::Tensor err) {
+  ROWS_CHECK(ids.is_cuda() && ids.dim() == 2 && ids.size(1) >= 1 &&
+                 (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt),
+             "expert_plan: experts must be int64 or int32 [T, k]");
+  ROWS_CHECK(E >= 1 && E <= sorted::kMaxBins && align >= 1, "expert_plan: 1 to %d experts and align >= 1, got %lld and "
+             "%lld", sorted::kMaxBins, (long long)E, (long long)align);
+  ids = ids.contiguous();
   const int64_t n = ids.numel();
-  LIBRA_CHECK(align >= 1 && n + (align - 1) * std::min(E, n) < (1ll << 31), "expert_plan: too many rows");
+  ROWS_CHECK(n < (1ll << 31) && align < (1ll << 31) && n + (align - 1) * std::min(E, n) < (1ll << 31),
+             "expert_plan: %lld pairs with align %lld do not fit 31 bits", (long long)n, (long long)align);
+  const int64_t cap = n + (align - 1) * std::min(E, n);
   LIBRA_CHECK(err.device() == ids.device() && err.scalar_type() == at::kInt, "expert_plan: error word");
   const c10::cuda::CUDAGuard guard(ids.device());
   const auto i32 = ids.options().dtype(at::kInt);
@@ -278,7 +283,7 @@ std::vector<torch::Tensor> expert_plan(torch::Tensor ids, int64_t E, int64_t ali
                counts.data_ptr<int>(), (int)E, (uint32_t)align, err.data_ptr<int>()};
   launch_rows(plan_kernel, ctas, sorted::kThreads, sorted::pass_smem((int)E), ctas, false,
               at::cuda::getCurrentCUDAStream(), (int)n, ctas, it);
-  return {rows_t, offs, counts};
+  return {rows_t, offs, counts, cap};
 }
 
 // ------------------------------------------------------------------ moves
@@ -317,7 +322,7 @@ template <class B>
 __global__ void __launch_bounds__(kMoveWarps * 32)
     dispatch_kernel(const typename B::T* __restrict__ x, int64_t ld, int N, int H, Plan pl, int clear,
                     typename B::T* __restrict__ out) {
-  constexpr int U = 4;
+  constexpr int U = 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lanes = B::lanes(H);
   if ((int)blockIdx.x < clear) {
     clear_padding<B>(pl, out, H, blockIdx.x * kMoveWarps + warp, (int64_t)clear * kMoveWarps);
@@ -327,17 +332,19 @@ __global__ void __launch_bounds__(kMoveWarps * 32)
   if (t >= N) return;
   const typename B::T* src = x + t * ld;
   const int* r = pl.rows + (int64_t)t * pl.k;
-  for (int c = lane; c < lanes; c += 32 * U) {
+  const int mine = lane < pl.k ? r[lane] : -1;
+  for (int c = lane; c - lane < lanes; c += 32 * U) {
     B b[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (c + 32 * u < lanes) b[u].load(src, c + 32 * u, H);
     for (int i = 0; i < pl.k; ++i) {
-      const int to = r[i];
+      const int to = i < 32 ? __shfl_sync(0xffffffffu, mine, i) : r[i];
       if ((unsigned)to >= (unsigned)pl.cap) continue;
+      typename B::T* dst = out + (int64_t)to * H;
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (c + 32 * u < lanes) b[u].store(out + (int64_t)to * H, c + 32 * u, H);
+        if (c + 32 * u < lanes) b[u].store(dst, c + 32 * u, H);
     }
   }
 }
@@ -357,19 +364,19 @@ __global__ void __launch_bounds__(256, 4)
     for (int i0 = 0; i0 < pl.k; i0 += U) {
       B b[U];
       float wi[U];
+      bool here[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int at = i0 + u < pl.k ? pl.rows[t * pl.k + i0 + u] : -1;
-        b[u].zero();
-        wi[u] = 0.f;
-        if ((unsigned)at < (unsigned)pl.cap) {
+        here[u] = (unsigned)at < (unsigned)pl.cap;
+        if (here[u]) {
           b[u].load_once(y + at * ldy, c, H);
           wi[u] = w ? w[t * pl.k + i0 + u] : 1.f;
         }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (i0 + u >= pl.k) break;
+        if (!here[u]) continue;
         float v[B::V];
         b[u].get(v);
 #pragma unroll
@@ -442,8 +449,8 @@ __global__ void __launch_bounds__(kMoveWarps * 32)
   if (dw && lane == 0) dw[j] = dot;
 }
 
-// CTAs that clear: as many as the padding rows could keep busy, at most two on every SM.
-static int clear_ctas(const Plan& pl) { return (int)std::max<int64_t>(1, std::min<int64_t>(pl.cap / kMoveWarps, 296)); }
+// CTAs that clear: as many as the padding rows could keep busy, at most four on every SM.
+static int clear_ctas(const Plan& pl) { return (int)std::max<int64_t>(1, std::min<int64_t>(pl.cap / kMoveWarps, 592)); }
 
 static Plan plan_of(const torch::Tensor& rows_t, const torch::Tensor& offs, const torch::Tensor& counts, int64_t k,
                     int64_t align, int64_t cap, int64_t N, const torch::Tensor& like, const char* op) {
@@ -451,17 +458,17 @@ static Plan plan_of(const torch::Tensor& rows_t, const torch::Tensor& offs, cons
   auto ints = [&](const torch::Tensor& t) {
     return t.device() == like.device() && t.scalar_type() == at::kInt && t.is_contiguous();
   };
-  LIBRA_CHECK(ints(rows_t) && ints(offs) && ints(counts) && offs.numel() == E + 1, "%s: not a plan on the rows' device",
-              op);
-  LIBRA_CHECK(k >= 1 && rows_t.numel() == N * k, "%s: %lld rows for a plan of %lld pairs, %lld a token", op,
-              (long long)N, (long long)rows_t.numel(), (long long)k);
-  LIBRA_CHECK(cap >= 0 && cap < (1ll << 31) && align >= 1 && align < (1ll << 31), "%s: capacity or alignment", op);
+  ROWS_CHECK(ints(rows_t) && ints(offs) && ints(counts) && offs.numel() == E + 1, "%s: not a plan on the rows' device",
+             op);
+  ROWS_CHECK(k >= 1 && rows_t.numel() == N * k, "%s: %lld tokens for a plan of %lld pairs, %lld a token", op,
+             (long long)N, (long long)rows_t.numel(), (long long)k);
+  ROWS_CHECK(cap >= 0 && cap < (1ll << 31) && align >= 1 && align < (1ll << 31), "%s: capacity or alignment", op);
   return {rows_t.data_ptr<int>(), offs.data_ptr<int>(), counts.data_ptr<int>(), (int)E, (int)k, (int)cap, align};
 }
 
 static void check_move(const torch::Tensor& x, const char* op, const char* what) {
-  LIBRA_CHECK(x.is_cuda() && x.dim() == 2 && row_type(x), "%s: %s must be a 2-D bf16 or fp32 CUDA tensor", op, what);
-  LIBRA_CHECK(x.size(0) < (1ll << 31) && x.size(1) < (1ll << 30), "%s: %s is too large", op, what);
+  ROWS_CHECK(x.is_cuda() && x.dim() == 2 && row_type(x), "%s: %s must be 2-D, bf16 or fp32", op, what);
+  ROWS_CHECK(x.size(0) < (1ll << 31) && x.size(1) < (1ll << 30), "%s: %s is too large", op, what);
 }
 
 // The plan's tensors and numbers, as the three entries hand them on.
@@ -498,14 +505,15 @@ static torch::Tensor sum_back(torch::Tensor y, const c10::optional<torch::Tensor
   const int64_t cap = y.size(0), H = y.size(1);
   const Plan pl = pa.of(cap, N, y, "moe_combine");
   if (w.has_value())
-    LIBRA_CHECK(vocab::vec_of(*w, y, at::kFloat, N * pa.k), "moe_combine: weights must be contiguous fp32 [T, k]");
+    ROWS_CHECK(w->dim() == 2 && w->size(0) == N && w->size(1) == pa.k && vocab::vec_of(*w, y, at::kFloat, N * pa.k),
+               "moe_combine: weights must be [%lld, %lld] on y's device", (long long)N, (long long)pa.k);
   const c10::cuda::CUDAGuard guard(y.device());
   y = unit_inner(y);
   torch::Tensor r;
   if (res.has_value()) {
-    LIBRA_CHECK(res->device() == y.device() && res->scalar_type() == y.scalar_type() && res->dim() == 2 &&
-                    res->size(0) == N && res->size(1) == H,
-                "moe_combine: the residual must be [T, H] of y's type");
+    ROWS_CHECK(res->device() == y.device() && res->scalar_type() == y.scalar_type() && res->dim() == 2 &&
+                   res->size(0) == N && res->size(1) == H,
+               "moe_combine: the residual must be [%lld, %lld] of y's type and device", (long long)N, (long long)H);
     r = unit_inner(*res);
   }
   auto out = torch::empty({N, H}, y.options());
@@ -599,7 +607,10 @@ struct Combine : public torch::autograd::Function<Combine> {
 };
 
 torch::Tensor moe_combine(torch::Tensor y, torch::Tensor w, c10::optional<torch::Tensor> res, torch::Tensor rows_t,
-                          torch::Tensor offs, torch::Tensor counts, int64_t k, int64_t align, int64_t N) {
+                          torch::Tensor offs, torch::Tensor counts, int64_t k, int64_t align, int64_t cap, int64_t N) {
+  ROWS_CHECK(y.dim() == 2 && y.size(0) == cap, "moe_combine: y must be [%lld, H], bf16 or fp32", (long long)cap);
+  if (w.scalar_type() != at::kFloat) w = w.to(at::kFloat);
+  if (!w.is_contiguous()) w = w.contiguous();
   if (at::GradMode::is_enabled() &&
       (y.requires_grad() || w.requires_grad() || (res.has_value() && res->requires_grad())))
     return Combine::apply(y, w, res, rows_t, offs, counts, k, align, N);

@@ -6,6 +6,16 @@
 #pragma once
 #include "vocab_rows.cuh"
 
+// Argument checks: ValueError in Python, as for CPU tensors.
+#define ROWS_CHECK(cond, ...)                                     \
+  do {                                                            \
+    if (!(cond)) {                                                \
+      char rows_msg_[768];                                        \
+      std::snprintf(rows_msg_, sizeof(rows_msg_), __VA_ARGS__);   \
+      throw std::invalid_argument(rows_msg_);                     \
+    }                                                             \
+  } while (0)
+
 namespace libra {
 namespace rows {
 

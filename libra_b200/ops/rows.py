@@ -15,6 +15,8 @@ from typing import Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
+import libra_b200.ops as _lib
+
 from . import reference as ref
 
 MAX_EXPERTS = 1024  # of route_topk and expert_plan
@@ -32,10 +34,8 @@ def embedding_rows(tokens: torch.Tensor, weight: torch.Tensor, scale: float, fir
     if weight.device.type != "cuda":
         with torch.no_grad():
             return ref.embedding(tokens, weight, scale, first, whole), tokens
-    from . import error_flag, ext
-
-    out, order = ext().embedding_fwd(tokens, weight, scale, first, whole, want_order, error_flag(weight.device))
-    return out, order
+    return tuple(_lib.ext().embedding_fwd(tokens, weight, scale, first, whole, want_order,
+                                          _lib.error_flag(weight.device)))
 
 
 def embedding_grad(order: torch.Tensor, g: torch.Tensor, weight: torch.Tensor, scale: float,
@@ -46,9 +46,7 @@ def embedding_grad(order: torch.Tensor, g: torch.Tensor, weight: torch.Tensor, s
     if weight.device.type != "cuda":
         dw = ref.embedding_grad(order, g.reshape(-1, weight.shape[1]), weight.shape[0], scale, first, main)
         return None if dw is None else dw.to(weight.dtype)
-    from . import ext
-
-    dw = ext().embedding_bwd(order, g, weight, scale, main)
+    dw = _lib.ext().embedding_bwd(order, g, weight, scale, main)
     if main is not None:
         torch.autograd.graph.increment_version(main)
         return None
@@ -83,6 +81,9 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     Differentiable with respect to the weight.  The gradient sums each token's
     rows in fp32 in a fixed order, so that it does not change from run to run.  It is added to ``weight.main_grad``
     (fp32) when there is one, else it is a dense tensor like the weight."""
+    first, whole = (0, True) if vocab_start is None else (int(vocab_start), False)
+    if weight.is_cuda:
+        return _lib.ext().embedding(tokens, weight, scale, first, whole, _lib.error_flag(weight.device))
     if weight.dim() != 2 or weight.dtype not in _ROW_TYPES:
         raise ValueError(f"embedding: weight must be [V, H], bf16 or fp32, got {tuple(weight.shape)} {weight.dtype}")
     if tokens.dtype not in (torch.int64, torch.int32) or tokens.device != weight.device:
@@ -90,13 +91,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
                          f"{tokens.device}")
     if weight.stride(1) != 1 and weight.shape[1] > 1:
         raise ValueError("embedding: the weight's rows must be contiguous")
-    tokens = tokens.contiguous()
-    first, whole = (0, True) if vocab_start is None else (int(vocab_start), False)
-    if weight.device.type != "cuda":
-        return _EmbeddingCPU.apply(tokens, weight, float(scale), first, whole)
-    from . import error_flag, ext
-
-    return ext().embedding(tokens, weight, scale, first, whole, error_flag(weight.device))
+    return _EmbeddingCPU.apply(tokens, weight, float(scale), first, whole)
 
 
 # ---------------------------------------------------------------------------
@@ -112,19 +107,15 @@ def route_topk(logits: torch.Tensor, k: int, *, normalize: bool = True) -> Tuple
     weight 0; a row of nothing but -inf has weights 0 and experts 0 to k - 1.
     NaN ranks above +inf and makes the row's weights NaN.  The weights are
     differentiable with respect to the logits."""
+    if logits.is_cuda:
+        return _lib.ext().route_topk(logits, k, normalize)
     k = int(k)
     if logits.dim() != 2 or logits.dtype not in _ROW_TYPES:
         raise ValueError(f"route_topk: logits must be [T, E], bf16 or fp32, got {tuple(logits.shape)} {logits.dtype}")
     E = logits.shape[1]
     if not 1 <= E <= MAX_EXPERTS or not 1 <= k <= E:
         raise ValueError(f"route_topk: 1 to {MAX_EXPERTS} experts and k in [1, {E}], got {E} and {k}")
-    if logits.device.type != "cuda":
-        return ref.route_topk(logits, k, normalize)
-    from . import ext
-
-    if logits.stride(1) != 1 and E > 1:
-        logits = logits.contiguous()
-    return tuple(ext().route_topk(logits, k, bool(normalize)))
+    return ref.route_topk(logits, k, normalize)
 
 
 # ---------------------------------------------------------------------------
@@ -153,6 +144,10 @@ def expert_plan(experts: torch.Tensor, num_experts: int, *, align: int = 128) ->
     A negative id leaves its pair without an expert (a padding token).  An id
     of ``num_experts`` or more does so too and sets the error word that
     ``check_kernel_errors`` raises (ValueError on the CPU)."""
+    if experts.is_cuda:
+        rows, offs, counts, capacity = _lib.ext().expert_plan(experts, num_experts, align,
+                                                              _lib.error_flag(experts.device))
+        return ExpertPlan(rows, offs, counts, experts.shape[0], experts.shape[1], align, capacity)
     if experts.dim() != 2 or experts.shape[1] < 1 or experts.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"expert_plan: experts must be int64 or int32 [T, k], got {tuple(experts.shape)} "
                          f"{experts.dtype}")
@@ -163,13 +158,7 @@ def expert_plan(experts: torch.Tensor, num_experts: int, *, align: int = 128) ->
     capacity = T * k + (align - 1) * min(num_experts, T * k)
     if capacity >= 2 ** 31:
         raise ValueError(f"expert_plan: {capacity} rows do not fit 31 bits")
-    if experts.device.type != "cuda":
-        rows, offs, counts = ref.expert_plan(experts, num_experts, align)
-    else:
-        from . import error_flag, ext
-
-        rows, offs, counts = ext().expert_plan(experts.contiguous(), num_experts, align, error_flag(experts.device))
-    return ExpertPlan(rows, offs, counts, T, k, align, capacity)
+    return ExpertPlan(*ref.expert_plan(experts, num_experts, align), T, k, align, capacity)
 
 
 def _check_rows(op: str, what: str, x: torch.Tensor, plan: ExpertPlan, count: int) -> None:
@@ -183,12 +172,10 @@ def moe_dispatch(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
     """Rows x [T, H] (bf16 or fp32) copied to their experts' groups:
     [capacity, H], zeros in every row that is no pair's.  Differentiable: a
     token's gradient is the fp32 sum over its pairs' rows."""
+    if x.is_cuda:
+        return _lib.ext().moe_dispatch(x, plan.rows, plan.offs, plan.counts, plan.k, plan.align, plan.capacity)
     _check_rows("moe_dispatch", "x", x, plan, plan.num_tokens)
-    if x.device.type != "cuda":
-        return ref.moe_dispatch(x, plan.rows, plan.k, plan.capacity)
-    from . import ext
-
-    return ext().moe_dispatch(x, plan.rows, plan.offs, plan.counts, plan.k, plan.align, plan.capacity)
+    return ref.moe_dispatch(x, plan.rows, plan.k, plan.capacity)
 
 
 def moe_combine(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan,
@@ -198,6 +185,9 @@ def moe_combine(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan,
     and an optional residual [T, H] of y's type: summed in fp32 in the order of
     i, one rounding.  A pair without an expert adds nothing.  Differentiable
     with respect to y (zeros in rows that are no pair's), weights and residual."""
+    if y.is_cuda:
+        return _lib.ext().moe_combine(y, weights, residual, plan.rows, plan.offs, plan.counts, plan.k, plan.align,
+                                      plan.capacity, plan.num_tokens)
     _check_rows("moe_combine", "y", y, plan, plan.capacity)
     if tuple(weights.shape) != (plan.num_tokens, plan.k) or weights.device != y.device:
         raise ValueError(f"moe_combine: weights must be [{plan.num_tokens}, {plan.k}] on {y.device}, got "
@@ -206,11 +196,4 @@ def moe_combine(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan,
                                  or residual.device != y.device):
         raise ValueError(f"moe_combine: the residual must be [{plan.num_tokens}, {y.shape[1]}] {y.dtype} on "
                          f"{y.device}, got {tuple(residual.shape)} {residual.dtype} on {residual.device}")
-    if weights.dtype != torch.float32:
-        weights = weights.float()
-    if y.device.type != "cuda":
-        return ref.moe_combine(y, weights, plan.rows, plan.k, residual)
-    from . import ext
-
-    return ext().moe_combine(y, weights.contiguous(), residual, plan.rows, plan.offs, plan.counts, plan.k,
-                             plan.align, plan.num_tokens)
+    return ref.moe_combine(y, weights.float(), plan.rows, plan.k, residual)
