@@ -76,80 +76,90 @@ struct Order {
   uint32_t *key, *pos, *seen, *scratch;  // scratch: 2 n
   int n, passes, bits, ctas;
 };
+// Few warps: with 512 bins a warp's counters cost more than its items (8192 tokens in 8 CTAs of 32 warps: 16 us).
+constexpr int kSortWarps = 8;
 constexpr int kDigit = 9;  // at most sorted::kWordBins bins a pass
 
 __device__ __forceinline__ void sort_tokens(const Tokens& tk, const Order& o, uint32_t* sm) {
   const uint32_t mask = (1u << o.bits) - 1;
   const int words = (tk.rows + 31) / 32;
   // cleared before the first put: a pass's barriers lie between
-  for (int i = blockIdx.x * sorted::kThreads + threadIdx.x; i < words; i += o.ctas * sorted::kThreads) o.seen[i] = 0;
+  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < words; i += o.ctas * blockDim.x) o.seen[i] = 0;
   auto key = [&](int p) { return ((o.passes - 1 - p) & 1) ? o.scratch : o.key; };
   auto pos = [&](int p) { return ((o.passes - 1 - p) & 1) ? o.scratch + o.n : o.pos; };
   FirstPass p0{tk, {0, mask}, key(0), pos(0), o.seen};
-  sorted::counting_pass(o.n, 1 << o.bits, 1u, sm, o.ctas, p0);
+  sorted::counting_pass<kSortWarps>(o.n, 1 << o.bits, 1u, sm, o.ctas, p0);
   for (int p = 1; p < o.passes; ++p) {
     NextPass q{key(p - 1), pos(p - 1), {p * o.bits, mask}, key(p), pos(p)};
-    sorted::counting_pass(o.n, 1 << o.bits, 1u, sm, o.ctas, q);
+    sorted::counting_pass<kSortWarps>(o.n, 1 << o.bits, 1u, sm, o.ctas, q);
   }
 }
 
 // ------------------------------------------------------------------ lookup
 
-// A warp takes a row, eight loads a lane at a time.
+// A warp takes an equal part of a row, at most eight loads a lane: part p of item i is unit i * parts + p.
+constexpr int kLookLoads = 8;
+struct Parts {
+  int parts, per;  // per: lanes of a part, a multiple of 32
+};
 template <class B>
-__device__ __forceinline__ void look_up(const Tokens& tk, int i, const typename B::T* w, int64_t ld, bool whole,
-                                        float scale, int H, typename B::T* out, int* err) {
-  constexpr int U = 8;
-  const int lane = threadIdx.x & 31, lanes = B::lanes(H);
+static Parts parts_of(int H) {
+  const int lanes = B::lanes(H), parts = std::max(1, (lanes + 32 * kLookLoads - 1) / (32 * kLookLoads));
+  return {parts, ((lanes + parts - 1) / parts + 31) / 32 * 32};
+}
+
+template <class B>
+__device__ __forceinline__ void look_up(const Tokens& tk, int64_t unit, const Parts& pt, const typename B::T* w, int64_t ld,
+                                        bool whole, float scale, int H, typename B::T* out, int* err) {
+  const int i = (int)(unit / pt.parts), p = (int)(unit - (int64_t)i * pt.parts);
+  const int lane = threadIdx.x & 31, c = p * pt.per + lane, stop = min(B::lanes(H), (p + 1) * pt.per);
   const uint32_t r = tk.row(i);
   const bool here = r < (uint32_t)tk.rows;
   if (!here && whole && lane == 0) atomicCAS(err, 0, kBadArgument);
   const typename B::T* src = w + (int64_t)r * ld;
   typename B::T* dst = out + (int64_t)i * H;
-  for (int c = lane; c < lanes; c += 32 * U) {
-    B b[U];
+  B b[kLookLoads];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (here && c + 32 * u < lanes) b[u].load(src, c + 32 * u, H);
-      else b[u].zero();
+  for (int u = 0; u < kLookLoads; ++u) {
+    if (here && c + 32 * u < stop) b[u].load(src, c + 32 * u, H);
+    else b[u].zero();
+  }
+#pragma unroll
+  for (int u = 0; u < kLookLoads; ++u) {
+    if (c + 32 * u >= stop) break;
+    if (scale != 1.f) {
+      float v[B::V];
+      b[u].get(v);
+#pragma unroll
+      for (int q = 0; q < B::V; ++q) v[q] *= scale;
+      b[u].set(v);
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (c + 32 * u >= lanes) break;
-      if (scale != 1.f) {
-        float v[B::V];
-        b[u].get(v);
-#pragma unroll
-        for (int q = 0; q < B::V; ++q) v[q] *= scale;
-        b[u].set(v);
-      }
-      b[u].store(dst, c + 32 * u, H);
-    }
+    b[u].store(dst, c + 32 * u, H);
   }
 }
 
 constexpr int kLookWarps = 4;
 template <class B>
 __global__ void __launch_bounds__(kLookWarps * 32)
-    lookup_kernel(Tokens tk, int n, const typename B::T* __restrict__ w, int64_t ld, bool whole, float scale, int H,
-                  typename B::T* __restrict__ out, int* err) {
-  const int i = blockIdx.x * kLookWarps + (threadIdx.x >> 5);
-  if (i < n) look_up<B>(tk, i, w, ld, whole, scale, H, out, err);
+    lookup_kernel(Tokens tk, int64_t units, Parts pt, const typename B::T* __restrict__ w, int64_t ld, bool whole,
+                  float scale, int H, typename B::T* __restrict__ out, int* err) {
+  const int64_t u = (int64_t)blockIdx.x * kLookWarps + (threadIdx.x >> 5);
+  if (u < units) look_up<B>(tk, u, pt, w, ld, whole, scale, H, out, err);
 }
 
 // The first cluster sorts, the CTAs behind it look up.
 template <class B>
-__global__ void __launch_bounds__(sorted::kThreads)
-    lookup_sort_kernel(Tokens tk, Order o, const typename B::T* __restrict__ w, int64_t ld, bool whole, float scale,
-                       int H, typename B::T* __restrict__ out, int* err) {
+__global__ void __launch_bounds__(kSortWarps * 32)
+    lookup_sort_kernel(Tokens tk, Order o, int64_t units, Parts pt, const typename B::T* __restrict__ w, int64_t ld,
+                       bool whole, float scale, int H, typename B::T* __restrict__ out, int* err) {
   extern __shared__ uint32_t sm[];
   if ((int)blockIdx.x < o.ctas) {
     sort_tokens(tk, o, sm);
     return;
   }
-  const int warps = (gridDim.x - o.ctas) * sorted::kWarps;
-  for (int i = (blockIdx.x - o.ctas) * sorted::kWarps + (threadIdx.x >> 5); i < o.n; i += warps)
-    look_up<B>(tk, i, w, ld, whole, scale, H, out, err);
+  const int64_t warps = (int64_t)(gridDim.x - o.ctas) * kSortWarps;
+  for (int64_t u = (int64_t)(blockIdx.x - o.ctas) * kSortWarps + (threadIdx.x >> 5); u < units; u += warps)
+    look_up<B>(tk, u, pt, w, ld, whole, scale, H, out, err);
 }
 
 // ------------------------------------------------------------------ sums of runs
@@ -182,8 +192,7 @@ __device__ __forceinline__ void write_row(const Target& to, uint32_t row, int i,
 // one that starts here.  The CTAs behind clear the rows of a dense gradient that no token names.
 //
 // Loads run ahead of the sums by U pairs, those of main's rows too (kMain): a run is one or two pairs long as a rule,
-// and what a row's sum is added to would else be waited for at every run.  (Reductions at L2 in its place, 8192 x 2560:
-// 43 us, bound by their rate, against 34 us of waiting.)
+// and what a row's sum is added to would else be waited for at every run.
 constexpr int kRunThreads = 192;  // at most
 template <class B, int L, bool kMain>
 __global__ void __launch_bounds__(kRunThreads)
@@ -191,6 +200,7 @@ __global__ void __launch_bounds__(kRunThreads)
                int n, uint32_t R, const typename B::T* __restrict__ g, int64_t ldg, int H, int chunks, int slices,
                Target to, float* __restrict__ parts) {
   static_assert(L <= 32, "a warp looks at a chunk");
+  pdl_launch_dependents();  // join_kernel may look for its runs; it waits for this kernel's end before it reads parts
   const int lane = threadIdx.x & 31, lanes = B::lanes(H);
   if ((int)blockIdx.x >= chunks * slices) {
     const int warp = (blockIdx.x - chunks * slices) * (blockDim.x / 32) + (threadIdx.x >> 5);
@@ -203,14 +213,14 @@ __global__ void __launch_bounds__(kRunThreads)
     }
     return;
   }
-  __shared__ uint32_t sk[3 * L + 2], sp[2 * L];
+  __shared__ uint32_t sk[3 * L + 2];
+  __shared__ int2 pair[2 * L];  // {position, row of the table | what follows << 30} of this CTA's pairs
   const int chunk = blockIdx.x / slices, i = (blockIdx.x - chunk * slices) * blockDim.x + threadIdx.x;
   const int lo = chunk * L, hi = min(n, lo + L);
   for (int t = threadIdx.x; t < 3 * L + 2; t += blockDim.x) {
     const int at = lo - L - 1 + t;
     sk[t] = at >= 0 && at < n ? key[at] : kNoKey;
   }
-  for (int t = threadIdx.x; t < 2 * L; t += blockDim.x) sp[t] = lo + t < n ? pos[lo + t] : 0;
   __syncthreads();
   auto K = [&](int at) { return sk[at - (lo - L - 1)]; };
 
@@ -230,39 +240,40 @@ __global__ void __launch_bounds__(kRunThreads)
     const bool here = !(from_far && k1 == k0) && beg < hi;  // the run starts in this chunk
     if (here && K(stop) != k1) end = stop;                  // (stop <= hi + L) and ends in the next
   }
-  if (i >= lanes) return;
-  float* part = parts + 2 * (int64_t)chunk * H;
-  // what becomes of the sum behind pair `at`: it goes on, is a part from the left or to the right, or a row
+  // what becomes of the sum behind a pair: it goes on, is a part from the left or to the right, or a row
   enum { kOn, kLeft, kRight, kRow };
-  auto then = [&](int at) {
+  for (int t = threadIdx.x; t < end - beg; t += blockDim.x) {
+    const int at = beg + t;
     const uint32_t k = K(at);
     const bool more = K(at + 1) == k;
-    if (more && at + 1 < end) return kOn;
-    return from_far && k == k0 ? kLeft : more ? kRight : kRow;
-  };
+    const uint32_t what = more && at + 1 < end ? kOn : from_far && k == k0 ? kLeft : more ? kRight : kRow;
+    pair[t] = k < R ? make_int2((int)pos[at], (int)(k | what << 30)) : make_int2(-1, 0);
+  }
+  __syncthreads();
+  if (i >= lanes) return;
+  float* part = parts + 2 * (int64_t)chunk * H;
   float acc[B::V] = {};
   constexpr int U = kMain ? 4 : 8;
-  for (int s = beg; s < end; s += U) {
+  for (int s = 0; s < end - beg; s += U) {
     B b[U];
     float m[kMain ? U : 1][B::V];
+    int2 p[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (s + u >= end || K(s + u) >= R) break;
-      b[u].load_once(g + (int64_t)sp[s + u - lo] * ldg, i, H);
+      p[u] = s + u < end - beg ? pair[s + u] : make_int2(-1, 0);
+      if (p[u].x >= 0) b[u].load_once(g + p[u].x * ldg, i, H);
       if constexpr (kMain) {
-        if (then(s + u) == kRow) B::get_f(to.main + (int64_t)K(s + u) * H, i, H, m[u]);
+        if ((uint32_t)p[u].y >> 30 == kRow) B::get_f(to.main + (int64_t)(p[u].y & 0x3fffffff) * H, i, H, m[u]);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (s + u >= end) break;
-      const uint32_t k = K(s + u);
-      if (k >= R) return;  // tokens outside the table, behind all others
+      if (p[u].x < 0) return;  // the end, or tokens outside the table, behind all others
       float v[B::V];
       b[u].get(v);
 #pragma unroll
       for (int q = 0; q < B::V; ++q) acc[q] += v[q];
-      const int what = then(s + u);
+      const uint32_t what = (uint32_t)p[u].y >> 30, k = p[u].y & 0x3fffffff;
       if (what == kOn) continue;
       if (what == kRow) {
         if constexpr (kMain) {
@@ -281,39 +292,70 @@ __global__ void __launch_bounds__(kRunThreads)
   }
 }
 
-// Joins the shared runs.  A CTA looks at 32 chunks (a lane each) for runs that start there and go on through the whole
-// next chunk, and sums their parts for a slice of the row.
+// Joins the shared runs.  A CTA looks at eight chunks for runs that start there and go on through the whole next chunk,
+// by the order alone and so ahead of run_kernel's end, and sums their parts for 32 lanes of the row: warp w those of
+// chunks w, w + 8, ... behind the first, and the warps' sums in their order.
+constexpr int kJoinChunks = 8, kJoinWarps = 8;
 template <class B, int L>
-__global__ void __launch_bounds__(kRunThreads)
+__global__ void __launch_bounds__(kJoinWarps * 32)
     join_kernel(const uint32_t* __restrict__ key, int n, uint32_t R, int H, int slices, Target to,
                 const float* __restrict__ parts) {
-  pdl_wait();
-  const int block = blockIdx.x / slices, i = (blockIdx.x - block * slices) * blockDim.x + threadIdx.x;
-  const int lane = threadIdx.x & 31;
-  const int64_t lo = (int64_t)(block * 32 + lane) * L, hi = lo + L;
+  __shared__ float sums[kJoinWarps][B::V][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int block = blockIdx.x / slices, i = (blockIdx.x - block * slices) * 32 + lane;
+  const int64_t lo = (int64_t)(block * kJoinChunks + lane) * L, hi = lo + L;
   uint32_t k = kNoKey;
   bool starts = false;
-  if (hi + L < n) {
+  if (lane < kJoinChunks && hi + L < n) {
     k = key[hi - 1];
-    starts = k < R && key[hi + L] == k && (lo == 0 || key[lo - 1] != k);
+    const uint32_t far = key[hi + L], before = lo ? key[lo - 1] : kNoKey;
+    starts = k < R && far == k && before != k;
   }
   uint32_t todo = __ballot_sync(0xffffffffu, starts);
-  if (i >= B::lanes(H)) return;
-  while (todo) {
-    const int at = __ffs(todo) - 1, chunk = block * 32 + at;
-    todo &= todo - 1;
-    const uint32_t kr = key[(int64_t)(chunk + 1) * L - 1];
-    int a = (chunk + 2) * L, b = n;  // the first pair behind the run
+  if (todo == 0) {
+    pdl_wait();
+    return;
+  }
+  int last = 0;  // of the run that starts in this lane's chunk
+  for (uint32_t left = todo; left; left &= left - 1) {
+    const int j = __ffs(left) - 1;
+    const uint32_t kj = __shfl_sync(0xffffffffu, k, j);
+    // the first pair behind the run lies in [a, b]; the lanes look at 32 places between them at a time
+    int a = (block * kJoinChunks + j + 2) * L, b = n;
     while (a < b) {
-      const int mid = a + (b - a) / 2;
-      if (key[mid] > kr) b = mid; else a = mid + 1;
+      const int at = a + (int)((int64_t)(b - a) * lane / 32);
+      const uint32_t same = __ballot_sync(0xffffffffu, key[at] <= kj);
+      if (same == 0) break;  // a itself
+      const int top = 31 - __clz(same), from = a;
+      a = from + (int)((int64_t)(b - from) * top / 32) + 1;
+      if (top < 31) b = from + (int)((int64_t)(b - from) * (top + 1) / 32);
     }
-    const int last = (a - 1) / L;
+    if (lane == j) last = (a - 1) / L;
+  }
+  pdl_wait();
+  const bool here = i < B::lanes(H);
+  for (; todo; todo &= todo - 1) {
+    const int j = __ffs(todo) - 1, chunk = block * kJoinChunks + j;
+    const int end = __shfl_sync(0xffffffffu, last, j);
     float acc[B::V] = {};
-    B::sum_f(parts + (2 * (int64_t)chunk + 1) * H, i, H, acc);
+    if (here) {
 #pragma unroll 8
-    for (int j = chunk + 1; j <= last; ++j) B::sum_f(parts + 2 * (int64_t)j * H, i, H, acc);
-    write_row<B>(to, kr, i, H, acc);
+      for (int c = chunk + warp; c <= end; c += kJoinWarps)
+        B::sum_f(parts + (2 * (int64_t)c + (c == chunk ? 1 : 0)) * H, i, H, acc);
+    }
+#pragma unroll
+    for (int q = 0; q < B::V; ++q) sums[warp][q][lane] = acc[q];
+    __syncthreads();
+    const uint32_t kj = __shfl_sync(0xffffffffu, k, j);
+    if (warp == 0 && here) {
+#pragma unroll
+      for (int w = 1; w < kJoinWarps; ++w) {
+#pragma unroll
+        for (int q = 0; q < B::V; ++q) acc[q] += sums[w][q][lane];
+      }
+      write_row<B>(to, kj, i, H, acc);
+    }
+    __syncthreads();
   }
 }
 
@@ -348,9 +390,11 @@ std::vector<torch::Tensor> embedding_fwd(torch::Tensor tokens, torch::Tensor w, 
     using T = typename B::T;
     const T* table = (const T*)w.data_ptr();
     T* to = (T*)out.data_ptr();
+    const Parts pt = parts_of<B>((int)H);
+    const int64_t units = n * pt.parts;
     if (!want_order) {
-      launch_rows(lookup_kernel<B>, (n + kLookWarps - 1) / kLookWarps, kLookWarps * 32, 0, 1, false, st, tk, (int)n, table,
-                  w.stride(0), whole, (float)scale, (int)H, to, err.data_ptr<int>());
+      launch_rows(lookup_kernel<B>, (units + kLookWarps - 1) / kLookWarps, kLookWarps * 32, 0, 1, false, st, tk, units, pt,
+                  table, w.stride(0), whole, (float)scale, (int)H, to, err.data_ptr<int>());
       return;
     }
     int total = 1;
@@ -364,10 +408,10 @@ std::vector<torch::Tensor> embedding_fwd(torch::Tensor tokens, torch::Tensor w, 
     o.pos = o.key + n;
     o.scratch = o.key + 2 * n;
     o.seen = o.key + 4 * n;
-    const int64_t look = std::min<int64_t>((n + sorted::kWarps - 1) / sorted::kWarps, 148 - o.ctas);
-    launch_rows(lookup_sort_kernel<B>, o.ctas * (1 + (look + o.ctas - 1) / o.ctas), sorted::kThreads,
-                sorted::pass_smem(1 << o.bits), o.ctas, false, st, tk, o, table, w.stride(0), whole, (float)scale, (int)H,
-                to, err.data_ptr<int>());
+    const int64_t look = std::min<int64_t>((units + kSortWarps - 1) / kSortWarps, 148 * 4);
+    launch_rows(lookup_sort_kernel<B>, o.ctas * (1 + (look + o.ctas - 1) / o.ctas), kSortWarps * 32,
+                sorted::pass_smem(kSortWarps, 1 << o.bits), o.ctas, false, st, tk, o, units, pt, table, w.stride(0), whole,
+                (float)scale, (int)H, to, err.data_ptr<int>());
   });
   return {out, order};
 }
@@ -402,27 +446,35 @@ torch::Tensor embedding_bwd(torch::Tensor order, torch::Tensor g, torch::Tensor 
   const bool wide = row_vectors(g) && (main.has_value() ? reinterpret_cast<uintptr_t>(to.main) % 16 == 0
                                                          : row_vectors(out));
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  by_lanes(w, wide, [&](auto lanes_type) {
+  auto sums = [&](auto lanes_type, auto to_main) {
     using B = decltype(lanes_type);
     using T = typename B::T;
+    constexpr bool kMain = decltype(to_main)::value;
     auto go = [&](auto len) {
       constexpr int L = decltype(len)::value;
       const int64_t chunks = (n + L - 1) / L;
       const int lanes = B::lanes((int)H), slices = (lanes + kRunThreads - 1) / kRunThreads;
       const int threads = ((lanes + slices - 1) / slices + 31) / 32 * 32;
       auto parts = torch::empty({chunks, 2, H}, w.options().dtype(at::kFloat));
-      const int64_t clear = main.has_value() ? 0 : std::min<int64_t>((R + 3) / 4, 148 * 8);
+      const int64_t clear = kMain ? 0 : std::min<int64_t>((R + 3) / 4, 148 * 8);
       LIBRA_CHECK(chunks * slices + clear < (1ll << 31), "embedding: too many tokens");
-      launch_rows(main.has_value() ? run_kernel<B, L, true> : run_kernel<B, L, false>, chunks * slices + clear, threads, 0, 1, false, st, key, pos, seen, (int)n,
+      launch_rows(run_kernel<B, L, kMain>, chunks * slices + clear, threads, 0, 1, false, st, key, pos, seen, (int)n,
                   (uint32_t)R, (const T*)g.data_ptr(), g.stride(0), (int)H, (int)chunks, slices, to,
                   parts.data_ptr<float>());
-      launch_rows(join_kernel<B, L>, (chunks + 31) / 32 * slices, threads, 0, 1, true, st, key, (int)n, (uint32_t)R,
-                  (int)H, slices, to, (const float*)parts.data_ptr<float>());
+      const int wide32 = (lanes + 31) / 32;
+      launch_rows(join_kernel<B, L>, (chunks + kJoinChunks - 1) / kJoinChunks * wide32, kJoinWarps * 32, 0, 1, true, st,
+                  key, (int)n, (uint32_t)R, (int)H, wide32, to, (const float*)parts.data_ptr<float>());
     };
     if (n <= 16384)
       go(std::integral_constant<int, 16>());
     else
       go(std::integral_constant<int, 32>());
+  };
+  by_lanes(w, wide, [&](auto b) {
+    if (main.has_value())
+      sums(b, std::true_type());
+    else
+      sums(b, std::false_type());
   });
   return out;
 }

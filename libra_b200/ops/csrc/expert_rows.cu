@@ -250,15 +250,16 @@ struct PlanItems {
 
 // CTAs of the cluster: as many as leave a warp the eight items a lane that it keeps in registers (131072 pairs of 128
 // experts: 26 us with 8 CTAs that load them twice).
+constexpr int kPlanWarps = 32;
 static int plan_ctas(int64_t n) {
   int ctas = 1;
-  while (ctas < sorted::kMaxCtas && ctas * 32 * 32 * sorted::kBatch < n) ctas *= 2;
+  while (ctas < sorted::kMaxCtas && ctas * kPlanWarps * 32 * sorted::kBatch < n) ctas *= 2;
   return ctas;
 }
 
-__global__ void __launch_bounds__(sorted::kThreads) plan_kernel(int n, int ctas, PlanItems items) {
+__global__ void __launch_bounds__(kPlanWarps * 32) plan_kernel(int n, int ctas, PlanItems items) {
   extern __shared__ uint32_t sm[];
-  sorted::counting_pass(n, items.E, items.align, sm, ctas, items);
+  sorted::counting_pass<kPlanWarps>(n, items.E, items.align, sm, ctas, items);
 }
 
 // experts [T, k] -> rows int32 [T * k], offs int32 [E + 1], counts int32 [E], and the layout's capacity
@@ -281,7 +282,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, int64_t> expert_plan(tor
   const int ctas = plan_ctas(n);
   PlanItems it{ids.data_ptr(), ids.scalar_type() == at::kLong, rows_t.data_ptr<int>(), offs.data_ptr<int>(),
                counts.data_ptr<int>(), (int)E, (uint32_t)align, err.data_ptr<int>()};
-  launch_rows(plan_kernel, ctas, sorted::kThreads, sorted::pass_smem((int)E), ctas, false,
+  launch_rows(plan_kernel, ctas, kPlanWarps * 32, sorted::pass_smem(kPlanWarps, (int)E), ctas, false,
               at::cuda::getCurrentCUDAStream(), (int)n, ctas, it);
   return {rows_t, offs, counts, cap};
 }

@@ -11,21 +11,22 @@
 namespace libra {
 namespace sorted {
 
-constexpr int kThreads = 1024, kWarps = 32, kMaxBins = 1024, kMaxCtas = 16;
+constexpr int kMaxBins = 1024, kMaxCtas = 16;
 
 // Bins up to which a warp's lanes find their equals through words in shared memory: each sets its bit in its bin's word.
 // (8192 items, 512 bins: about 1 us for a CTA, with __match_any_sync 8.6 us, which takes a step for every distinct key.)
 constexpr int kWordBins = 512;
 
-inline size_t pass_smem(int bins) {
-  return ((size_t)kWarps * bins * (bins <= kWordBins ? 2 : 1) + bins + 64) * 4;
+inline size_t pass_smem(int warps, int bins) {
+  return ((size_t)warps * bins * (bins <= kWordBins ? 2 : 1) + bins + 64) * 4;
 }
 
 __device__ __forceinline__ uint32_t ld_cluster_u32(const uint32_t* p, uint32_t rank) {
   return (uint32_t)vocab::ld_cluster(reinterpret_cast<const int*>(p), rank);
 }
 
-// Exclusive sum over the block's 1024 threads.
+// Exclusive sum over the block's threads.
+template <int kWarps>
 __device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t* tmp) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t s = v;
@@ -36,20 +37,17 @@ __device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t* tmp) {
   }
   if (lane == 31) tmp[warp] = s;
   __syncthreads();
-  if (warp == 0) {
-    uint32_t t = tmp[lane];
+  uint32_t t = lane < kWarps ? tmp[lane] : 0;
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const uint32_t o = __shfl_up_sync(0xffffffffu, t, off);
-      if (lane >= off) t += o;
-    }
-    tmp[lane] = t;
+  for (int off = 1; off < kWarps; off <<= 1) {
+    const uint32_t o = __shfl_up_sync(0xffffffffu, t, off);
+    if (lane >= off) t += o;
   }
-  __syncthreads();
-  return s - v + (warp ? tmp[warp - 1] : 0);
+  t = __shfl_sync(0xffffffffu, t, warp ? warp - 1 : 0);
+  return s - v + (warp ? t : 0);
 }
 
-// Up to this many items a warp stay in registers between the two walks.
+// Up to this many items a lane stay in registers between the two walks.
 constexpr int kBatch = 8;
 
 // One pass.  Items has
@@ -57,11 +55,12 @@ constexpr int kBatch = 8;
 //   int bin(const Item&)        its bin, or -1 for an item that gets no place
 //   void put(int i, Item, uint32_t place)   (place 0xffffffff for none)
 //   void group(int bin, uint32_t start, uint32_t count)   once for each bin; starts are multiples of `align`
-// Every CTA of the cluster (of `ctas`, at most 16) calls it with all its threads; sm: pass_smem(bins) bytes.  What put
-// writes to global memory is visible to the whole cluster afterwards.
-template <class Items>
+// Every CTA of the cluster (of `ctas`, at most 16) calls it with all its kWarps warps; sm: pass_smem(kWarps, bins) bytes.
+// What put writes to global memory is visible to the whole cluster afterwards.
+template <int kWarps, class Items>
 __device__ __forceinline__ void counting_pass(int n, int bins, uint32_t align, uint32_t* sm, int ctas, Items& items) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = threadIdx.x;
+  constexpr int kThreads = kWarps * 32, kMine = kMaxBins / kThreads;  // bins a thread
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = ctas > 1 ? (int)cluster_ctarank() : 0;
   uint32_t* total = sm + kWarps * bins;
   uint32_t* tmp = total + bins;
@@ -96,37 +95,48 @@ __device__ __forceinline__ void counting_pass(int n, int bins, uint32_t align, u
   }
   __syncthreads();
 
-  uint32_t sum = 0;
-  if (b < bins) {
+  // this thread's bins: m neighbours from b0
+  const int m = (bins + kThreads - 1) / kThreads, b0 = threadIdx.x * m;
+  uint32_t all[kMine], below[kMine], room = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum += sm[w * bins + b];
-    total[b] = sum;
+  for (int q = 0; q < kMine; ++q) {
+    all[q] = below[q] = 0;
+    if (q >= m || b0 + q >= bins) continue;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) all[q] += sm[w * bins + b0 + q];
+    total[b0 + q] = all[q];
   }
-  uint32_t all = sum, below = 0;
   if (ctas > 1) {
     vocab::cluster_meet();
-    if (b < bins) {
-      uint32_t v[16];
 #pragma unroll
-      for (int c = 0; c < 16; ++c) v[c] = c < ctas ? ld_cluster_u32(total + b, c) : 0u;
-      all = 0;
+    for (int q = 0; q < kMine; ++q) {
+      if (q >= m || b0 + q >= bins) continue;
+      uint32_t v[kMaxCtas];
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        all += v[c];
-        below += c < rank ? v[c] : 0u;
+      for (int c = 0; c < kMaxCtas; ++c) v[c] = c < ctas ? ld_cluster_u32(total + b0 + q, c) : 0u;
+      all[q] = 0;
+#pragma unroll
+      for (int c = 0; c < kMaxCtas; ++c) {
+        all[q] += v[c];
+        below[q] += c < rank ? v[c] : 0u;
       }
     }
   } else {
     __syncthreads();
   }
-  const uint32_t start = block_before(b < bins ? (all + align - 1) / align * align : 0, tmp);
-  if (b < bins) {
-    if (rank == 0) items.group(b, start, all);
-    uint32_t at = start + below;
+#pragma unroll
+  for (int q = 0; q < kMine; ++q) room += (all[q] + align - 1) / align * align;
+  uint32_t start = block_before<kWarps>(room, tmp);
+#pragma unroll
+  for (int q = 0; q < kMine; ++q) {
+    if (q >= m || b0 + q >= bins) continue;
+    if (rank == 0) items.group(b0 + q, start, all[q]);
+    uint32_t at = start + below[q];
+    start += (all[q] + align - 1) / align * align;
 #pragma unroll 8
     for (int w = 0; w < kWarps; ++w) {
-      const uint32_t c = sm[w * bins + b];
-      sm[w * bins + b] = at;
+      const uint32_t c = sm[w * bins + b0 + q];
+      sm[w * bins + b0 + q] = at;
       at += c;
     }
   }
