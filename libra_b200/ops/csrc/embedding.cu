@@ -187,12 +187,15 @@ __device__ __forceinline__ void write_row(const Target& to, uint32_t row, int i,
   }
 }
 
-// A chunk has L pairs, the last one fewer; chunk c of the grid's first `chunks * slices` CTAs, slice by slice of the
-// rows.  parts holds two fp32 rows a chunk: its part of a shared run that came in from the left, and of
-// one that starts here.  The CTAs behind clear the rows of a dense gradient that no token names.
+// A chunk has L pairs, the last one fewer; the grid's first `chunks * slices` CTAs take one each, for a slice of the rows'
+// lanes.  parts holds two fp32 rows a chunk: its part of a shared run that came in from the left, and of one that starts
+// here.  The CTAs behind clear the rows of a dense gradient that no token names.
 //
 // Loads run ahead of the sums by U pairs, those of main's rows too (kMain): a run is one or two pairs long as a rule,
-// and what a row's sum is added to would else be waited for at every run.
+// and what a row's sum is added to would else be waited for at every run.  Bound by DRAM: 8192 text-like tokens x 2560
+// into main take 40 us with the join (178 MB, 0.68 of the copy rate), into a dense gradient of 151936 rows 136 us (0.92).
+// Tried without gain: reductions at L2 instead of loads and stores of main (43 us for this kernel against 33), pairs
+// copied ahead into shared memory (50), four elements a lane (34), chunks of 8 and 32 (32 and 37).
 constexpr int kRunThreads = 192;  // at most
 template <class B, int L, bool kMain>
 __global__ void __launch_bounds__(kRunThreads)
@@ -455,15 +458,18 @@ torch::Tensor embedding_bwd(torch::Tensor order, torch::Tensor g, torch::Tensor 
       const int64_t chunks = (n + L - 1) / L;
       const int lanes = B::lanes((int)H), slices = (lanes + kRunThreads - 1) / kRunThreads;
       const int threads = ((lanes + slices - 1) / slices + 31) / 32 * 32;
-      auto parts = torch::empty({chunks, 2, H}, w.options().dtype(at::kFloat));
+      const bool shared = n > 2 * L;  // a run can only then go on through a whole chunk
+      torch::Tensor parts;
+      if (shared) parts = torch::empty({chunks, 2, H}, w.options().dtype(at::kFloat));
+      float* const part = shared ? parts.data_ptr<float>() : nullptr;
       const int64_t clear = kMain ? 0 : std::min<int64_t>((R + 3) / 4, 148 * 8);
       LIBRA_CHECK(chunks * slices + clear < (1ll << 31), "embedding: too many tokens");
       launch_rows(run_kernel<B, L, kMain>, chunks * slices + clear, threads, 0, 1, false, st, key, pos, seen, (int)n,
-                  (uint32_t)R, (const T*)g.data_ptr(), g.stride(0), (int)H, (int)chunks, slices, to,
-                  parts.data_ptr<float>());
+                  (uint32_t)R, (const T*)g.data_ptr(), g.stride(0), (int)H, (int)chunks, slices, to, part);
+      if (!shared) return;
       const int wide32 = (lanes + 31) / 32;
       launch_rows(join_kernel<B, L>, (chunks + kJoinChunks - 1) / kJoinChunks * wide32, kJoinWarps * 32, 0, 1, true, st,
-                  key, (int)n, (uint32_t)R, (int)H, wide32, to, (const float*)parts.data_ptr<float>());
+                  key, (int)n, (uint32_t)R, (int)H, wide32, to, (const float*)part);
     };
     if (n <= 16384)
       go(std::integral_constant<int, 16>());

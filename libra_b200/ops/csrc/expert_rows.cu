@@ -169,26 +169,27 @@ static std::vector<torch::Tensor> route_fwd(const torch::Tensor& z, int64_t k, b
   return {w, ids, stats};
 }
 
-static torch::Tensor route_bwd(const torch::Tensor& z, const torch::Tensor& w, const torch::Tensor& ids,
-                               const torch::Tensor& stats, const torch::Tensor& g) {
-  const int64_t N = z.size(0), E = z.size(1), k = w.size(1);
-  const c10::cuda::CUDAGuard guard(z.device());
-  auto dz = torch::empty({N, E}, z.options());
+// z: the logits where the weights were not renormalised (stats is then defined); else only E and their type are needed.
+static torch::Tensor route_bwd(const torch::Tensor& z, int64_t E, at::ScalarType type, const torch::Tensor& w,
+                               const torch::Tensor& ids, const torch::Tensor& stats, const torch::Tensor& g) {
+  const int64_t N = w.size(0), k = w.size(1);
+  const c10::cuda::CUDAGuard guard(w.device());
+  auto dz = torch::empty({N, E}, w.options().dtype(type));
   if (N == 0) return dz;
-  cudaStream_t st = at::cuda::getCurrentCUDAStream();
   by_width((int)E, [&](auto v) {
     auto go = [&](auto* p) {
-      using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+      using T = std::remove_pointer_t<decltype(p)>;
       launch_rows(route_bwd_kernel<T, decltype(v)::value>, (N + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32, 0, 1,
-                  false, st, p, z.stride(0), (int)N, (int)E, (int)k, (const float*)w.data_ptr<float>(),
+                  false, at::cuda::getCurrentCUDAStream(), z.defined() ? (const T*)z.data_ptr() : (const T*)nullptr,
+                  z.defined() ? z.stride(0) : 0, (int)N, (int)E, (int)k, (const float*)w.data_ptr<float>(),
                   (const int64_t*)ids.data_ptr<int64_t>(),
                   stats.defined() ? (const float2*)stats.data_ptr<float>() : (const float2*)nullptr,
                   (const float*)g.data_ptr<float>(), (T*)dz.data_ptr());
     };
-    if (z.scalar_type() == at::kFloat)
-      go((const float*)z.data_ptr());
+    if (type == at::kFloat)
+      go((float*)nullptr);
     else
-      go((const __nv_bfloat16*)z.data_ptr());
+      go((__nv_bfloat16*)nullptr);
   });
   return dz;
 }
@@ -197,7 +198,9 @@ struct RouteTopk : public torch::autograd::Function<RouteTopk> {
   using List = torch::autograd::variable_list;
   static List forward(torch::autograd::AutogradContext* ctx, torch::Tensor z, int64_t k, bool normalize) {
     auto r = route_fwd(z, k, normalize, !normalize);
-    ctx->save_for_backward({z, r[0], r[1], r[2]});
+    ctx->save_for_backward({normalize ? torch::Tensor() : z, r[0], r[1], r[2]});
+    ctx->saved_data["E"] = z.size(1);
+    ctx->saved_data["type"] = (int64_t)z.scalar_type();
     ctx->mark_non_differentiable({r[1]});
     ctx->set_materialize_grads(false);
     return {r[0], r[1]};
@@ -207,7 +210,8 @@ struct RouteTopk : public torch::autograd::Function<RouteTopk> {
     List out(3);
     if (!up[0].defined()) return out;
     const auto s = ctx->get_saved_variables();
-    out[0] = route_bwd(s[0], s[1], s[2], s[3], up[0].contiguous());
+    out[0] = route_bwd(s[0], ctx->saved_data["E"].toInt(), (at::ScalarType)ctx->saved_data["type"].toInt(), s[1], s[2],
+                       s[3], up[0].contiguous());
     return out;
   }
 };

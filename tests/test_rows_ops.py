@@ -169,6 +169,60 @@ def test_embedding_gradient_of_strided_and_expanded_rows_is_the_same_every_time(
     _check("cuda")
 
 
+def _grad64(tokens, g, rows):
+    """As oracle.embedding_grad, without a loop."""
+    g = g.double()
+    total = torch.zeros(rows, g.shape[1], dtype=torch.float64).index_add_(0, tokens, g)
+    size = torch.zeros_like(total).index_add_(0, tokens, g.abs())
+    return total, size, torch.bincount(tokens, minlength=rows).double().unsqueeze(1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [15, 16, 17, 31, 32, 33, 47, 48, 49, 64, 65, 1024, 1025, 8192, 16384, 16385, 40000])
+@pytest.mark.parametrize("run", [1, 2, 15, 16, 17, 32, 33, 64, 65, 97, 1000])
+def test_embedding_gradient_of_runs_that_end_anywhere(n, run):
+    """Every token occurs `run` times (the last one less often), shuffled: sums that lie in one chunk of the sorted
+    tokens, in two, or in many, with borders at every offset."""
+    gen = _gen(n + run)
+    tokens = (torch.arange(n) // run + 3)[torch.randperm(n, generator=gen)]
+    rows = int(tokens.max()) + 5
+    for H, dtype in ((40, torch.bfloat16), (12, torch.float32), (7, torch.float32)):
+        w = torch.zeros(rows, H, dtype=dtype, device="cuda", requires_grad=True)
+        g = torch.randn(n, H, generator=gen).to(dtype)
+        total, size, many = _grad64(tokens, g, rows)
+        for main in (None, torch.randn(rows, H, generator=gen)):
+            w.main_grad = None if main is None else main.clone().cuda()
+            out = ops.embedding(tokens.cuda(), w)
+            w.grad = None
+            out.backward(g.cuda())
+            if main is None:
+                _close(w.grad, total, size * many * U * 1.01 + total.abs() * _half(dtype) * 1.01)
+            else:
+                assert w.grad is None
+                _close(w.main_grad, main.double() + total, (size * (many + 1) + main.abs().double()) * U * 1.01)
+    _check("cuda")
+
+
+@pytest.mark.gpu
+def test_embedding_looked_up_twice_and_backward_twice():
+    gen = _gen(5)
+    a, b = torch.randint(0, 30, (100,), generator=gen), torch.randint(0, 30, (70,), generator=gen)
+    ga, gb = torch.randn(100, 16, generator=gen), torch.randn(70, 16, generator=gen)
+    w = torch.randn(30, 16, generator=gen).cuda().requires_grad_(True)
+    total, size, many = _grad64(torch.cat([a, b]), torch.cat([ga, gb]), 30)
+    for main in (False, True):
+        w.grad = None
+        w.main_grad = torch.zeros(30, 16, device="cuda") if main else None
+        outs = [ops.embedding(a.cuda(), w), ops.embedding(b.cuda(), w)]
+        for times in (1, 2):
+            torch.autograd.backward(outs, [ga.cuda(), gb.cuda()], retain_graph=True)
+            _close(w.main_grad if main else w.grad, times * total, times * size * (many + 2) * U * 1.01)
+    with torch.no_grad():
+        w.add_(1.0)  # an optimizer step between the passes: the gradient does not need the table's values
+    torch.autograd.backward(outs, [ga.cuda(), gb.cuda()])
+    _close(w.main_grad, 3 * total, 3 * size * (many + 2) * U * 1.01)
+
+
 # ------------------------------------------------------------------ router
 
 def _logits(n, E, gen, dtype):
@@ -408,6 +462,26 @@ def test_plan_reports_ids_beyond_the_experts():
     _check("cuda")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k,E,align", [(16384, 8, 128, 128), (8193, 1, 512, 128), (40000, 8, 513, 16),
+                                         (20000, 4, 1024, 1), (100001, 3, 1, 128), (1, 8, 1024, 128), (5000, 7, 37, 3)])
+def test_plan_of_many_pairs(n, k, E, align):
+    gen = _gen(n + E)
+    ids = (torch.rand(n, k, generator=gen).pow(2) * E).long()
+    ids[torch.rand(n, k, generator=gen) < 0.01] = -1
+    flat = ids.reshape(-1)
+    counts = torch.bincount(flat[flat >= 0], minlength=E)
+    padded = (counts + align - 1) // align * align
+    start = padded.cumsum(0) - padded
+    order = torch.argsort(torch.where(flat >= 0, flat, E), stable=True)[:int(counts.sum())]
+    rows = torch.full_like(flat, -1)
+    rows[order] = torch.arange(order.numel()) - (counts.cumsum(0) - counts)[flat[order]] + start[flat[order]]
+    plan = ops.expert_plan(ids.cuda(), E, align=align)
+    assert torch.equal(plan.rows.cpu().long(), rows) and torch.equal(plan.counts.cpu().long(), counts)
+    assert torch.equal(plan.offs.cpu().long(), torch.cat([start, padded.sum()[None] if E else start]))
+    _check("cuda")
+
+
 # ------------------------------------------------------------------ together
 
 def _block(h, logits, res, plan_of):
@@ -511,4 +585,30 @@ def test_training_block_in_a_captured_graph():
     torch.cuda.synchronize()
     for a, b in zip(list(got) + [main], want):
         assert torch.equal(a, b)
+    _check("cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 33, 300])
+def test_moe_block_gradients_match_the_loop(T):
+    """The model's block on the row operators against its per-expert loop: outputs and the gradients of tokens, router
+    and experts, to a few bf16 roundings (relative, in norm)."""
+    from libra_b200.models.moe import moe_mlp, moe_mlp_looped
+    from libra_b200.models.qwen3 import get_config
+
+    cfg = get_config("tiny-moe")
+    gen = _gen(T)
+    H, E, F = cfg.hidden_size, cfg.num_experts, cfg.moe_intermediate_size
+    data = [torch.randn(T, H, generator=gen).bfloat16(), torch.randn(T, H, generator=gen).bfloat16(),
+            torch.randn(E, H, generator=gen) * 0.05, (torch.randn(E, 2 * F, H, generator=gen) * 0.05).bfloat16(),
+            (torch.randn(E, H, F, generator=gen) * 0.05).bfloat16()]
+    g = torch.randn(T, H, generator=gen).bfloat16().cuda()
+    got = []
+    for block in (moe_mlp, moe_mlp_looped):
+        leaves = [t.cuda().requires_grad_(True) for t in data]
+        out = block(*leaves, cfg)
+        got.append([out.detach()] + list(torch.autograd.grad(out, leaves, g)))
+    for a, b in zip(*got):
+        # gate, up, their product, the expert's output, dy, dgu and dx each round once to bf16 on either side
+        assert float((a.double() - b.double()).norm()) <= 2 * 7 * _half(torch.bfloat16) * float(b.double().norm())
     _check("cuda")
