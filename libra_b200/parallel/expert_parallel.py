@@ -102,11 +102,14 @@ class RoutePlan:
     k: int
 
 
-def route_plan(experts: torch.Tensor, counts_all: torch.Tensor, me: int, align: int = 128) -> RoutePlan:
+def route_plan(experts: torch.Tensor, counts_all: torch.Tensor, me: int, align: int = 128,
+               own: Optional[ops.ExpertPlan] = None) -> RoutePlan:
     """Destination of every assignment, from all ranks' per-expert counts.
 
     ``experts`` [T, k] global expert ids of this rank's tokens; ``counts_all``
-    [n, E] the number of assignments each rank sends to each expert.  The
+    [n, E] the number of assignments each rank sends to each expert; ``own``
+    the ids sorted without padding (``ops.expert_plan`` with ``align=1``;
+    computed if absent).  The
     receive slot of rank d holds one group per local expert, each starting at a
     multiple of ``align`` rows (so the expert GEMM runs as one grouped launch
     over tile-aligned groups), ordered inside by (source rank, source order):
@@ -119,20 +122,16 @@ def route_plan(experts: torch.Tensor, counts_all: torch.Tensor, me: int, align: 
     E_l = E // n
     T, k = experts.shape
     flat = experts.reshape(-1)
-    order = torch.argsort(flat, stable=True)
-    g = flat[order]
+    if own is None:
+        own = ops.expert_plan(experts, E, align=1)
     cnt = counts_all.to(torch.int64)
     per_dest = cnt.sum(0).view(n, E_l)
     padded = (per_dest + align - 1) // align * align
     base = (padded.cumsum(1) - padded).reshape(-1)
     lower = (cnt.cumsum(0) - cnt)[me]
-    start = cnt[me].cumsum(0) - cnt[me]
-    i = torch.arange(flat.numel(), device=flat.device)
-    row_sorted = base[g] + lower[g] + i - start[g]
-    dst_rank = torch.empty(flat.numel(), dtype=torch.int32, device=flat.device)
-    dst_row = torch.empty_like(dst_rank)
-    dst_rank[order] = (g // E_l).to(torch.int32)
-    dst_row[order] = row_sorted.to(torch.int32)
+    shift = base + lower - own.offs[:E]  # from a row of ``own`` to its expert's rows on the owner
+    dst_rank = (flat // E_l).to(torch.int32)
+    dst_row = (own.rows + shift[flat]).to(torch.int32)
     offs = torch.zeros(E_l + 1, dtype=torch.int64, device=flat.device)
     offs[1:] = padded[me].cumsum(0)
     total = int(offs[-1])
@@ -200,7 +199,8 @@ class PeerExpertExchange:
         return self.buf[off:off + rows * self.H * 2].view(torch.bfloat16).view(rows, self.H)
 
     def plan(self, experts: torch.Tensor, num_experts: int) -> RoutePlan:
-        cnt = torch.bincount(experts.reshape(-1), minlength=num_experts).to(torch.int32)
+        own = ops.expert_plan(experts, num_experts, align=1)
+        cnt = own.counts
         if self.n > 1:
             parts = [torch.empty_like(cnt) for _ in range(self.n)]
             dist.all_gather(parts, cnt, group=self.group)
@@ -208,7 +208,7 @@ class PeerExpertExchange:
         else:
             counts_all = cnt[None]
         # rows beyond max_rows are refused by the dispatch kernel (error word), not checked here
-        return route_plan(experts, counts_all, self.me)
+        return route_plan(experts, counts_all, self.me, own=own)
 
     def push(self, x: torch.Tensor, plan: RoutePlan, scale: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Rows x[j // k] (times scale[j]) to their owners; returns this rank's received rows."""
