@@ -8,8 +8,8 @@
 // that fills half the batch is spread over as many CTAs as any other half.
 //
 // A forward pass whose table wants a gradient sorts its tokens in the first CTAs of the lookup's own launch: the sort
-// is a chain of barriers on a few SMs that moves next to nothing, and the lookup has the others meanwhile (8192 tokens:
-// 16 us as a launch of its own).
+// is a chain of barriers on a few SMs that moves next to nothing, and the lookup has the others meanwhile (8192 tokens of
+// 2560 bf16: 16.4 us without the sort, 20.5 with it; of 8, where next to nothing is moved: 4.2 and 14.4).
 #include "row_moves.cuh"
 #include "sorted_keys.cuh"
 
@@ -76,10 +76,13 @@ struct Order {
   uint32_t *key, *pos, *seen, *scratch;  // scratch: 2 n
   int n, passes, bits, ctas;
 };
-// Few warps: with 512 bins a warp's counters cost more than its items (8192 tokens in 8 CTAs of 32 warps: 16 us).
-constexpr int kSortWarps = 8;
+// Warps of a sorting CTA.  Few are quicker while a warp's 512 counters outnumber its tokens (2048 tokens: 12 us of the
+// device with 8, 16 with 32), many for longer batches, whose lookup they also leave alone on their SMs (131072 x 2560:
+// 232 us with 8, 204 with 32, 184 for the lookup alone).
+constexpr int kFewWarps = 8, kManyWarps = 32, kFewTokens = 4096;
 constexpr int kDigit = 9;  // at most sorted::kWordBins bins a pass
 
+template <int kWarps>
 __device__ __forceinline__ void sort_tokens(const Tokens& tk, const Order& o, uint32_t* sm) {
   const uint32_t mask = (1u << o.bits) - 1;
   const int words = (tk.rows + 31) / 32;
@@ -88,10 +91,10 @@ __device__ __forceinline__ void sort_tokens(const Tokens& tk, const Order& o, ui
   auto key = [&](int p) { return ((o.passes - 1 - p) & 1) ? o.scratch : o.key; };
   auto pos = [&](int p) { return ((o.passes - 1 - p) & 1) ? o.scratch + o.n : o.pos; };
   FirstPass p0{tk, {0, mask}, key(0), pos(0), o.seen};
-  sorted::counting_pass<kSortWarps>(o.n, 1 << o.bits, 1u, sm, o.ctas, p0);
+  sorted::counting_pass<kWarps>(o.n, 1 << o.bits, 1u, sm, o.ctas, p0);
   for (int p = 1; p < o.passes; ++p) {
     NextPass q{key(p - 1), pos(p - 1), {p * o.bits, mask}, key(p), pos(p)};
-    sorted::counting_pass<kSortWarps>(o.n, 1 << o.bits, 1u, sm, o.ctas, q);
+    sorted::counting_pass<kWarps>(o.n, 1 << o.bits, 1u, sm, o.ctas, q);
   }
 }
 
@@ -148,17 +151,17 @@ __global__ void __launch_bounds__(kLookWarps * 32)
 }
 
 // The first cluster sorts, the CTAs behind it look up.
-template <class B>
-__global__ void __launch_bounds__(kSortWarps * 32)
+template <class B, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32)
     lookup_sort_kernel(Tokens tk, Order o, int64_t units, Parts pt, const typename B::T* __restrict__ w, int64_t ld,
                        bool whole, float scale, int H, typename B::T* __restrict__ out, int* err) {
   extern __shared__ uint32_t sm[];
   if ((int)blockIdx.x < o.ctas) {
-    sort_tokens(tk, o, sm);
+    sort_tokens<kWarps>(tk, o, sm);
     return;
   }
-  const int64_t warps = (int64_t)(gridDim.x - o.ctas) * kSortWarps;
-  for (int64_t u = (int64_t)(blockIdx.x - o.ctas) * kSortWarps + (threadIdx.x >> 5); u < units; u += warps)
+  const int64_t warps = (int64_t)(gridDim.x - o.ctas) * kWarps;
+  for (int64_t u = (int64_t)(blockIdx.x - o.ctas) * kWarps + (threadIdx.x >> 5); u < units; u += warps)
     look_up<B>(tk, u, pt, w, ld, whole, scale, H, out, err);
 }
 
@@ -411,10 +414,18 @@ std::vector<torch::Tensor> embedding_fwd(torch::Tensor tokens, torch::Tensor w, 
     o.pos = o.key + n;
     o.scratch = o.key + 2 * n;
     o.seen = o.key + 4 * n;
-    const int64_t look = std::min<int64_t>((units + kSortWarps - 1) / kSortWarps, 148 * 4);
-    launch_rows(lookup_sort_kernel<B>, o.ctas * (1 + (look + o.ctas - 1) / o.ctas), kSortWarps * 32,
-                sorted::pass_smem(kSortWarps, 1 << o.bits), o.ctas, false, st, tk, o, units, pt, table, w.stride(0), whole,
-                (float)scale, (int)H, to, err.data_ptr<int>());
+    auto go = [&](auto warps) {
+      constexpr int kWarps = decltype(warps)::value;
+      // four rounds of 32-warp CTAs (131072 x 2560: 204 us, with one round 235)
+      const int64_t look = std::min<int64_t>((units + kWarps - 1) / kWarps, 148 * 4);
+      launch_rows(lookup_sort_kernel<B, kWarps>, o.ctas * (1 + (look + o.ctas - 1) / o.ctas), kWarps * 32,
+                  sorted::pass_smem(kWarps, 1 << o.bits), o.ctas, false, st, tk, o, units, pt, table, w.stride(0), whole,
+                  (float)scale, (int)H, to, err.data_ptr<int>());
+    };
+    if (n <= kFewTokens)
+      go(std::integral_constant<int, kFewWarps>());
+    else
+      go(std::integral_constant<int, kManyWarps>());
   });
   return {out, order};
 }

@@ -14,7 +14,7 @@ namespace sorted {
 constexpr int kMaxBins = 1024, kMaxCtas = 16;
 
 // Bins up to which a warp's lanes find their equals through words in shared memory: each sets its bit in its bin's word.
-// (8192 items, 512 bins: about 1 us for a CTA, with __match_any_sync 8.6 us, which takes a step for every distinct key.)
+// (131072 pairs by 128 experts: 11.4 us; with __match_any_sync, which takes a step for every distinct key, 15.9.)
 constexpr int kWordBins = 512;
 
 inline size_t pass_smem(int warps, int bins) {
