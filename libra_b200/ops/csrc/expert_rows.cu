@@ -331,9 +331,10 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, int64_t> expert_plan(tor
              "%lld", sorted::kMaxBins, (long long)E, (long long)align);
   ids = ids.contiguous();
   const int64_t n = ids.numel();
-  ROWS_CHECK(n < (1ll << 31) && align < (1ll << 31) && n + (align - 1) * std::min(E, n) < (1ll << 31),
+  // no pairs still leave one group's rows, so that the grouped products have something to stand on
+  const int64_t cap = n == 0 && align > 1 ? align : n + (align - 1) * std::min(E, n);
+  ROWS_CHECK(n < (1ll << 31) && align < (1ll << 31) && cap < (1ll << 31),
              "expert_plan: %lld pairs with align %lld do not fit 31 bits", (long long)n, (long long)align);
-  const int64_t cap = n + (align - 1) * std::min(E, n);
   LIBRA_CHECK(err.device() == ids.device() && err.scalar_type() == at::kInt, "expert_plan: error word");
   const c10::cuda::CUDAGuard guard(ids.device());
   const auto i32 = ids.options().dtype(at::kInt);
@@ -599,7 +600,7 @@ static std::vector<torch::Tensor> combine_bwd(torch::Tensor g, torch::Tensor y, 
   g = unit_inner(g);
   y = unit_inner(y);
   torch::Tensor dy, dw;
-  if (want_y) dy = torch::empty({cap, H}, y.options());
+  if (want_y) dy = pairs == 0 ? torch::zeros({cap, H}, y.options()) : torch::empty({cap, H}, y.options());
   if (want_w) dw = H == 0 ? torch::zeros_like(w) : torch::empty_like(w);
   if (H == 0 || pairs == 0) return {dy, dw};
   const int clear = want_y ? clear_ctas(pl) : 0;

@@ -225,7 +225,7 @@ def embedding(tokens, w, scale, first, whole):
         raise ValueError("embedding: a token lies outside the table")
     out = w.index_select(0, r.clamp(0, max(w.shape[0] - 1, 0))) if w.shape[0] else w.new_zeros(r.numel(), w.shape[1])
     if scale != 1.0:
-        out = (out.float() * scale).to(w.dtype)
+        out = (out.to(torch.promote_types(w.dtype, torch.float32)) * scale).to(w.dtype)
     if not whole:
         out = out.masked_fill(~here.unsqueeze(1), 0)
     return out.view(*tokens.shape, w.shape[1])
@@ -235,7 +235,7 @@ def embedding_grad(tokens, g, rows, scale, first, main):
     """Adds scale * sum of g over each token's positions to ``main``, or returns it as [rows, H] of g's type."""
     r = tokens.reshape(-1).long() - first
     here = (r >= 0) & (r < rows)
-    g = g.float()
+    g = g.to(torch.float32 if main is not None else torch.promote_types(g.dtype, torch.float32))
     if not bool(here.all()):
         g, r = g[here], r[here]
     if scale != 1.0:
@@ -243,7 +243,7 @@ def embedding_grad(tokens, g, rows, scale, first, main):
     if main is not None:
         main.view(rows, -1).index_add_(0, r, g)
         return None
-    return torch.zeros(rows, g.shape[1]).index_add_(0, r, g)
+    return torch.zeros(rows, g.shape[1], dtype=g.dtype).index_add_(0, r, g)
 
 
 def route_topk(logits, k, normalize):
@@ -278,8 +278,9 @@ def expert_plan(experts, num_experts, align):
 
 def moe_dispatch(x, rows, k, capacity):
     to = torch.where(rows >= 0, rows, capacity).long()
-    out = x.new_zeros(capacity + 1, x.shape[1], dtype=torch.float32)
-    return out.index_copy(0, to, x.float().repeat_interleave(k, dim=0))[:capacity].to(x.dtype)
+    v = x.to(torch.promote_types(x.dtype, torch.float32))  # the gradient's sums too
+    out = v.new_zeros(capacity + 1, x.shape[1])
+    return out.index_copy(0, to, v.repeat_interleave(k, dim=0))[:capacity].to(x.dtype)
 
 
 def moe_combine(y, weights, rows, k, residual):

@@ -3,8 +3,8 @@ summed by sorted tokens, and a mixture-of-experts layer's router, plan, dispatch
 and combine.
 
 They dispatch like the other operators of :mod:`libra_b200.ops`: CUDA tensors
-run the kernels of ``embedding.cu`` and ``expert_rows.cu``; CPU tensors run
-:mod:`libra_b200.ops.reference`.  The same inputs give the same bits.
+run the kernels of ``embedding.cu`` and ``expert_rows.cu`` (bf16 and fp32); CPU
+tensors run :mod:`libra_b200.ops.reference`, whatever floats they hold.  The same inputs give the same bits.
 """
 
 from __future__ import annotations
@@ -20,8 +20,6 @@ import libra_b200.ops as _lib
 from . import reference as ref
 
 MAX_EXPERTS = 1024  # of route_topk and expert_plan
-
-_ROW_TYPES = (torch.bfloat16, torch.float32)
 
 
 # ---------------------------------------------------------------------------
@@ -69,8 +67,8 @@ class _EmbeddingCPU(torch.autograd.Function):
 
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
               vocab_start: Optional[int] = None) -> torch.Tensor:
-    """``scale * weight[tokens]``, of the weight's type (bf16 or fp32) with one
-    rounding: tokens int64 or int32 of any shape, weight [V, H], result
+    """``scale * weight[tokens]``, of the weight's type (bf16 or fp32; any floats
+    on the CPU) with one rounding: tokens int64 or int32 of any shape, weight [V, H], result
     [*tokens.shape, H].
 
     With ``vocab_start`` the weight is a shard that begins at that token:
@@ -84,8 +82,8 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     first, whole = (0, True) if vocab_start is None else (int(vocab_start), False)
     if weight.is_cuda:
         return _lib.ext().embedding(tokens, weight, scale, first, whole, _lib.error_flag(weight.device))
-    if weight.dim() != 2 or weight.dtype not in _ROW_TYPES:
-        raise ValueError(f"embedding: weight must be [V, H], bf16 or fp32, got {tuple(weight.shape)} {weight.dtype}")
+    if weight.dim() != 2 or not weight.is_floating_point():
+        raise ValueError(f"embedding: weight must be [V, H] of floats, got {tuple(weight.shape)} {weight.dtype}")
     if tokens.dtype not in (torch.int64, torch.int32) or tokens.device != weight.device:
         raise ValueError(f"embedding: tokens must be int64 or int32 on {weight.device}, got {tokens.dtype} on "
                          f"{tokens.device}")
@@ -110,8 +108,8 @@ def route_topk(logits: torch.Tensor, k: int, *, normalize: bool = True) -> Tuple
     if logits.is_cuda:
         return _lib.ext().route_topk(logits, k, normalize)
     k = int(k)
-    if logits.dim() != 2 or logits.dtype not in _ROW_TYPES:
-        raise ValueError(f"route_topk: logits must be [T, E], bf16 or fp32, got {tuple(logits.shape)} {logits.dtype}")
+    if logits.dim() != 2 or not logits.is_floating_point():
+        raise ValueError(f"route_topk: logits must be [T, E] of floats, got {tuple(logits.shape)} {logits.dtype}")
     E = logits.shape[1]
     if not 1 <= E <= MAX_EXPERTS or not 1 <= k <= E:
         raise ValueError(f"route_topk: 1 to {MAX_EXPERTS} experts and k in [1, {E}], got {E} and {k}")
@@ -156,14 +154,16 @@ def expert_plan(experts: torch.Tensor, num_experts: int, *, align: int = 128) ->
         raise ValueError(f"expert_plan: 1 to {MAX_EXPERTS} experts and align >= 1, got {num_experts} and {align}")
     T, k = experts.shape
     capacity = T * k + (align - 1) * min(num_experts, T * k)
+    if capacity == 0 and align > 1:
+        capacity = align  # no pairs still leave one group's rows: the grouped products take no empty tensor
     if capacity >= 2 ** 31:
         raise ValueError(f"expert_plan: {capacity} rows do not fit 31 bits")
     return ExpertPlan(*ref.expert_plan(experts, num_experts, align), T, k, align, capacity)
 
 
 def _check_rows(op: str, what: str, x: torch.Tensor, plan: ExpertPlan, count: int) -> None:
-    if x.dim() != 2 or x.dtype not in _ROW_TYPES or x.shape[0] != count:
-        raise ValueError(f"{op}: {what} must be [{count}, H], bf16 or fp32, got {tuple(x.shape)} {x.dtype}")
+    if x.dim() != 2 or not x.is_floating_point() or x.shape[0] != count:
+        raise ValueError(f"{op}: {what} must be [{count}, H] of floats, got {tuple(x.shape)} {x.dtype}")
     if x.device != plan.rows.device:
         raise ValueError(f"{op}: {what} on {x.device}, the plan on {plan.rows.device}")
 
