@@ -4,7 +4,8 @@ and combine.
 
 They dispatch like the other operators of :mod:`libra_b200.ops`: CUDA tensors
 run the kernels of ``embedding.cu`` and ``expert_rows.cu`` (bf16 and fp32); CPU
-tensors run :mod:`libra_b200.ops.reference`, whatever floats they hold.  The same inputs give the same bits.
+tensors run :mod:`libra_b200.ops.reference`, whatever floats they hold.  The same
+inputs give the same bits.
 """
 
 from __future__ import annotations
@@ -68,8 +69,8 @@ class _EmbeddingCPU(torch.autograd.Function):
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
               vocab_start: Optional[int] = None) -> torch.Tensor:
     """``scale * weight[tokens]``, of the weight's type (bf16 or fp32; any floats
-    on the CPU) with one rounding: tokens int64 or int32 of any shape, weight [V, H], result
-    [*tokens.shape, H].
+    on the CPU) with one rounding: tokens int64 or int32 of any shape, weight
+    [V, H], result [*tokens.shape, H].
 
     With ``vocab_start`` the weight is a shard that begins at that token:
     tokens outside it give rows of zeros and no gradient.  Without it they are
@@ -77,8 +78,10 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     raises (ValueError on the CPU).
 
     Differentiable with respect to the weight.  The gradient sums each token's
-    rows in fp32 in a fixed order, so that it does not change from run to run.  It is added to ``weight.main_grad``
-    (fp32) when there is one, else it is a dense tensor like the weight."""
+    rows in fp32 in a fixed order, so that it does not change from run to run.
+    It is added to ``weight.main_grad`` (contiguous fp32) when there is one, else
+    it is a dense tensor like the weight.  Until the backward pass the tokens'
+    order is kept, 16 bytes a token."""
     first, whole = (0, True) if vocab_start is None else (int(vocab_start), False)
     if weight.is_cuda:
         return _lib.ext().embedding(tokens, weight, scale, first, whole, _lib.error_flag(weight.device))

@@ -119,6 +119,30 @@ def test_embedding_shards_add_up_and_leave_other_tokens_out(device):
     _check(device)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_vocab_parallel_embedding_of_one_rank_at_a_time(device):
+    """The tensor-parallel lookup on each rank's shard, without the reduction: partial rows and the shards' gradients."""
+    from libra_b200.parallel.tensor_parallel import vocab_parallel_embedding
+
+    gen = _gen(14)
+    tokens = _tokens(130, 64, gen, "few")
+    w, g = torch.randn(64, 24, generator=gen).bfloat16(), torch.randn(130, 24, generator=gen).bfloat16()
+    total, size, many = oracle.embedding_grad(tokens, g, 64, 1.0)
+    whole = 0
+    for rank in range(4):
+        shard = w[16 * rank:16 * (rank + 1)].clone().to(device).requires_grad_(True)
+        shard.main_grad = torch.zeros(16, 24, device=device) if rank % 2 else None
+        out = vocab_parallel_embedding(tokens.to(device), shard, None, rank, reduce=False)
+        out.backward(g.to(device))
+        rows = slice(16 * rank, 16 * (rank + 1))
+        got = shard.main_grad if rank % 2 else shard.grad
+        _close(got, total[rows], size[rows] * (many[rows] + 1) * U * 1.01
+               + (0 if rank % 2 else total[rows].abs() * _half(torch.bfloat16) * 1.01))
+        whole = whole + out.detach()
+    _close(whole, oracle.embedding(tokens, w, 1.0), 0.0)
+    _check(device)
+
+
 def test_embedding_refusals_on_the_cpu():
     w = torch.zeros(4, 8)
     for bad in (-1, 4):
